@@ -652,6 +652,94 @@ int scope_decoder_step(const scope_decoder_step_params* p, const scope_decoder_l
  * reference, which has no decode loop. */
 int scope_argmax_f32(const float* x, int64_t n, int64_t* out, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The paged cache of a decode loop over several sequences.  No reference
+ * counterpart (the reference has no decode path).
+ *   k_pages, v_pages  [P][Hkv][bs][D], element strides (page, head, row), d
+ *                     stride 1, rows 16-byte aligned; 16-bit values of `type`,
+ *                     or e4m3 bytes (fp8 != 0) that stand for byte · scale[h]
+ *                     (k_scale, v_scale [Hkv] fp32; NULL: 1)
+ *   table [B][MP]     int32 page of each block of bs positions; an entry
+ *                     outside [0, P) is a block without a page
+ *   lens [B]          int32 positions of each sequence; kept to [0, MP·bs]
+ * D in {64, 128, 256}, bs in {16, 32, 64, 128, 256}, MP·bs < 2^31.
+ * ---------------------------------------------------------------------- */
+enum { SCOPE_BF16 = 0, SCOPE_FP16 = 1, SCOPE_FP32 = 2 };
+typedef struct {
+  int B, Hkv, D, bs, MP;
+  int type; /* SCOPE_BF16 or SCOPE_FP16: q, k, v and out, and the pages unless fp8 */
+  int fp8;  /* the pages hold e4m3 */
+  int64_t P;
+  int64_t k_sp, k_sh, k_sr, v_sp, v_sh, v_sr;
+} scope_paged_cache;
+
+/* N rows of k and v ([N][Hkv][D], strides (row, head)) into the pages: row i
+ * belongs to the sequence b with cu[b] <= i < cu[b + 1] (cu [B + 1], not
+ * decreasing; NULL: sequence i) and goes to position lens[b] + i - cu[b].  A
+ * row of no sequence, past the table or of a block without a page is not
+ * written; two rows for the same slot of the same page leave either.  e4m3:
+ * x / scale[h], cut to +-448, rounded to nearest even. */
+int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k, int64_t k_sn, int64_t k_sh,
+                       const uint16_t* v, int64_t v_sn, int64_t v_sh, const int32_t* cu, const int32_t* table,
+                       const int32_t* lens, const float* k_scale, const float* v_scale, void* k_pages, void* v_pages,
+                       void* stream);
+
+/* The attention of one new token per sequence: q [B][Hq][D] (strides q_sb,
+ * q_sh; Hq a multiple of Hkv, query head h reads key head h / (Hq / Hkv)).
+ * Position j is seen where first[b] <= j < lens[b] (first NULL: 0), its block
+ * has a page and, with lists, j / bs is among kv_idx [B][Hkv][maxkv] up to
+ * kv_num [B][Hkv] (entries outside [0, MP) are skipped, kv_num is kept to
+ * [0, maxkv]; an entry listed twice counts twice).
+ *   out [B][Hq][D]     softmax(scale · q·k) · v; zeros where nothing is seen
+ *   lse [B][Hq]        natural logarithm of the sum; -inf there
+ *   mass [B][Hkv][MP]  or NULL: each block's probabilities, summed over its
+ *                      positions and the group's query heads, are added (lists
+ *                      without repeats; two calls on one mass at a time race) */
+int64_t scope_paged_attn_workspace_bytes(const scope_paged_cache* c, int Hq, int maxkv, int with_mass);
+int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float scale, const uint16_t* q, int64_t q_sb,
+                            int64_t q_sh, const void* k_pages, const void* v_pages, const float* k_scale,
+                            const float* v_scale, const int32_t* table, const int32_t* lens, const int32_t* first,
+                            const int32_t* kv_num, const int32_t* kv_idx, float* mass, void* work, uint16_t* out,
+                            float* lse, void* stream);
+
+/* Takes the pages of least accumulated weight out of the table.  Of sequence
+ * b's n = ceil(lens[b] / bs) blocks those with a table entry >= 0 are held;
+ * the first n_global blocks and the last `window` (at least 1) stay.  Where
+ * more than budget[b] are held, the surplus goes: the blocks of least
+ * Σ_h mass[b][h][i] (summed in fp64, compared in fp32; NaN above everything;
+ * the lower index on ties), all that may go where they do not suffice.
+ *   table_out [B][MP]  the table with -1 in their place (may be table)
+ *   freed [B][MP]      their pages in the blocks' order, then -1
+ *   n_freed [B]        how many */
+#define SCOPE_PAGED_EVICT_MAX_PAGES 65536
+int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, const int32_t* table, const float* mass,
+                      const int32_t* lens, const int32_t* budget, int32_t* table_out, int32_t* freed, int32_t* n_freed,
+                      void* stream);
+
+/* Penalties, biases and grammar bits on logits [B][V] (row stride z_sb; fp32,
+ * bf16 or fp16; out alike with o_sb, may be logits).  History of row b:
+ * tokens[b][first[b] .. min(lens[b], T)) (row stride tok_sb, 0 for one history;
+ * first NULL: 0; tokens outside [0, V) are passed over); seen(v): v occurs in
+ * it; c(v): how often at positions >= n_prompt[b] (NULL: 0).  In fp32, one
+ * rounding a step, the result rounded once to the logits' type:
+ *   seen: z > 0 ? z / repetition : z · repetition;  c > 0: z - frequency · c,
+ *   then z - presence;  z + bias[b][v] (row stride bias_sb, 0 for one row);
+ *   z / temperature;  -inf where bit v % 32 of mask[b][v / 32] (row stride
+ *   mask_sb) is 0.
+ * repetition, presence, frequency and temperature are [B] arrays, or NULL for
+ * the parameters' numbers; repetition and temperature are positive. */
+typedef struct {
+  int B, type, tokens64, lens64; /* 64: int64, else int32 */
+  int64_t V, T;
+  int64_t z_sb, o_sb, tok_sb, bias_sb, mask_sb;
+  float repetition, presence, frequency, temperature;
+} scope_penalty_params;
+
+int scope_logit_penalties(const scope_penalty_params* p, const void* logits, const void* tokens, const void* lens,
+                          const int32_t* first, const int32_t* n_prompt, const float* repetition, const float* presence,
+                          const float* frequency, const float* temperature, const float* bias, const int32_t* mask,
+                          void* out, void* stream);
+
 int64_t scope_attn_bwd_workspace_bytes(const scope_attn_params* p);
 int scope_attn_bwd(const scope_attn_params* p, const uint16_t* q, const uint16_t* k,
                    const uint16_t* v, const uint16_t* out, const uint16_t* dout, const float* lse,

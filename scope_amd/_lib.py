@@ -93,6 +93,18 @@ class DecoderStepParams(C.Structure):
                 ("v_sh", c_int64), ("v_st", c_int64), ("spin_ticks", c_uint64), ("gang_ticks", c_uint64)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("B", c_int), ("Hkv", c_int), ("D", c_int), ("bs", c_int), ("MP", c_int), ("type", c_int),
+                ("fp8", c_int), ("P", c_int64), ("k_sp", c_int64), ("k_sh", c_int64), ("k_sr", c_int64),
+                ("v_sp", c_int64), ("v_sh", c_int64), ("v_sr", c_int64)]
+
+
+class PenaltyParams(C.Structure):
+    _fields_ = [("B", c_int), ("type", c_int), ("tokens64", c_int), ("lens64", c_int), ("V", c_int64), ("T", c_int64),
+                ("z_sb", c_int64), ("o_sb", c_int64), ("tok_sb", c_int64), ("bias_sb", c_int64), ("mask_sb", c_int64),
+                ("repetition", c_float), ("presence", c_float), ("frequency", c_float), ("temperature", c_float)]
+
+
 P = c_void_p
 _PROTOS = {
     "scope_abi_version": (c_int, []),
@@ -150,6 +162,11 @@ _PROTOS = {
                                           c_int64, P, P, P, P, P, P, P, P, P, P]),
     "scope_decoder_step_prologue": (c_int, [P, P, c_int64, c_int64, c_int, c_float, c_int64, P, P, P, P, P, P, P, P,
                                             P]),
+    "scope_paged_append": (c_int, [C.POINTER(PagedCache), c_int64, P, c_int64, c_int64, P, c_int64, c_int64] + [P] * 8),
+    "scope_paged_attn_workspace_bytes": (c_int64, [C.POINTER(PagedCache), c_int, c_int, c_int]),
+    "scope_paged_decode_attn": (c_int, [C.POINTER(PagedCache), c_int, c_int, c_float, P, c_int64, c_int64] + [P] * 14),
+    "scope_paged_evict": (c_int, [c_int] * 6 + [P] * 8),
+    "scope_logit_penalties": (c_int, [C.POINTER(PenaltyParams)] + [P] * 13),
     "scope_attn_bwd": (c_int, [C.POINTER(AttnParams)] + [P] * 30),
     "scope_attn_bwd_phase": (c_int, [C.POINTER(AttnParams), c_int] + [P] * 30),
     "scope_probe_mfma_flops": (c_int64, [c_int, c_int]),

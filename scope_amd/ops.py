@@ -6,6 +6,7 @@ GPU tensors; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import threading
 
 import torch
@@ -1102,6 +1103,235 @@ def decoder_step(prm, table: torch.Tensor, work: torch.Tensor, tok: torch.Tensor
     call("scope_decoder_step", C.byref(prm), _p(table), _p(tok), _p(t_dev), _p(tokens), _p(docs), _p(embed),
          *(_p(v) for v in tabs), _p(cos), _p(sin), _p(x), _p(work), _p(host_status), _stream(dev))
     return x
+
+
+# ---- the paged cache of a decode loop over several sequences --------------------
+_PAGED_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_FP8 = torch.float8_e4m3fn
+EVICT_MAX_PAGES = 65536  # include/scope_amd.h SCOPE_PAGED_EVICT_MAX_PAGES
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """``call`` with ``dev`` as the current device (a launch takes the current
+    device's kernels, whatever device its stream is on)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args)
+
+
+def _ints(who: str, name: str, x, n: int, dev: torch.device) -> torch.Tensor | None:
+    """n int32 numbers on dev: of an integer tensor of n elements, or one number for all."""
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor):
+        return torch.full((n,), int(x), dtype=torch.int32, device=dev)
+    if x.numel() != n or x.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{who}: {name} must be int32 or int64 [{n}] (got {x.dtype} {tuple(x.shape)})")
+    return _i32(x)
+
+
+def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, dtype: torch.dtype,
+                 k_scale, v_scale) -> "_lib.PagedCache":
+    """The C description of a cache, its tensors checked."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise RuntimeError(f"{who}: k_pages and v_pages must be [P, Hkv, bs, D] of one shape and type")
+    fp8 = k_pages.dtype == _FP8
+    if dtype not in (torch.bfloat16, torch.float16) or not (fp8 or k_pages.dtype == dtype):
+        raise RuntimeError(f"{who}: bfloat16 or float16 rows with pages of their type or float8_e4m3fn "
+                           f"(got {dtype} and {k_pages.dtype})")
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP]")
+    P, Hkv, bs, D = k_pages.shape
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is not None and (not fp8 or t.dtype != torch.float32 or t.numel() != Hkv or not t.is_contiguous()):
+            raise RuntimeError(f"{who}: {name} must be a contiguous float32 [{Hkv}], with float8_e4m3fn pages")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise RuntimeError(f"{who}: the pages' last dimension must be contiguous")
+    B, MP = table.shape
+    return _lib.PagedCache(B, Hkv, D, bs, MP, _PAGED_TYPES[dtype], int(fp8), P, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                 lens: torch.Tensor, *, cu: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None) -> None:
+    """Writes the rows of new tokens into a paged cache, in place.
+
+    k, v [N, Hkv, D] bf16 or fp16 (any row and head strides, rows 16-byte
+    aligned); k_pages, v_pages [P, Hkv, bs, D] of the same type, or
+    float8_e4m3fn holding x / scale[h] cut to ±448 (k_scale, v_scale [Hkv]
+    fp32); table [B, MP] int32 page ids; lens [B] the positions each sequence
+    holds before the call (it is not changed).  Row i goes to sequence b with
+    cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing; without it N <= B
+    and row i to sequence i), position lens[b] + i - cu[b].  Rows of no
+    sequence, past the table, or of a block whose entry is outside [0, P) are
+    not written; no two rows may share a slot."""
+    who = "paged_append"
+    dev = _gpu(who, k, v, k_pages, v_pages, table, lens, cu, k_scale, v_scale)
+    c = _paged_cache(who, k_pages, v_pages, table, k.dtype, k_scale, v_scale)
+    if k.dim() != 3 or k.shape != v.shape or v.dtype != k.dtype or k.shape[1] != c.Hkv or k.shape[2] != c.D \
+            or k.stride(2) != 1 or v.stride(2) != 1:
+        raise RuntimeError(f"{who}: k and v must be [N, {c.Hkv}, {c.D}] of one type with a contiguous last dimension")
+    for n_, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            raise RuntimeError(f"{who}: {n_} is an expanded tensor: its rows share memory")
+    lens = _ints(who, "lens", lens, c.B, dev)
+    cu = _ints(who, "cu", cu, c.B + 1, dev)
+    _call_on(dev, "scope_paged_append", C.byref(c), k.shape[0], _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
+             v.stride(1), _p(cu), _p(table), _p(lens), _p(k_scale), _p(v_scale), _p(k_pages), _p(v_pages), _stream(dev))
+
+
+def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                      lens: torch.Tensor, *, scale: float, first: torch.Tensor | None = None,
+                      kv_num: torch.Tensor | None = None, kv_idx: torch.Tensor | None = None,
+                      mass: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                      v_scale: torch.Tensor | None = None):
+    """The attention of one new token per sequence over a paged cache ->
+    (out [B, Hq, D] of q's type, lse [B, Hq] fp32).
+
+    q [B, Hq, D] bf16 or fp16, Hq a multiple of Hkv (query head h reads key
+    head h // (Hq // Hkv)); the cache as ``paged_append`` fills it, lens [B]
+    the positions each sequence holds, the new token's among them.  A position
+    is seen from ``first`` [B] on (a document's start, a window's edge), where
+    its block has a page, and with lists where its block is among kv_idx [B,
+    Hkv, maxkv] up to kv_num [B, Hkv] (blocks of bs positions; those outside
+    the table are skipped).  A row that sees nothing gives 0 and lse -inf.
+    ``mass`` [B, Hkv, MP] fp32 contiguous gets each block's probabilities,
+    summed over its positions and the group's query heads, added in place
+    (lists without repeats then; not two calls on one mass at a time).
+    Nothing of it waits for the GPU or reads a length on the host, so a call
+    can be captured and replayed while the lengths and the table change."""
+    who = "paged_decode_attn"
+    dev = _gpu(who, q, k_pages, v_pages, table, lens, first, kv_num, kv_idx, mass, k_scale, v_scale)
+    c = _paged_cache(who, k_pages, v_pages, table, q.dtype, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[0] != c.B or q.shape[2] != c.D or q.shape[1] % c.Hkv or q.shape[1] < 1 or q.stride(2) != 1:
+        raise RuntimeError(f"{who}: q must be [{c.B}, a multiple of {c.Hkv}, {c.D}] with a contiguous last dimension "
+                           f"(got {tuple(q.shape)})")
+    B, Hq, D = q.shape
+    maxkv = 0
+    if (kv_num is None) != (kv_idx is None):
+        raise RuntimeError(f"{who}: kv_num and kv_idx come together")
+    if kv_idx is not None:
+        maxkv = kv_idx.shape[-1]
+        if kv_idx.dim() != 3 or maxkv < 1 or kv_idx.shape[:2] != (B, c.Hkv) or kv_num.shape != (B, c.Hkv):
+            raise RuntimeError(f"{who}: kv_num must be [{B}, {c.Hkv}] and kv_idx [{B}, {c.Hkv}, maxkv]")
+        kv_num, kv_idx = _i32(kv_num), _i32(kv_idx)
+    if mass is not None and (mass.dtype != torch.float32 or mass.shape != (B, c.Hkv, c.MP) or not mass.is_contiguous()):
+        raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, {c.Hkv}, {c.MP}]")
+    lens = _ints(who, "lens", lens, B, dev)
+    first = _ints(who, "first", first, B, dev)
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+    need = query("scope_paged_attn_workspace_bytes", C.byref(c), Hq, maxkv, int(mass is not None))
+    work = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), _p(q), q.stride(0), q.stride(1),
+             _p(k_pages), _p(v_pages), _p(k_scale), _p(v_scale), _p(table), _p(lens), _p(first), _p(kv_num), _p(kv_idx),
+             _p(mass), _p(work), _p(out), _p(lse), _stream(dev))
+    return out, lse
+
+
+def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, budget, *, bs: int, window: int = 1,
+                n_global: int = 0, out: torch.Tensor | None = None):
+    """Takes the blocks of least accumulated attention weight out of a page
+    table -> (table [B, MP], freed [B, MP], n_freed [B]), all int32.
+
+    Of sequence b's ceil(lens[b] / bs) blocks those with a table entry >= 0
+    are held.  Where more than budget[b] (a tensor [B] or one number) are, the
+    surplus goes: the blocks of least Σ_h mass[b, h, i] (mass [B, Hkv, MP]
+    fp32; summed in 64 bits, compared in 32; NaN above everything, the lower
+    index on ties), except the first ``n_global`` blocks and the last
+    ``window`` ones; all the others where they do not suffice.  The returned
+    table has -1 in their place (a new tensor, or ``out``, which may be the
+    table itself); freed holds their pages in the blocks' order, then -1."""
+    who = "paged_evict"
+    dev = _gpu(who, table, mass, lens, budget if isinstance(budget, torch.Tensor) else None, out)
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP]")
+    B, MP = table.shape
+    if mass.dtype != torch.float32 or mass.dim() != 3 or mass.shape[0] != B or mass.shape[2] != MP or not mass.is_contiguous():
+        raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, Hkv, {MP}]")
+    if out is None:
+        out = torch.empty_like(table)
+    elif out.dtype != torch.int32 or out.shape != table.shape or not out.is_contiguous():
+        raise RuntimeError(f"{who}: out must be a contiguous int32 [{B}, {MP}]")
+    lens = _ints(who, "lens", lens, B, dev)
+    budget = _ints(who, "budget", budget, B, dev)
+    freed = torch.empty((B, MP), dtype=torch.int32, device=dev)
+    n_freed = torch.empty(B, dtype=torch.int32, device=dev)
+    _call_on(dev, "scope_paged_evict", B, mass.shape[1], MP, int(bs), int(window), int(n_global), _p(table), _p(mass),
+             _p(lens), _p(budget), _p(out), _p(freed), _p(n_freed), _stream(dev))
+    return out, freed, n_freed
+
+
+def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=None, n_prompt=None, repetition=1.0,
+                    presence=0.0, frequency=0.0, temperature=1.0, bias: torch.Tensor | None = None,
+                    mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties for repeated tokens, a bias and grammar bits on the logits of
+    one step, [B, V] or [V] in fp32, bf16 or fp16 -> the same shape and type.
+
+    The history of row b is tokens[b, first[b] : lens[b]] (tokens [B, T], or
+    [T] for all rows, int32 or int64; lens and first [B] or one number); a word
+    in it was seen, and c counts its occurrences at positions from
+    n_prompt[b] on.  In this order, in fp32, rounded once at the end:
+
+        z = z / repetition if z > 0 else z * repetition     (seen words)
+        z = z - frequency * c, then z - presence            (words with c > 0)
+        z = z + bias[v]                                     (bias [V] or [B, V] fp32)
+        z = z / temperature
+        z = -inf                                            (words whose bit is 0)
+
+    ``mask`` [W] or [B, W] int32 holds word v's bit at v % 32 of entry v // 32.
+    repetition, presence, frequency and temperature are numbers or fp32 [B];
+    repetition and temperature must be positive (numbers are checked).
+    ``out`` may be the logits themselves."""
+    who = "logit_penalties"
+    dev = _gpu(who, logits, tokens, bias, mask, out,
+               *(x for x in (lens, first, n_prompt, repetition, presence, frequency, temperature) if isinstance(x, torch.Tensor)))
+    if logits.dtype not in _PAGED_TYPES or logits.dim() not in (1, 2) or logits.stride(-1) != 1 or logits.numel() < 1:
+        raise RuntimeError(f"{who}: logits must be fp32, bf16 or fp16 [B, V] or [V] with contiguous rows")
+    V = logits.shape[-1]
+    B = logits.shape[0] if logits.dim() == 2 else 1
+
+    def row_stride(x):
+        return x.stride(0) if x.dim() == 2 else 0
+
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() not in (1, 2) \
+            or (tokens.dim() == 2 and tokens.shape[0] != B) or (tokens.shape[-1] > 1 and tokens.stride(-1) != 1):
+        raise RuntimeError(f"{who}: tokens must be int32 or int64 [{B}, T] or [T] with contiguous rows")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)) or bias.stride(-1) != 1):
+        raise RuntimeError(f"{who}: bias must be float32 [{V}] or [{B}, {V}] with contiguous rows")
+    W = (V + 31) // 32
+    if mask is not None and (mask.dtype != torch.int32 or mask.shape not in ((W,), (B, W)) or mask.stride(-1) != 1):
+        raise RuntimeError(f"{who}: mask must be int32 [{W}] or [{B}, {W}] with contiguous rows")
+    if out is None:
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    elif out.dtype != logits.dtype or out.shape != logits.shape or out.stride(-1) != 1 or (B > 1 and out.stride(0) < V) \
+            or (out.data_ptr() == logits.data_ptr() and B > 1 and out.stride(0) != logits.stride(0)):
+        raise RuntimeError(f"{who}: out must have the logits' shape and type, rows of its own, and their strides if it is them")
+    num, arr = {}, {}
+    for name, x, positive in (("repetition", repetition, True), ("presence", presence, False),
+                              ("frequency", frequency, False), ("temperature", temperature, True)):
+        if isinstance(x, torch.Tensor):
+            if x.numel() != B or not x.is_floating_point():
+                raise RuntimeError(f"{who}: {name} must be a number or a float tensor [{B}]")
+            num[name], arr[name] = 0.0, _f32(x)
+        else:
+            if not math.isfinite(x) or (positive and x <= 0):
+                raise ValueError(f"{who}: {name} must be finite{' and positive' if positive else ''}, got {x}")
+            num[name], arr[name] = float(x), None
+    if isinstance(lens, torch.Tensor) and lens.dtype == torch.int64 and lens.numel() == B and lens.is_contiguous():
+        lens64 = 1
+    else:
+        lens, lens64 = _ints(who, "lens", lens, B, dev), 0
+    first, n_prompt = _ints(who, "first", first, B, dev), _ints(who, "n_prompt", n_prompt, B, dev)
+    prm = _lib.PenaltyParams(B, _PAGED_TYPES[logits.dtype], int(tokens.dtype == torch.int64), lens64, V, tokens.shape[-1],
+                             row_stride(logits), row_stride(out), row_stride(tokens),
+                             row_stride(bias) if bias is not None else 0, row_stride(mask) if mask is not None else 0, **num)
+    _call_on(dev, "scope_logit_penalties", C.byref(prm), _p(logits), _p(tokens), _p(lens), _p(first), _p(n_prompt),
+             *(_p(x) for x in arr.values()), _p(bias), _p(mask), _p(out), _stream(dev))
+    return out
 
 
 def attn_bwd(q, k, v, out, dout, lse, kv_num, kv_idx, q_off, q_list, docs, ds_tok_end, *, bs: int, scale: float,
