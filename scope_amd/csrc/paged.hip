@@ -8,30 +8,20 @@
 // evicted): nothing is written to it and no key of it is seen.
 #include <math.h>
 
-#include "common.h"
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.h"
+#include "paged_plan.h"
 
 namespace scope {
 
 namespace {
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
 __device__ __forceinline__ float half_to_f32(uint16_t h) { return static_cast<float>(__builtin_bit_cast(_Float16, h)); }
 __device__ __forceinline__ uint16_t f32_to_half(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
 
-// positions that sequence b holds: its length cut to the table's, the first one seen
-__device__ __forceinline__ int64_t seq_end(const scope_paged_cache& c, const int32_t* lens, int b) {
-  const int64_t n = lens[b], cap = static_cast<int64_t>(c.MP) * c.bs;
-  return n < 0 ? 0 : n < cap ? n : cap;
-}
-
-// two floats from two e4m3 bytes (the low two, or the high two, of w)
-template <bool HI>
-__device__ __forceinline__ float2 e4m3x2(uint32_t w) {
-  typedef float f32x2_t __attribute__((ext_vector_type(2)));
-  const f32x2_t f = __builtin_amdgcn_cvt_pk_f32_fp8(w, HI);
-  return make_float2(f[0], f[1]);
-}
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 }  // namespace
 
 // ---- append ------------------------------------------------------------------
@@ -63,22 +53,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(scope_paged_cache c, 
   const int lane = threadIdx.x & 63;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (i >= a.N) return;
-  int b = static_cast<int>(i);
-  int64_t pos = 0;
-  if (a.cu) {
-    int lo = 0, hi = c.B;  // the last b in [0, B) with cu[b] <= i
-    while (lo + 1 < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= i) lo = mid; else hi = mid;
-    }
-    b = lo;
-    if (i < a.cu[b] || i >= a.cu[b + 1]) return;  // a row of no sequence
-    pos = i - a.cu[b];
-  }
-  pos += a.lens[b];
-  if (pos < 0 || pos >= static_cast<int64_t>(c.MP) * c.bs) return;
-  const int64_t page = a.table[static_cast<int64_t>(b) * c.MP + pos / c.bs];
-  if (page < 0 || page >= c.P) return;
+  int b;
+  const int64_t pos = row_position(a.cu, a.lens, c.B, i, &b);
+  if (pos < 0) return;
+  const int64_t page = block_page(a.table + static_cast<int64_t>(b) * c.MP, c.MP, pos / c.bs, c.P);
+  if (page < 0) return;
   const int64_t r = pos % c.bs;
   for (int e = lane; e < c.Hkv * c.D; e += 64) {
     const int h = e / c.D, d = e % c.D;
@@ -116,100 +95,469 @@ struct PagedAttnArgs {
   float* lse;
 };
 
-__device__ __forceinline__ float paged_value(const scope_paged_cache& c, const void* pages, int64_t off) {
-  if (c.fp8) return e4m3x2<false>(static_cast<const uint8_t*>(pages)[off]).x;
-  const uint16_t x = static_cast<const uint16_t*>(pages)[off];
-  return c.type == SCOPE_FP16 ? half_to_f32(x) : bf16_to_f32(x);
+// Workgroups of kAttnWaves wavefronts; piece i of the batch (paged_plan.h) is
+// blockIdx.x, (key head, group of 16 query heads) blockIdx.y.
+constexpr int kAttnWaves = 4;
+constexpr int kAttnThreads = 64 * kAttnWaves;
+constexpr int kPieces = 1024;     // workgroups aimed at
+constexpr int kPieceTiles = 16;   // a piece's least tiles: 4 a wavefront
+
+struct AttnSplit {
+  int pieces, slots;   // pieces aimed at and slots of a (key head, group); with lists: pieces of every list
+  int64_t tiles_cap;   // tiles of a full table row (list)
+  float* po;           // [slots][Hq][D] partial P·V, unnormalised
+  float* pml;          // [slots][Hq][2] their maxima (log2 units) and sums
+  int2* plan;          // [B] (pieces, first slot) of each sequence
+  float* lse2;         // [B][Hq] log2 of the whole sums, for the mass
+  float* tile_lse;     // [B][Hq][tiles_cap][halves] log2 of each tile's (half tile's) sum, for the mass
+};
+
+// piece i of n of sequence b: its tiles, and the sequence's first slot
+struct Piece {
+  int b, t0, t1, i, n, slot;
+};
+
+// The piece of this workgroup, found by every wavefront for itself: the batch's
+// tiles are summed, then the sequences' numbers of pieces.  false: there is none.
+__device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const PagedAttnArgs& a, const AttnSplit& s, int x,
+                                           Piece& p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
+  const auto tiles_of = [&](int b, int* lo) {
+    *lo = 0;
+    return b < c.B ? seq_tiles(a.lens[b], a.first ? a.first[b] : 0, cap, lo) : 0;
+  };
+  int lo0;
+  const int tiles0 = tiles_of(lane, &lo0);
+  int64_t total = tiles0;
+  for (int b = 64 + lane; b < c.B; b += 64) {
+    int lo;
+    total += tiles_of(b, &lo);
+  }
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, kWave);
+  const int64_t piece = piece_tiles(total, s.pieces, kPieceTiles);
+  int before = 0;
+  for (int b0 = 0; b0 < c.B; b0 += 64) {
+    int lo = lo0;
+    const int tiles = b0 ? tiles_of(b0 + lane, &lo) : tiles0;
+    const int n = b0 + lane < c.B ? seq_pieces(tiles, piece) : 0;
+    int upto = n;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += v;
+    }
+    const uint64_t hit = __ballot(x < before + upto);
+    if (hit) {
+      const int at = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+      p.b = b0 + at;
+      p.n = __builtin_amdgcn_readlane(n, at);
+      p.slot = before + __builtin_amdgcn_readlane(upto, at) - p.n;
+      p.i = x - p.slot;
+      piece_range(__builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(tiles, at), p.n, p.i, &p.t0, &p.t1);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
 }
 
-// One workgroup per (sequence, key head), its wavefronts taking keys in turn
-// with the running maximum and sum of a softmax, merged at the end; then, for
-// the mass, the probabilities of every page's keys once more.
-constexpr int kSimpleWaves = 16;
-
-__global__ __launch_bounds__(64 * kSimpleWaves) void paged_attn_simple_kernel(scope_paged_cache c, PagedAttnArgs a) {
-  const int b = blockIdx.x, hk = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int G = a.Hq / c.Hkv, per = c.D / 64;
-  __shared__ float sm[kSimpleWaves], sl[kSimpleWaves], so[kSimpleWaves][256], s_lse;
-  const int64_t end = seq_end(c, a.lens, b);
-  const int64_t low = a.first ? max(a.first[b], 0) : 0;
-  const int64_t row = static_cast<int64_t>(b) * c.Hkv + hk;
-  const int n = a.kv_idx ? min(max(a.kv_num[row], 0), a.maxkv) : static_cast<int>((end + c.bs - 1) / c.bs);
-  const float ks = a.k_scale ? a.k_scale[hk] : 1.f, vs = a.v_scale ? a.v_scale[hk] : 1.f;
-  for (int g = 0; g < G; ++g) {
-    const int h = hk * G + g;
-    float qv[4];
-    for (int i = 0; i < per; ++i) {
-      const uint16_t x = a.q[b * a.q_sb + h * a.q_sh + lane * per + i];
-      qv[i] = (c.type == SCOPE_FP16 ? half_to_f32(x) : bf16_to_f32(x)) * (a.scale * kLog2e * ks);
-    }
-    const auto page_of = [&](int e, int64_t& lb) -> int64_t {
-      lb = a.kv_idx ? a.kv_idx[row * a.maxkv + e] : e;
-      if (lb < 0 || lb >= c.MP) return -1;
-      const int64_t page = a.table[static_cast<int64_t>(b) * c.MP + lb];
-      return page < c.P ? page : -1;
-    };
-    const auto score = [&](int64_t page, int r) {
-      float s = 0.f;
-      for (int i = 0; i < per; ++i)
-        s = fmaf(paged_value(c, a.k_pages, page * c.k_sp + hk * c.k_sh + r * c.k_sr + lane * per + i), qv[i], s);
-      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
-      return s;
-    };
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int e = 0; e < n; ++e) {
-      int64_t lb;
-      const int64_t page = page_of(e, lb);
-      if (page < 0) continue;
-      for (int r = wave; r < c.bs; r += kSimpleWaves) {
-        const int64_t j = lb * c.bs + r;
-        if (j < low || j >= end) continue;
-        const float s = score(page, r);
-        const float mn = !(s <= m) ? s : m;  // NaN stays
-        const float keep = m == -INFINITY ? 0.f : exp2f(m - mn), pr = s == -INFINITY ? 0.f : exp2f(s - mn);
-        l = l * keep + pr;
-        for (int i = 0; i < per; ++i)
-          o[i] = o[i] * keep + pr * paged_value(c, a.v_pages, page * c.v_sp + hk * c.v_sh + r * c.v_sr + lane * per + i);
-        m = mn;
-      }
-    }
-    if (lane == 0) {
-      sm[wave] = m;
-      sl[wave] = l;
-    }
-    for (int i = 0; i < per; ++i) so[wave][lane * per + i] = o[i];
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < kSimpleWaves; ++w) M = !(sm[w] <= M) ? sm[w] : M;
-    for (int w = 0; w < kSimpleWaves; ++w) L += sm[w] == -INFINITY ? 0.f : exp2f(sm[w] - M) * sl[w];
-    for (int d = threadIdx.x; d < c.D; d += blockDim.x) {
-      float acc = 0.f;
-      for (int w = 0; w < kSimpleWaves; ++w) acc += sm[w] == -INFINITY ? 0.f : exp2f(sm[w] - M) * so[w][d];
-      const float y = L == 0.f ? 0.f : acc / L * vs;
-      a.out[(static_cast<int64_t>(b) * a.Hq + h) * c.D + d] = c.type == SCOPE_FP16 ? f32_to_half(y) : f32_to_bf16(y);
-    }
-    const float lse2 = L == 0.f ? -INFINITY : M + log2f(L);
-    if (threadIdx.x == 0) {
-      a.lse[static_cast<int64_t>(b) * a.Hq + h] = lse2 * kLn2;
-      s_lse = lse2;
-    }
-    __syncthreads();
-    if (a.mass) {
-      for (int e = wave; e < n; e += kSimpleWaves) {
-        int64_t lb;
-        const int64_t page = page_of(e, lb);
-        if (page < 0) continue;
-        float w = 0.f;
-        for (int r = 0; r < c.bs; ++r) {
-          const int64_t j = lb * c.bs + r;
-          if (j < low || j >= end) continue;
-          w += exp2f(score(page, r) - s_lse);
-        }
-        if (lane == 0 && w != 0.f) a.mass[row * c.MP + lb] += w;
-      }
-    }
-    __syncthreads();
+template <int TYPE>
+__device__ __forceinline__ f32x4_t mfma_16(const uint4& a, const uint4& b, const f32x4_t& acc) {
+  if constexpr (TYPE == SCOPE_BF16) {
+    return mfma16(a, b, acc);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), acc, 0, 0, 0);
   }
+}
+
+// two 16-bit values, rounded to nearest even
+template <int TYPE>
+__device__ __forceinline__ uint32_t round2(float lo, float hi) {
+  if constexpr (TYPE == SCOPE_BF16) {
+    return cvt_pk_bf16(lo, hi);
+  } else {
+    f16x2_t v;
+    v[0] = static_cast<_Float16>(lo);
+    v[1] = static_cast<_Float16>(hi);
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// two e4m3 bytes as 16-bit values (exact)
+template <int TYPE, bool HI>
+__device__ __forceinline__ uint32_t widen2(uint32_t w) {
+  if constexpr (TYPE == SCOPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+}
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+
+// The attention of one new token.  For a tile of 32 keys and 16 query heads of
+// one key head (those past the group are zero), with lane l, g = l / 16, c = l % 16:
+//   S^T = K·Q^T   two products; operand A's row m is key 8(m/4) + 4t + m%4 of
+//                 the tile in product t, so that lane l holds of query c the
+//                 scores of the eight keys 8g .. 8g+7;
+//   O^T = V^T·P^T the same eight probabilities are operand B without moving;
+//                 operand A takes for feature f = VE·m + j (product j) the
+//                 eight keys' values, an 8 x VE transposition of 16-bit values
+//                 within the lane (v_perm) of rows loaded 16 lanes wide.
+// So K and V go from memory to the matrix units through registers alone, and a
+// query's maximum, sum and outputs stay in the lanes of its column.  Scores are
+// scaled into log2 units in fp32; the maximum that the probabilities are taken
+// relative to moves only when a score passes it by more than 8 (p <= 256 until
+// then, no loss in floating point); they are rounded to the 16-bit type for the
+// product with V, as the type's own matrix instruction takes them, and summed
+// before that rounding.
+template <int TYPE, bool FP8, int D>
+__global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void paged_attn_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
+  constexpr int NJ = D / 32;                     // products over D
+  constexpr int VE = D / 16 < 8 ? D / 16 : 8;    // features of a lane in a row of V
+  constexpr int NH = D / (16 * VE);              // rows of V in halves
+  constexpr int ES = FP8 ? 1 : 2;                // bytes of an element
+  constexpr int KV = FP8 ? NJ / 2 : NJ;          // 16-byte loads of a row of K a lane
+  constexpr int VW = VE * ES / 4;                // words of a lane in a row of V
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g4 = lane >> 4, c16 = lane & 15;
+  const int G = a.Hq / c.Hkv, ng = (G + 15) / 16;
+  const int hk = blockIdx.y / ng, cg = blockIdx.y % ng, nq = min(16, G - 16 * cg);
+  const int h0 = hk * G + 16 * cg;  // first query head
+  const bool lists = a.kv_idx != nullptr;
+  Piece p;
+  int n_list = 0;
+  if (lists) {
+    p.b = blockIdx.x / s.pieces;
+    p.i = blockIdx.x % s.pieces;
+    p.n = s.pieces;
+    p.slot = p.b * s.pieces;
+    n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
+    // pieces of one length for every list, so that the join knows which there are
+    piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
+    p.t1 = min(p.t1, static_cast<int>((static_cast<int64_t>(n_list) * c.bs + kTileKeys - 1) / kTileKeys));
+  } else if (!find_piece(c, a, s, blockIdx.x, p)) {
+    return;
+  }
+  const int b = p.b;
+  if (s.plan && blockIdx.y == 0 && p.i == 0 && threadIdx.x == 0) s.plan[b] = make_int2(p.n, p.slot);
+  const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
+  const int end = static_cast<int>(seq_end(a.lens[b], cap)), low = a.first ? max(a.first[b], 0) : 0;
+  const int32_t* row = a.table + static_cast<int64_t>(b) * c.MP;
+  const int32_t* list = lists ? a.kv_idx + (static_cast<int64_t>(b) * c.Hkv + hk) * a.maxkv : nullptr;
+  const int shift = __builtin_ctz(c.bs);
+  const bool small = c.bs == 16;  // a tile is two pages
+
+  // Q^T: column c is query head h0 + c
+  uint4 qf[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int d = FP8 ? (j / 2) * 64 + g4 * 16 + (j % 2) * 8 : j * 32 + g4 * 8;
+    qf[j] = make_uint4(0, 0, 0, 0);
+    if (c16 < nq) qf[j] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (h0 + c16) * a.q_sh + d);
+  }
+  const float to_log2 = a.scale * kLog2e * (a.k_scale ? a.k_scale[hk] : 1.f);
+
+  f32x4_t acc[NH * VE];
+#pragma unroll
+  for (int i = 0; i < NH * VE; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  const char* kbase = static_cast<const char*>(a.k_pages) + hk * c.k_sh * ES;
+  const char* vbase = static_cast<const char*>(a.v_pages) + hk * c.v_sh * ES;
+  const int krow = (c16 >> 2) * 8 + (c16 & 3), vrow = g4 * 8;
+  const int64_t koff = ((small ? krow & 15 : krow) * c.k_sr + g4 * (16 / ES)) * ES;
+  const int64_t voff = ((small ? vrow & 15 : vrow) * c.v_sr + c16 * VE) * ES;
+
+  // pages and blocks of this wavefront's next 64 tiles, one a lane (two where a tile is two pages)
+  int pg0 = -1, pg1 = -1, lb0 = 0, lb1 = 0;
+  const auto resolve = [&](int t) {
+    const auto one = [&](int64_t e, int& lb) -> int {  // entry e of the list, or block e
+      int64_t blk = e;
+      if (lists) {
+        if (e >= n_list) return -1;
+        blk = list[e];
+      }
+      const int64_t page = block_page(row, c.MP, blk, c.P);
+      lb = page < 0 ? 0 : static_cast<int>(blk);
+      return static_cast<int>(page);
+    };
+    pg0 = pg1 = -1;
+    lb0 = lb1 = 0;
+    if (t < p.t1) {
+      const int64_t e = (static_cast<int64_t>(t) * kTileKeys) >> shift;
+      pg0 = one(e, lb0);
+      if (small) pg1 = one(e + 1, lb1);
+    }
+  };
+
+  int u = 64;
+  for (int t = p.t0 + wave; t < p.t1; t += kAttnWaves, ++u) {
+    if (u == 64) {
+      resolve(t + lane * kAttnWaves);
+      u = 0;
+    }
+    const int page0 = __builtin_amdgcn_readlane(pg0, u), page1 = small ? __builtin_amdgcn_readlane(pg1, u) : page0;
+    const int64_t stat = s.tile_lse ? (((static_cast<int64_t>(b) * a.Hq + h0 + c16) * s.tiles_cap + t) << small) : 0;
+    if (page0 < 0 && page1 < 0) {  // nothing to see
+      if (s.tile_lse && c16 < nq && (g4 & (small ? 1 : 3)) == 0) s.tile_lse[stat + (small ? g4 >> 1 : 0)] = -INFINITY;
+      continue;
+    }
+    const int r0 = small ? 0 : (t * kTileKeys) & (c.bs - 1);  // the tile's first row in its page
+    // this lane's rows of K (product operand) and of V (and of the scores)
+    const int kp = small && krow >= 16 ? page1 : page0, vp = small && vrow >= 16 ? page1 : page0;
+    const char* kr = kbase + (static_cast<int64_t>(max(kp, 0)) * c.k_sp + r0 * c.k_sr) * ES + koff;
+    const char* vr = vbase + (static_cast<int64_t>(max(vp, 0)) * c.v_sp + r0 * c.v_sr) * ES + voff;
+    uint4 kf[2][KV];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < KV; ++j) kf[i][j] = *reinterpret_cast<const uint4*>(kr + 4 * i * c.k_sr * ES + j * 64);
+    Words<VW> vf[NH][8];
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vf[h][i] = *reinterpret_cast<const Words<VW>*>(vr + (i * c.v_sr + h * 128) * ES);
+
+    // scores
+    f32x4_t sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if constexpr (FP8) {
+          const uint4 w = kf[i][j / 2];
+          const uint32_t x = j % 2 ? w.z : w.x, y = j % 2 ? w.w : w.y;
+          sc[i] = mfma_16<TYPE>(make_uint4(widen2<TYPE, false>(x), widen2<TYPE, true>(x), widen2<TYPE, false>(y),
+                                           widen2<TYPE, true>(y)), qf[j], sc[i]);
+        } else {
+          sc[i] = mfma_16<TYPE>(kf[i][j], qf[j], sc[i]);
+        }
+      }
+    }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * to_log2;
+    // the lane's first key; keys outside [low, end) and of no page are not seen
+    const int lbl = small && vrow >= 16 ? __builtin_amdgcn_readlane(lb1, u) : __builtin_amdgcn_readlane(lb0, u);
+    const int64_t pos = static_cast<int64_t>(lbl) * c.bs + r0 + (small ? vrow & 15 : vrow);
+    const int from = vp < 0 ? 8 : static_cast<int>(min(max(low - pos, static_cast<int64_t>(0)), static_cast<int64_t>(8)));
+    const int to = static_cast<int>(min(max(end - pos, static_cast<int64_t>(0)), static_cast<int64_t>(8)));
+    if (__any(from > 0 || to < 8)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool see = i >= from && i < to;
+        x[i] = see ? x[i] : -INFINITY;
+        // (a row that is not seen may hold anything, and 0 times NaN is NaN)
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vf[h][i].w[w] = see ? vf[h][i].w[w] : 0u;
+      }
+    }
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    if (__any(top > m + 8.f)) {
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < NH * VE; ++i) acc[i] *= f;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float lt = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+      lt += x[i];
+    }
+    l += lt;
+    if (s.tile_lse) {
+      lt += __shfl_xor(lt, 16, kWave);
+      if (!small) lt += __shfl_xor(lt, 32, kWave);
+      if (c16 < nq && (g4 & (small ? 1 : 3)) == 0) s.tile_lse[stat + (small ? g4 >> 1 : 0)] = ref + __builtin_amdgcn_logf(lt);
+    }
+    const uint4 pf = make_uint4(round2<TYPE>(x[0], x[1]), round2<TYPE>(x[2], x[3]), round2<TYPE>(x[4], x[5]),
+                                round2<TYPE>(x[6], x[7]));
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      uint32_t v[8][VE / 2];  // the eight rows as 16-bit pairs of neighbouring features
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int w = 0; w < VE / 2; ++w) {
+          if constexpr (FP8)
+            v[i][w] = w % 2 ? widen2<TYPE, true>(vf[h][i].w[w / 2]) : widen2<TYPE, false>(vf[h][i].w[w / 2]);
+          else
+            v[i][w] = vf[h][i].w[w];
+        }
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        uint32_t o[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          o[w] = j % 2 ? pack_hi16(v[2 * w][j / 2], v[2 * w + 1][j / 2]) : pack_lo16(v[2 * w][j / 2], v[2 * w + 1][j / 2]);
+        acc[h * VE + j] = mfma_16<TYPE>(make_uint4(o[0], o[1], o[2], o[3]), pf, acc[h * VE + j]);
+      }
+    }
+  }
+
+  // the wavefronts' shares: maxima and sums, then the outputs of the group's queries
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  float* sm = lds;                       // [waves][16]
+  float* sl = lds + kAttnWaves * 16;     // [waves][16]
+  float* so = lds + kAttnWaves * 32;     // [waves][nq][D]
+  if (g4 == 0) {
+    sm[wave * 16 + c16] = m;
+    sl[wave * 16 + c16] = l;
+  }
+  if (c16 < nq) {
+    float* o = so + (wave * nq + c16) * D + g4 * 4 * VE;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VE; j += 4)
+          *reinterpret_cast<float4*>(o + h * 128 + r * VE + j) = make_float4(
+              acc[h * VE + j][r], acc[h * VE + j + 1][r], acc[h * VE + j + 2][r], acc[h * VE + j + 3][r]);
+  }
+  __syncthreads();
+  const float vs = a.v_scale ? a.v_scale[hk] : 1.f;
+  for (int i = threadIdx.x; i < nq * D; i += kAttnThreads) {
+    const int q = i / D, d = i % D, h = h0 + q;
+    float M = sm[q];
+#pragma unroll
+    for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, sm[w * 16 + q]);
+    float L = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) {
+      // (a sum of 0 is a share without keys; a NaN stays one, whatever its maximum)
+      const float f = sl[w * 16 + q] == 0.f ? 0.f : __builtin_amdgcn_exp2f(sm[w * 16 + q] - M);
+      L += f * sl[w * 16 + q];
+      o += f * so[(w * nq + q) * D + d];
+    }
+    if (p.n == 1) {
+      const float y = L == 0.f ? 0.f : o / L * vs;
+      a.out[(static_cast<int64_t>(b) * a.Hq + h) * D + d] = TYPE == SCOPE_FP16 ? f32_to_half(y) : f32_to_bf16(y);
+      if (d == 0) {
+        const float e = L == 0.f ? -INFINITY : M + __builtin_amdgcn_logf(L);
+        a.lse[static_cast<int64_t>(b) * a.Hq + h] = e * kLn2;
+        if (s.lse2) s.lse2[static_cast<int64_t>(b) * a.Hq + h] = e;
+      }
+    } else {
+      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.Hq + h;
+      s.po[at * D + d] = o;
+      if (d == 0) {
+        s.pml[2 * at] = M;
+        s.pml[2 * at + 1] = L;
+      }
+    }
+  }
+}
+
+// The pieces of one (sequence, query head) joined: relative to the largest of
+// their maxima, sixteen bytes of the output row a thread, the pieces shared out
+// over the groups of threads.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
+  const int b = blockIdx.x, h = blockIdx.y;
+  const bool lists = a.kv_idx != nullptr;
+  const int2 plan = lists ? make_int2(s.pieces, b * s.pieces) : s.plan[b];
+  const int n = plan.x;
+  if (n == 1) return;  // written by its only piece
+  constexpr int LD = D / 4, NG = 256 / LD;
+  __shared__ float w[kPieces], red[2][4], so[NG][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* ml = s.pml + (static_cast<int64_t>(plan.y) * a.Hq + h) * 2;
+  float M = -INFINITY;
+  for (int i = tid; i < n; i += 256) M = fmaxf(M, ml[static_cast<int64_t>(i) * a.Hq * 2]);
+  M = wave_max_f32(M);
+  if (lane == 0) red[0][wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float L = 0.f;
+  for (int i = tid; i < n; i += 256) {
+    const float mi = ml[static_cast<int64_t>(i) * a.Hq * 2], li = ml[static_cast<int64_t>(i) * a.Hq * 2 + 1];
+    const float f = li == 0.f ? 0.f : __builtin_amdgcn_exp2f(mi - M);
+    w[i] = f;
+    L += f * li;
+  }
+  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, kWave);
+  if (lane == 0) red[1][wave] = L;
+  __syncthreads();
+  L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  const int dl = tid % LD, grp = tid / LD;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float* po = s.po + (static_cast<int64_t>(plan.y) * a.Hq + h) * D + 4 * dl;
+  for (int i = grp; i < n; i += NG) {
+    const float4 v = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(i) * a.Hq * D);
+    const float f = w[i];
+    acc.x += f * v.x;
+    acc.y += f * v.y;
+    acc.z += f * v.z;
+    acc.w += f * v.w;
+  }
+  *reinterpret_cast<float4*>(&so[grp][4 * dl]) = acc;
+  __syncthreads();
+  if (tid < D) {
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) o += so[i][tid];
+    const float y = L == 0.f ? 0.f : o / L * (a.v_scale ? a.v_scale[h / (a.Hq / c.Hkv)] : 1.f);
+    a.out[(static_cast<int64_t>(b) * a.Hq + h) * D + tid] = c.type == SCOPE_FP16 ? f32_to_half(y) : f32_to_bf16(y);
+    if (tid == 0) {
+      const float e = L == 0.f ? -INFINITY : M + __builtin_amdgcn_logf(L);
+      a.lse[static_cast<int64_t>(b) * a.Hq + h] = e * kLn2;
+      if (s.lse2) s.lse2[static_cast<int64_t>(b) * a.Hq + h] = e;
+    }
+  }
+}
+
+// Every block's probabilities, from its tiles' sums and the rows' whole ones:
+// one thread per listed block (or block of the sequence), its heads and tiles in
+// order.
+__global__ __launch_bounds__(256) void paged_mass_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
+  const int b = blockIdx.x, hk = blockIdx.y, G = a.Hq / c.Hkv;
+  const int64_t e = static_cast<int64_t>(blockIdx.z) * 256 + threadIdx.x, bh = static_cast<int64_t>(b) * c.Hkv + hk;
+  const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
+  int64_t lb = e;
+  int lo = 0;
+  int64_t hi;
+  if (a.kv_idx) {
+    const int n = min(max(a.kv_num[bh], 0), a.maxkv);
+    if (e >= n) return;
+    lb = a.kv_idx[bh * a.maxkv + e];
+    hi = (static_cast<int64_t>(n) * c.bs + kTileKeys - 1) / kTileKeys;
+  } else {
+    const int tiles = seq_tiles(a.lens[b], a.first ? a.first[b] : 0, cap, &lo);
+    hi = lo + tiles;
+  }
+  if (lb < 0 || lb >= c.MP) return;
+  // the block's tiles (half tiles of blocks of 16) among those that were formed
+  const int halves = c.bs == 16 ? 2 : 1, per = c.bs == 16 ? 1 : c.bs / kTileKeys;
+  const int64_t u0 = max(e * per, static_cast<int64_t>(lo) * halves), u1 = min((e + 1) * per, hi * halves);
+  if (u0 >= u1) return;
+  float w = 0.f;
+  for (int g = 0; g < G; ++g) {
+    const int64_t h = static_cast<int64_t>(b) * a.Hq + hk * G + g;
+    const float all = s.lse2[h];
+    if (all == -INFINITY) continue;
+    const float* t = s.tile_lse + h * s.tiles_cap * halves;
+    for (int64_t u = u0; u < u1; ++u) w += __builtin_amdgcn_exp2f(t[u] - all);
+  }
+  // (a list may name a block once; an atomic for the lists that break this)
+  if (a.kv_idx)
+    atomicAdd(a.mass + bh * c.MP + lb, w);
+  else
+    a.mass[bh * c.MP + lb] += w;
 }
 
 // ---- eviction -----------------------------------------------------------------
@@ -323,6 +671,38 @@ int check_cache(const scope_paged_cache* c, const void* k_pages, const void* v_p
                 "%s: the rows of the pages must be 16-byte aligned", fn);
   return SCOPE_OK;
 }
+
+// The pieces of a call and its workspace (laid out in `work` where s is given);
+// returns its bytes.
+int64_t plan_split(const scope_paged_cache& c, int Hq, int maxkv, bool with_mass, AttnSplit* out, void* work) {
+  const int G = Hq / c.Hkv, ng = (G + 15) / 16;
+  const int64_t keys = static_cast<int64_t>(maxkv ? maxkv : c.MP) * c.bs;
+  AttnSplit s{};
+  s.tiles_cap = (keys + kTileKeys - 1) / kTileKeys;
+  const int64_t cols = static_cast<int64_t>(c.Hkv) * ng * (maxkv ? c.B : 1);
+  const int64_t most = (s.tiles_cap + kPieceTiles - 1) / kPieceTiles;
+  s.pieces = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((kPieces + cols - 1) / cols, maxkv ? most : kPieces)));
+  const bool split = most > 1 && s.pieces > 1;
+  s.slots = maxkv ? s.pieces * c.B : split ? s.pieces + c.B : c.B;
+  if (!split) s.pieces = 1;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    char* p = work ? static_cast<char*>(work) + at : nullptr;
+    at += (bytes + 15) & ~static_cast<int64_t>(15);
+    return p;
+  };
+  if (split) {
+    s.po = reinterpret_cast<float*>(take(4ll * s.slots * Hq * c.D));
+    s.pml = reinterpret_cast<float*>(take(8ll * s.slots * Hq));
+    s.plan = reinterpret_cast<int2*>(take(8ll * c.B));
+  }
+  if (with_mass) {
+    s.lse2 = reinterpret_cast<float*>(take(4ll * c.B * Hq));
+    s.tile_lse = reinterpret_cast<float*>(take(4ll * c.B * Hq * s.tiles_cap * (c.bs == 16 ? 2 : 1)));
+  }
+  if (out) *out = s;
+  return at;
+}
 }  // namespace
 
 }  // namespace scope
@@ -348,7 +728,10 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
   return check_launch("paged_append_kernel");
 }
 
-int64_t scope_paged_attn_workspace_bytes(const scope_paged_cache* c, int Hq, int maxkv, int with_mass) { return 16; }
+int64_t scope_paged_attn_workspace_bytes(const scope_paged_cache* c, int Hq, int maxkv, int with_mass) {
+  if (!c || c->Hkv < 1 || Hq < 1 || Hq % c->Hkv) return 0;
+  return plan_split(*c, Hq, maxkv, with_mass != 0, nullptr, nullptr);
+}
 
 int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float scale, const uint16_t* q, int64_t q_sb,
                             int64_t q_sh, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -359,14 +742,54 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
   if (int rc = check_cache(c, k_pages, v_pages, fn)) return rc;
   SCOPE_REQUIRE(Hq >= 1 && Hq <= 65535 && Hq % c->Hkv == 0, "%s: Hq=%d must be a multiple of Hkv=%d, at most 65535", fn, Hq,
                 c->Hkv);
-  SCOPE_REQUIRE((kv_num != nullptr) == (kv_idx != nullptr) && (!kv_idx || maxkv >= 1),
-                "%s: kv_num and kv_idx come together, with maxkv >= 1 (got %d)", fn, maxkv);
-  SCOPE_REQUIRE(q && table && lens && out && lse, "%s: null pointer", fn);
-  SCOPE_REQUIRE(aligned16(q) && q_sb % 8 == 0 && q_sh % 8 == 0, "%s: the rows of q must be 16-byte aligned", fn);
+  SCOPE_REQUIRE((kv_num != nullptr) == (kv_idx != nullptr) &&
+                    (kv_idx ? maxkv >= 1 && static_cast<int64_t>(maxkv) * c->bs <= INT32_MAX : maxkv == 0),
+                "%s: kv_num and kv_idx come together, with 1 .. 2^31 / bs entries (maxkv=%d; 0 without lists)", fn, maxkv);
+  SCOPE_REQUIRE(q && table && lens && out && lse && work, "%s: null pointer", fn);
+  SCOPE_REQUIRE(aligned16(q) && aligned16(work) && q_sb % 8 == 0 && q_sh % 8 == 0,
+                "%s: the rows of q and the workspace must be 16-byte aligned", fn);
   const PagedAttnArgs a{Hq,    maxkv, scale, q_sb,   q_sh,   q,    k_pages, v_pages, k_scale,
                         v_scale, table, lens,  first, kv_num, kv_idx, mass, out,     lse};
-  hipLaunchKernelGGL(paged_attn_simple_kernel, dim3(c->B, c->Hkv), dim3(64 * kSimpleWaves), 0, as_stream(stream), *c, a);
-  return check_launch("paged_attn_simple_kernel");
+  AttnSplit s;
+  plan_split(*c, Hq, maxkv, mass != nullptr, &s, work);
+  const int G = Hq / c->Hkv, ng = (G + 15) / 16;
+  const dim3 grid(s.slots, c->Hkv * ng);
+  const size_t lds = sizeof(float) * kAttnWaves * (32 + static_cast<size_t>(std::min(G, 16)) * c->D);
+  hipStream_t st = as_stream(stream);
+  const auto launch = [&](auto type, auto fp8) {
+    constexpr int T = decltype(type)::value;
+    constexpr bool F = decltype(fp8)::value;
+    if (c->D == 64)
+      hipLaunchKernelGGL((paged_attn_kernel<T, F, 64>), grid, dim3(kAttnThreads), lds, st, *c, a, s);
+    else if (c->D == 128)
+      hipLaunchKernelGGL((paged_attn_kernel<T, F, 128>), grid, dim3(kAttnThreads), lds, st, *c, a, s);
+    else
+      hipLaunchKernelGGL((paged_attn_kernel<T, F, 256>), grid, dim3(kAttnThreads), lds, st, *c, a, s);
+  };
+  using std::integral_constant;
+  if (c->type == SCOPE_BF16)
+    c->fp8 ? launch(integral_constant<int, SCOPE_BF16>{}, integral_constant<bool, true>{})
+           : launch(integral_constant<int, SCOPE_BF16>{}, integral_constant<bool, false>{});
+  else
+    c->fp8 ? launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, true>{})
+           : launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, false>{});
+  if (int rc = check_launch("paged_attn_kernel")) return rc;
+  if (s.po) {  // some sequence may be in several pieces
+    const dim3 jg(c->B, Hq);
+    if (c->D == 64)
+      hipLaunchKernelGGL(paged_join_kernel<64>, jg, dim3(256), 0, st, *c, a, s);
+    else if (c->D == 128)
+      hipLaunchKernelGGL(paged_join_kernel<128>, jg, dim3(256), 0, st, *c, a, s);
+    else
+      hipLaunchKernelGGL(paged_join_kernel<256>, jg, dim3(256), 0, st, *c, a, s);
+    if (int rc = check_launch("paged_join_kernel")) return rc;
+  }
+  if (mass) {
+    const int blocks = kv_idx ? maxkv : c->MP;
+    hipLaunchKernelGGL(paged_mass_kernel, dim3(c->B, c->Hkv, ceil_div(blocks, 256)), dim3(256), 0, st, *c, a, s);
+    return check_launch("paged_mass_kernel");
+  }
+  return SCOPE_OK;
 }
 
 int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, const int32_t* table, const float* mass,
