@@ -27,9 +27,12 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 // ---- append ------------------------------------------------------------------
 // Row i of the N new ones belongs to the sequence b with cu[b] <= i < cu[b + 1]
 // (row i to sequence i without cu) and goes to position lens[b] + i - cu[b].
-// One wavefront per row.
+// Bound by memory: a wavefront takes `rows` rows; lane r finds the place of its
+// r-th row (a search, two loads), so the chain of loads is paid once for all of
+// them, then every row moves 16 bytes a lane.
 struct AppendArgs {
   int64_t N, k_sn, k_sh, v_sn, v_sh;
+  int rows;
   const uint16_t* k;
   const uint16_t* v;
   const int32_t* cu;
@@ -41,36 +44,80 @@ struct AppendArgs {
   void* v_pages;
 };
 
-// the e4m3 byte of x / s: the quotient cut to the largest finite value, then
-// rounded to nearest even (one rounding each; NaN stays NaN)
-__device__ __forceinline__ uint8_t to_e4m3(float x, float s) {
-  const float q = x / s;
-  const float y = q > 448.f ? 448.f : q < -448.f ? -448.f : q;
-  return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xff);
+// 1 / s where the quotient x / s may be formed by it (quotient below), else 0
+__device__ __forceinline__ float quotient_factor(float s) {
+  return s >= 0x1p-60f && s <= 0x1p60f ? 1.f / s : 0.f;
 }
 
+// The fp32 quotient x / s of a 16-bit x, rounded to nearest as a division rounds
+// it, as far as e4m3 can tell.  With r = 1 / s to nearest, q = x·r is off by at
+// most two steps, and one residual step q + r·(x - q·s) is the quotient to
+// nearest (the residual is exact while it does not fall below 2^-126: with s in
+// 2^-60 .. 2^60 that is only where |q| < 2^-20, which is 0 in e4m3 either way).
+// Quotients past every finite e4m3, infinities and NaN need no residual.  Three
+// instructions for the division's ten.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+  if (r == 0.f) return x / s;
+  const float q = x * r;
+  const float a = fabsf(q);
+  return a >= 0x1p-20f && a < 0x1p20f ? __builtin_fmaf(__builtin_fmaf(-q, s, x), r, q) : q;
+}
+
+// eight 16-bit values as e4m3 of x / s: cut to the largest finite value, rounded
+// to nearest even; NaN stays NaN
+template <int TYPE>
+__device__ __forceinline__ uint2 e4m3x8(const uint4& u, float s, float r) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t h = static_cast<uint16_t>(i % 2 ? w[i / 2] >> 16 : w[i / 2]);
+    const float q = quotient(TYPE == SCOPE_FP16 ? half_to_f32(h) : bf16_to_f32(h), s, r);
+    f[i] = q > 448.f ? 448.f : q < -448.f ? -448.f : q;
+  }
+  uint32_t o[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    o[i] = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+    o[i] = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], o[i], true);
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+template <int TYPE, bool FP8>
 __global__ __launch_bounds__(256) void paged_append_kernel(scope_paged_cache c, AppendArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (i >= a.N) return;
-  int b;
-  const int64_t pos = row_position(a.cu, a.lens, c.B, i, &b);
-  if (pos < 0) return;
-  const int64_t page = block_page(a.table + static_cast<int64_t>(b) * c.MP, c.MP, pos / c.bs, c.P);
-  if (page < 0) return;
-  const int64_t r = pos % c.bs;
-  for (int e = lane; e < c.Hkv * c.D; e += 64) {
-    const int h = e / c.D, d = e % c.D;
-    const uint16_t xk = a.k[i * a.k_sn + h * a.k_sh + d], xv = a.v[i * a.v_sn + h * a.v_sh + d];
-    const int64_t ok = page * c.k_sp + h * c.k_sh + r * c.k_sr + d, ov = page * c.v_sp + h * c.v_sh + r * c.v_sr + d;
-    if (c.fp8) {
-      const float fk = c.type == SCOPE_FP16 ? half_to_f32(xk) : bf16_to_f32(xk);
-      const float fv = c.type == SCOPE_FP16 ? half_to_f32(xv) : bf16_to_f32(xv);
-      static_cast<uint8_t*>(a.k_pages)[ok] = to_e4m3(fk, a.k_scale ? a.k_scale[h] : 1.f);
-      static_cast<uint8_t*>(a.v_pages)[ov] = to_e4m3(fv, a.v_scale ? a.v_scale[h] : 1.f);
-    } else {
-      static_cast<uint16_t*>(a.k_pages)[ok] = xk;
-      static_cast<uint16_t*>(a.v_pages)[ov] = xv;
+  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * a.rows;
+  // lane r: page (-1: the row is not written) and slot of row i0 + r
+  int page_l = -1, slot_l = 0;
+  if (lane < a.rows && i0 + lane < a.N) {
+    int b;
+    const int64_t pos = row_position(a.cu, a.lens, c.B, i0 + lane, &b);
+    if (pos >= 0 && pos < static_cast<int64_t>(c.MP) * c.bs) {
+      page_l = static_cast<int>(block_page(a.table + static_cast<int64_t>(b) * c.MP, c.MP, pos / c.bs, c.P));
+      slot_l = static_cast<int>(pos % c.bs);
+    }
+  }
+  const int chunks = c.Hkv * c.D / 8, dshift = __builtin_ctz(c.D) - 3;
+  for (int r = 0; r < a.rows; ++r) {
+    const int page = __builtin_amdgcn_readlane(page_l, r), slot = __builtin_amdgcn_readlane(slot_l, r);
+    if (page < 0) continue;
+    const uint16_t* ks = a.k + (i0 + r) * a.k_sn;
+    const uint16_t* vs = a.v + (i0 + r) * a.v_sn;
+    const int64_t ko = static_cast<int64_t>(page) * c.k_sp + slot * c.k_sr, vo = static_cast<int64_t>(page) * c.v_sp + slot * c.v_sr;
+    for (int e = lane; e < chunks; e += 64) {
+      const int h = e >> dshift, d = (e & ((1 << dshift) - 1)) * 8;
+      const uint4 xk = *reinterpret_cast<const uint4*>(ks + h * a.k_sh + d);
+      const uint4 xv = *reinterpret_cast<const uint4*>(vs + h * a.v_sh + d);
+      const int64_t ok = ko + h * c.k_sh + d, ov = vo + h * c.v_sh + d;
+      if constexpr (FP8) {
+        const float sk = a.k_scale ? a.k_scale[h] : 1.f, sv = a.v_scale ? a.v_scale[h] : 1.f;
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.k_pages) + ok) = e4m3x8<TYPE>(xk, sk, quotient_factor(sk));
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v_pages) + ov) = e4m3x8<TYPE>(xv, sv, quotient_factor(sv));
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.k_pages) + ok) = xk;
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.v_pages) + ov) = xv;
+      }
     }
   }
 }
@@ -573,82 +620,167 @@ struct EvictArgs {
 };
 
 // A total order of the accumulated weights: unsigned keys that compare as the
-// floats do, -0 as +0, NaN above everything.
+// floats do, -0 as +0, NaN above them, and above all a block that may not go.
+constexpr uint32_t kKeyNaN = 0xfffffffeu, kKeyStays = 0xffffffffu;
 __device__ __forceinline__ uint32_t weight_key(float f) {
-  if (f != f) return 0xffffffffu;
+  if (f != f) return kKeyNaN;
   const uint32_t u = __float_as_uint(f + 0.f);
   return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-// One workgroup per sequence.  The number of candidate pages with a smaller
-// key, or the same key and a smaller index, is a page's rank; the first ones
-// go.  The keys sit in the freed row until the ids replace them.
-constexpr int kEvictThreads = 1024;
+// One workgroup per sequence, K blocks a thread (block i = 1024·k + thread) with
+// their keys in registers, so that mass is read once.  The n-th smallest key is
+// found two bits a step: a step counts the keys below three probes (a comparison
+// and a popcount of its mask a key and probe) and costs one barrier.  Blocks with
+// a smaller key go, of those with the same key the first ones.
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 
-__device__ __forceinline__ int block_sum(int v, int* red) {
-  v = wave_sum_i32(v);
+// counts[k·16 + wavefront] = the set flags before that group of 64 blocks, in the
+// blocks' order; returns the sum of all.  counts: K·16 + 1 ints of LDS.
+template <int K, class Flag>
+__device__ __forceinline__ int prefix_flags(Flag flag, int* counts) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int n = __popcll(__ballot(flag(k)));
+    if (lane == 0) counts[k * kEvictWaves + wave] = n;
+  }
   __syncthreads();
-  int s = 0;
-  for (int w = 0; w < kEvictThreads / 64; ++w) s += red[w];
-  return s;
+  if (wave == 0) {  // K·16 counts, K/4 neighbouring ones a lane
+    constexpr int N = K * kEvictWaves, PER = N < 64 ? 1 : N / 64;
+    int v[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      v[i] = lane * PER + i < N ? counts[lane * PER + i] : 0;
+      sum += v[i];
+    }
+    int upto = sum;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += x;
+    }
+    int at = upto - sum;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (lane * PER + i < N) counts[lane * PER + i] = at;
+      at += v[i];
+    }
+    if (lane == 63) counts[N] = upto;
+  }
+  __syncthreads();
+  return counts[K * kEvictWaves];
 }
 
+template <int K>
 __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(EvictArgs a) {
-  const int b = blockIdx.x, tid = threadIdx.x;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t base = static_cast<int64_t>(b) * a.MP;
-  __shared__ int red[kEvictThreads / 64];
+  __shared__ int counts[K * kEvictWaves + 1];
+  __shared__ int4 steps[2][kEvictWaves];
   const int64_t len = a.lens[b];
   const int n = len <= 0 ? 0 : static_cast<int>(min((len + a.bs - 1) / a.bs, static_cast<int64_t>(a.MP)));
-  int held = 0, may = 0;
-  for (int i = tid; i < n; i += kEvictThreads) {
-    const bool here = a.table[base + i] >= 0;
-    held += here;
-    may += here && i >= a.n_global && i < n - a.window;
+  uint32_t key[K];
+  int held = 0, may = 0;  // of the wavefront
+  // KG blocks at a time, so that their loads are under way together (block
+  // indices past the row are cut to it, and left out of the keys)
+  constexpr int KG = K < 8 ? K : 8, UH = KG == 8 ? 2 : 8;
+#pragma unroll
+  for (int g = 0; g < K; g += KG) {
+#pragma unroll
+    for (int k = 0; k < KG; ++k) key[g + k] = kKeyStays;
+    if (g * kEvictThreads >= n) continue;
+    int id[KG];
+    double sum[KG];
+    const float* w[KG];
+#pragma unroll
+    for (int k = 0; k < KG; ++k) {
+      const int i = min((g + k) * kEvictThreads + tid, a.MP - 1);
+      id[k] = a.table[base + i];
+      w[k] = a.mass + static_cast<int64_t>(b) * a.Hkv * a.MP + i;
+      sum[k] = 0.0;
+    }
+#pragma unroll UH
+    for (int h = 0; h < a.Hkv; ++h) {
+#pragma unroll
+      for (int k = 0; k < KG; ++k) sum[k] += w[k][static_cast<int64_t>(h) * a.MP];
+    }
+#pragma unroll
+    for (int k = 0; k < KG; ++k) {
+      const int i = (g + k) * kEvictThreads + tid;
+      const bool here = i < n && id[k] >= 0, can = here && i >= a.n_global && i < n - a.window;
+      held += __popcll(__ballot(here));
+      may += __popcll(__ballot(can));
+      if (can) key[g + k] = weight_key(static_cast<float>(sum[k]));
+    }
   }
-  held = block_sum(held, red);
-  may = block_sum(may, red);
-  const int over = held - max(a.budget[b], 0);
-  const int n_drop = min(max(over, 0), may);
-  const auto key_of = [&](int i) -> uint64_t {  // above every weight where the page may not go
-    if (i < a.n_global || i >= n - a.window || a.table[base + i] < 0) return ~0ull;
-    double s = 0.0;
-    for (int h = 0; h < a.Hkv; ++h) s += a.mass[(static_cast<int64_t>(b) * a.Hkv + h) * a.MP + i];
-    return static_cast<uint64_t>(weight_key(static_cast<float>(s))) << 31 | static_cast<uint32_t>(i);
-  };
-  // the n_drop-th smallest (key, index), bit by bit: pages at or below it go
-  uint64_t cut = 0;
+  if (lane == 0) steps[1][wave] = make_int4(held, may, 0, 0);
+  __syncthreads();
+  held = may = 0;
+#pragma unroll
+  for (int w = 0; w < kEvictWaves; ++w) {
+    held += steps[1][w].x;
+    may += steps[1][w].y;
+  }
+  const int n_drop = min(max(held - max(a.budget[b], 0), 0), may);
+  uint64_t go = 0;  // bit k: block k of this thread
   if (n_drop > 0) {
-    for (int bit = 62; bit >= 0; --bit) {
-      const uint64_t probe = cut | 1ull << bit;
-      int below = 0;
-      for (int i = tid; i < n; i += kEvictThreads) below += key_of(i) < probe;
-      if (block_sum(below, red) < n_drop) cut = probe;
+    uint32_t cut = 0;  // the largest value that fewer than n_drop keys lie below
+    int below = 0;     // keys below it
+#pragma unroll 1
+    for (int bit = 30, at = 0; bit >= 0; bit -= 2, at ^= 1) {
+      const uint32_t p1 = cut | 1u << bit, p2 = cut | 2u << bit, p3 = cut | 3u << bit;
+      int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        n1 += __popcll(__ballot(key[k] < p1));
+        n2 += __popcll(__ballot(key[k] < p2));
+        n3 += __popcll(__ballot(key[k] < p3));
+      }
+      if (lane == 0) steps[at][wave] = make_int4(n1, n2, n3, 0);
+      __syncthreads();  // (the other half of steps is written in the next step)
+      n1 = n2 = n3 = 0;
+#pragma unroll
+      for (int w = 0; w < kEvictWaves; ++w) {
+        const int4 x = steps[at][w];
+        n1 += x.x;
+        n2 += x.y;
+        n3 += x.z;
+      }
+      if (n3 < n_drop) {
+        cut = p3;
+        below = n3;
+      } else if (n2 < n_drop) {
+        cut = p2;
+        below = n2;
+      } else if (n1 < n_drop) {
+        cut = p1;
+        below = n1;
+      }
+    }
+    prefix_flags<K>([&](int k) { return key[k] == cut; }, counts);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const uint64_t same = __ballot(key[k] == cut);
+      const int rank = below + counts[k * kEvictWaves + wave] + __popcll(same & ((1ull << lane) - 1));
+      if (key[k] < cut || (key[k] == cut && rank < n_drop)) go |= 1ull << k;
     }
   }
-  // ids in the pages' order
-  int done = 0;
-  for (int i0 = 0; i0 < a.MP; i0 += kEvictThreads) {
-    const int i = i0 + tid;
-    const int id = i < a.MP ? a.table[base + i] : -1;
-    const bool go = n_drop > 0 && i < n && key_of(i) <= cut;
-    const uint64_t ballot = __ballot(go);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = __popcll(ballot);
-    __syncthreads();
-    int at = done + __popcll(ballot & ((1ull << (tid & 63)) - 1));
-    int all = 0;
-    for (int w = 0; w < kEvictThreads / 64; ++w) {
-      if (w < (tid >> 6)) at += red[w];
-      all += red[w];
+  // ids in the blocks' order
+  const int all = prefix_flags<K>([&](int k) { return go >> k & 1; }, counts);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = k * kEvictThreads + tid;
+    const bool mine = go >> k & 1;
+    const uint64_t gone = __ballot(mine);
+    if (i < a.MP) {
+      const int id = a.table[base + i];  // (this thread alone writes table_out's entry, which may be this one)
+      if (mine) a.freed[base + counts[k * kEvictWaves + wave] + __popcll(gone & ((1ull << lane) - 1))] = id;
+      a.table_out[base + i] = mine ? -1 : id;
     }
-    if (go) a.freed[base + at] = id;
-    if (i < a.MP) a.table_out[base + i] = go ? -1 : id;
-    done += all;
   }
-  for (int i = done + tid; i < a.MP; i += kEvictThreads) a.freed[base + i] = -1;
-  if (tid == 0) a.n_freed[b] = done;
+  for (int i = all + tid; i < a.MP; i += kEvictThreads) a.freed[base + i] = -1;
+  if (tid == 0) a.n_freed[b] = all;
 }
 
 namespace {
@@ -723,8 +855,17 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
   SCOPE_REQUIRE(k && v && table && lens, "%s: null pointer", fn);
   SCOPE_REQUIRE(aligned16(k) && aligned16(v) && k_sn % 8 == 0 && k_sh % 8 == 0 && v_sn % 8 == 0 && v_sh % 8 == 0,
                 "%s: the rows of k and v must be 16-byte aligned", fn);
-  const AppendArgs a{N, k_sn, k_sh, v_sn, v_sh, k, v, cu, table, lens, k_scale, v_scale, k_pages, v_pages};
-  hipLaunchKernelGGL(paged_append_kernel, dim3(ceil_div(N, 4)), dim3(256), 0, as_stream(stream), *c, a);
+  // a row a wavefront until 16 wavefronts a CU have work, then up to 8
+  const int rows = static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, N / 4096)));
+  const AppendArgs a{N, k_sn, k_sh, v_sn, v_sh, rows, k, v, cu, table, lens, k_scale, v_scale, k_pages, v_pages};
+  const dim3 grid(ceil_div(N, 4 * rows)), block(256);
+  hipStream_t st = as_stream(stream);
+  if (!c->fp8)  // (16-bit values are moved as they are)
+    hipLaunchKernelGGL((paged_append_kernel<SCOPE_BF16, false>), grid, block, 0, st, *c, a);
+  else if (c->type == SCOPE_BF16)
+    hipLaunchKernelGGL((paged_append_kernel<SCOPE_BF16, true>), grid, block, 0, st, *c, a);
+  else
+    hipLaunchKernelGGL((paged_append_kernel<SCOPE_FP16, true>), grid, block, 0, st, *c, a);
   return check_launch("paged_append_kernel");
 }
 
@@ -745,13 +886,13 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
   SCOPE_REQUIRE((kv_num != nullptr) == (kv_idx != nullptr) &&
                     (kv_idx ? maxkv >= 1 && static_cast<int64_t>(maxkv) * c->bs <= INT32_MAX : maxkv == 0),
                 "%s: kv_num and kv_idx come together, with 1 .. 2^31 / bs entries (maxkv=%d; 0 without lists)", fn, maxkv);
-  SCOPE_REQUIRE(q && table && lens && out && lse && work, "%s: null pointer", fn);
+  SCOPE_REQUIRE(q && table && lens && out && lse, "%s: null pointer", fn);
+  AttnSplit s;
+  SCOPE_REQUIRE(plan_split(*c, Hq, maxkv, mass != nullptr, &s, work) == 0 || work, "%s: null pointer (the workspace)", fn);
   SCOPE_REQUIRE(aligned16(q) && aligned16(work) && q_sb % 8 == 0 && q_sh % 8 == 0,
                 "%s: the rows of q and the workspace must be 16-byte aligned", fn);
   const PagedAttnArgs a{Hq,    maxkv, scale, q_sb,   q_sh,   q,    k_pages, v_pages, k_scale,
                         v_scale, table, lens,  first, kv_num, kv_idx, mass, out,     lse};
-  AttnSplit s;
-  plan_split(*c, Hq, maxkv, mass != nullptr, &s, work);
   const int G = Hq / c->Hkv, ng = (G + 15) / 16;
   const dim3 grid(s.slots, c->Hkv * ng);
   const size_t lds = sizeof(float) * kAttnWaves * (32 + static_cast<size_t>(std::min(G, 16)) * c->D);
@@ -802,7 +943,16 @@ int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, 
                 fn, window, n_global);
   SCOPE_REQUIRE(table && mass && lens && budget && table_out && freed && n_freed, "%s: null pointer", fn);
   const EvictArgs a{B, Hkv, MP, bs, window, n_global, table, mass, lens, budget, table_out, freed, n_freed};
-  hipLaunchKernelGGL(paged_evict_kernel, dim3(B), dim3(kEvictThreads), 0, as_stream(stream), a);
+  const dim3 grid(B), block(kEvictThreads);
+  hipStream_t st = as_stream(stream);
+  if (MP <= kEvictThreads)
+    hipLaunchKernelGGL(paged_evict_kernel<1>, grid, block, 0, st, a);
+  else if (MP <= 4 * kEvictThreads)
+    hipLaunchKernelGGL(paged_evict_kernel<4>, grid, block, 0, st, a);
+  else if (MP <= 16 * kEvictThreads)
+    hipLaunchKernelGGL(paged_evict_kernel<16>, grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL(paged_evict_kernel<64>, grid, block, 0, st, a);
   return check_launch("paged_evict_kernel");
 }
 

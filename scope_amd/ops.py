@@ -6,6 +6,7 @@ GPU tensors; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import threading
 
@@ -1111,6 +1112,23 @@ _FP8 = torch.float8_e4m3fn
 EVICT_MAX_PAGES = 65536  # include/scope_amd.h SCOPE_PAGED_EVICT_MAX_PAGES
 
 
+def _device(who: str, first: torch.Tensor, *ts: torch.Tensor | None) -> torch.device:
+    """``_gpu`` for calls of a few microseconds: device indices are compared, and
+    only a call that fails the comparison looks closer."""
+    index = first.get_device()
+    if index < 0:
+        return _gpu(who, first, *ts)
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            return _gpu(who, first, *ts)
+    return first.device
+
+
+def _ptr(t: torch.Tensor | None):
+    """The address of a tensor that the caller holds until its call returns."""
+    return None if t is None else t.data_ptr()
+
+
 def _call_on(dev: torch.device, name: str, *args) -> None:
     """``call`` with ``dev`` as the current device (a launch takes the current
     device's kernels, whatever device its stream is on)."""
@@ -1127,31 +1145,41 @@ def _ints(who: str, name: str, x, n: int, dev: torch.device) -> torch.Tensor | N
         return None
     if not isinstance(x, torch.Tensor):
         return torch.full((n,), int(x), dtype=torch.int32, device=dev)
-    if x.numel() != n or x.dtype not in (torch.int32, torch.int64):
+    dt = x.dtype
+    if x.numel() != n or (dt != torch.int32 and dt != torch.int64):
         raise RuntimeError(f"{who}: {name} must be int32 or int64 [{n}] (got {x.dtype} {tuple(x.shape)})")
-    return _i32(x)
+    return x if dt == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_work_bytes(B: int, Hkv: int, D: int, bs: int, MP: int, Hq: int, maxkv: int, with_mass: bool) -> int:
+    """The attention's workspace, a function of these sizes alone."""
+    c = _lib.PagedCache(B, Hkv, D, bs, MP)
+    return query("scope_paged_attn_workspace_bytes", C.byref(c), Hq, maxkv, int(with_mass))
 
 
 def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, dtype: torch.dtype,
                  k_scale, v_scale) -> "_lib.PagedCache":
     """The C description of a cache, its tensors checked."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    shape, pt = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or pt != v_pages.dtype:
         raise RuntimeError(f"{who}: k_pages and v_pages must be [P, Hkv, bs, D] of one shape and type")
-    fp8 = k_pages.dtype == _FP8
-    if dtype not in (torch.bfloat16, torch.float16) or not (fp8 or k_pages.dtype == dtype):
+    fp8 = pt == _FP8
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or not (fp8 or pt == dtype):
         raise RuntimeError(f"{who}: bfloat16 or float16 rows with pages of their type or float8_e4m3fn "
-                           f"(got {dtype} and {k_pages.dtype})")
+                           f"(got {dtype} and {pt})")
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP]")
-    P, Hkv, bs, D = k_pages.shape
+    P, Hkv, bs, D = shape
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
         if t is not None and (not fp8 or t.dtype != torch.float32 or t.numel() != Hkv or not t.is_contiguous()):
             raise RuntimeError(f"{who}: {name} must be a contiguous float32 [{Hkv}], with float8_e4m3fn pages")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if ks[3] != 1 or vs[3] != 1:
+    kp, kh, kr, kd = k_pages.stride()
+    vp, vh, vr, vd = v_pages.stride()
+    if kd != 1 or vd != 1:
         raise RuntimeError(f"{who}: the pages' last dimension must be contiguous")
     B, MP = table.shape
-    return _lib.PagedCache(B, Hkv, D, bs, MP, _PAGED_TYPES[dtype], int(fp8), P, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+    return _lib.PagedCache(B, Hkv, D, bs, MP, _PAGED_TYPES[dtype], fp8, P, kp, kh, kr, vp, vh, vr)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -1169,18 +1197,20 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     sequence, past the table, or of a block whose entry is outside [0, P) are
     not written; no two rows may share a slot."""
     who = "paged_append"
-    dev = _gpu(who, k, v, k_pages, v_pages, table, lens, cu, k_scale, v_scale)
-    c = _paged_cache(who, k_pages, v_pages, table, k.dtype, k_scale, v_scale)
-    if k.dim() != 3 or k.shape != v.shape or v.dtype != k.dtype or k.shape[1] != c.Hkv or k.shape[2] != c.D \
-            or k.stride(2) != 1 or v.stride(2) != 1:
+    dev = _device(who, k, v, k_pages, v_pages, table, lens, cu, k_scale, v_scale)
+    dtype, shape, ks, vs = k.dtype, k.shape, k.stride(), v.stride()
+    c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)
+    if len(shape) != 3 or shape != v.shape or v.dtype != dtype or shape[1] != c.Hkv or shape[2] != c.D or ks[2] != 1 or vs[2] != 1:
         raise RuntimeError(f"{who}: k and v must be [N, {c.Hkv}, {c.D}] of one type with a contiguous last dimension")
-    for n_, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-            raise RuntimeError(f"{who}: {n_} is an expanded tensor: its rows share memory")
+    if not (c.k_sp and c.k_sh and c.k_sr and c.v_sp and c.v_sh and c.v_sr):
+        for t in (k_pages, v_pages):
+            if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise RuntimeError(f"{who}: the pages are an expanded tensor: their rows share memory")
     lens = _ints(who, "lens", lens, c.B, dev)
     cu = _ints(who, "cu", cu, c.B + 1, dev)
-    _call_on(dev, "scope_paged_append", C.byref(c), k.shape[0], _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
-             v.stride(1), _p(cu), _p(table), _p(lens), _p(k_scale), _p(v_scale), _p(k_pages), _p(v_pages), _stream(dev))
+    _call_on(dev, "scope_paged_append", C.byref(c), shape[0], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+             _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(),
+             v_pages.data_ptr(), _stream(dev))
 
 
 def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -1204,31 +1234,32 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     Nothing of it waits for the GPU or reads a length on the host, so a call
     can be captured and replayed while the lengths and the table change."""
     who = "paged_decode_attn"
-    dev = _gpu(who, q, k_pages, v_pages, table, lens, first, kv_num, kv_idx, mass, k_scale, v_scale)
-    c = _paged_cache(who, k_pages, v_pages, table, q.dtype, k_scale, v_scale)
-    if q.dim() != 3 or q.shape[0] != c.B or q.shape[2] != c.D or q.shape[1] % c.Hkv or q.shape[1] < 1 or q.stride(2) != 1:
-        raise RuntimeError(f"{who}: q must be [{c.B}, a multiple of {c.Hkv}, {c.D}] with a contiguous last dimension "
-                           f"(got {tuple(q.shape)})")
-    B, Hq, D = q.shape
-    maxkv = 0
-    if (kv_num is None) != (kv_idx is None):
-        raise RuntimeError(f"{who}: kv_num and kv_idx come together")
-    if kv_idx is not None:
-        maxkv = kv_idx.shape[-1]
-        if kv_idx.dim() != 3 or maxkv < 1 or kv_idx.shape[:2] != (B, c.Hkv) or kv_num.shape != (B, c.Hkv):
-            raise RuntimeError(f"{who}: kv_num must be [{B}, {c.Hkv}] and kv_idx [{B}, {c.Hkv}, maxkv]")
+    dev = _device(who, q, k_pages, v_pages, table, lens, first, kv_num, kv_idx, mass, k_scale, v_scale)
+    shape, qs, dtype = q.shape, q.stride(), q.dtype
+    c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)
+    B, Hkv, D, MP = c.B, c.Hkv, c.D, c.MP
+    if len(shape) != 3 or shape[0] != B or shape[2] != D or shape[1] % Hkv or shape[1] < 1 or qs[2] != 1:
+        raise RuntimeError(f"{who}: q must be [{B}, a multiple of {Hkv}, {D}] with a contiguous last dimension "
+                           f"(got {tuple(shape)})")
+    Hq, maxkv = shape[1], 0
+    if kv_num is not None or kv_idx is not None:
+        if kv_num is None or kv_idx is None:
+            raise RuntimeError(f"{who}: kv_num and kv_idx come together")
+        if kv_idx.dim() != 3 or kv_idx.shape[2] < 1 or kv_idx.shape[:2] != (B, Hkv) or kv_num.shape != (B, Hkv):
+            raise RuntimeError(f"{who}: kv_num must be [{B}, {Hkv}] and kv_idx [{B}, {Hkv}, maxkv]")
+        maxkv = kv_idx.shape[2]
         kv_num, kv_idx = _i32(kv_num), _i32(kv_idx)
-    if mass is not None and (mass.dtype != torch.float32 or mass.shape != (B, c.Hkv, c.MP) or not mass.is_contiguous()):
-        raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, {c.Hkv}, {c.MP}]")
+    if mass is not None and (mass.dtype != torch.float32 or mass.shape != (B, Hkv, MP) or not mass.is_contiguous()):
+        raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, {Hkv}, {MP}]")
     lens = _ints(who, "lens", lens, B, dev)
     first = _ints(who, "first", first, B, dev)
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
-    need = query("scope_paged_attn_workspace_bytes", C.byref(c), Hq, maxkv, int(mass is not None))
-    work = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), _p(q), q.stride(0), q.stride(1),
-             _p(k_pages), _p(v_pages), _p(k_scale), _p(v_scale), _p(table), _p(lens), _p(first), _p(kv_num), _p(kv_idx),
-             _p(mass), _p(work), _p(out), _p(lse), _stream(dev))
+    out = torch.empty(shape, dtype=dtype, device=dev)
+    lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
+    need = _paged_work_bytes(B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, scale, q.data_ptr(), qs[0], qs[1], k_pages.data_ptr(),
+             v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _ptr(first),
+             _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr(), _stream(dev))
     return out, lse
 
 
@@ -1246,22 +1277,23 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     table has -1 in their place (a new tensor, or ``out``, which may be the
     table itself); freed holds their pages in the blocks' order, then -1."""
     who = "paged_evict"
-    dev = _gpu(who, table, mass, lens, budget if isinstance(budget, torch.Tensor) else None, out)
+    dev = _device(who, table, mass, lens, budget if isinstance(budget, torch.Tensor) else None, out)
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
         raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP]")
     B, MP = table.shape
-    if mass.dtype != torch.float32 or mass.dim() != 3 or mass.shape[0] != B or mass.shape[2] != MP or not mass.is_contiguous():
+    ms = mass.shape
+    if mass.dtype != torch.float32 or len(ms) != 3 or ms[0] != B or ms[2] != MP or not mass.is_contiguous():
         raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, Hkv, {MP}]")
     if out is None:
-        out = torch.empty_like(table)
+        out = torch.empty((B, MP), dtype=torch.int32, device=dev)
     elif out.dtype != torch.int32 or out.shape != table.shape or not out.is_contiguous():
         raise RuntimeError(f"{who}: out must be a contiguous int32 [{B}, {MP}]")
     lens = _ints(who, "lens", lens, B, dev)
     budget = _ints(who, "budget", budget, B, dev)
     freed = torch.empty((B, MP), dtype=torch.int32, device=dev)
     n_freed = torch.empty(B, dtype=torch.int32, device=dev)
-    _call_on(dev, "scope_paged_evict", B, mass.shape[1], MP, int(bs), int(window), int(n_global), _p(table), _p(mass),
-             _p(lens), _p(budget), _p(out), _p(freed), _p(n_freed), _stream(dev))
+    _call_on(dev, "scope_paged_evict", B, ms[1], MP, bs, window, n_global, table.data_ptr(), mass.data_ptr(),
+             lens.data_ptr(), budget.data_ptr(), out.data_ptr(), freed.data_ptr(), n_freed.data_ptr(), _stream(dev))
     return out, freed, n_freed
 
 
@@ -1287,50 +1319,51 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
     repetition and temperature must be positive (numbers are checked).
     ``out`` may be the logits themselves."""
     who = "logit_penalties"
-    dev = _gpu(who, logits, tokens, bias, mask, out,
-               *(x for x in (lens, first, n_prompt, repetition, presence, frequency, temperature) if isinstance(x, torch.Tensor)))
-    if logits.dtype not in _PAGED_TYPES or logits.dim() not in (1, 2) or logits.stride(-1) != 1 or logits.numel() < 1:
+    numbers = (repetition, presence, frequency, temperature)
+    dev = _device(who, logits, tokens, bias, mask, out,
+                  *(x for x in (lens, first, n_prompt, *numbers) if isinstance(x, torch.Tensor)))
+    zd, shape, dtype = logits.dim(), logits.shape, logits.dtype
+    if dtype not in _PAGED_TYPES or not 1 <= zd <= 2 or logits.stride(-1) != 1 or logits.numel() < 1:
         raise RuntimeError(f"{who}: logits must be fp32, bf16 or fp16 [B, V] or [V] with contiguous rows")
-    V = logits.shape[-1]
-    B = logits.shape[0] if logits.dim() == 2 else 1
-
-    def row_stride(x):
-        return x.stride(0) if x.dim() == 2 else 0
-
-    if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() not in (1, 2) \
-            or (tokens.dim() == 2 and tokens.shape[0] != B) or (tokens.shape[-1] > 1 and tokens.stride(-1) != 1):
+    V, B = shape[-1], shape[0] if zd == 2 else 1
+    T, td = tokens.shape[-1] if tokens.dim() else 0, tokens.dim()
+    if (tokens.dtype != torch.int64 and tokens.dtype != torch.int32) or not 1 <= td <= 2 \
+            or (td == 2 and tokens.shape[0] != B) or (T > 1 and tokens.stride(-1) != 1):
         raise RuntimeError(f"{who}: tokens must be int32 or int64 [{B}, T] or [T] with contiguous rows")
+    W = (V + 31) // 32
     if bias is not None and (bias.dtype != torch.float32 or bias.shape not in ((V,), (B, V)) or bias.stride(-1) != 1):
         raise RuntimeError(f"{who}: bias must be float32 [{V}] or [{B}, {V}] with contiguous rows")
-    W = (V + 31) // 32
     if mask is not None and (mask.dtype != torch.int32 or mask.shape not in ((W,), (B, W)) or mask.stride(-1) != 1):
         raise RuntimeError(f"{who}: mask must be int32 [{W}] or [{B}, {W}] with contiguous rows")
     if out is None:
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    elif out.dtype != logits.dtype or out.shape != logits.shape or out.stride(-1) != 1 or (B > 1 and out.stride(0) < V) \
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    elif out.dtype != dtype or out.shape != shape or out.stride(-1) != 1 or (B > 1 and out.stride(0) < V) \
             or (out.data_ptr() == logits.data_ptr() and B > 1 and out.stride(0) != logits.stride(0)):
         raise RuntimeError(f"{who}: out must have the logits' shape and type, rows of its own, and their strides if it is them")
-    num, arr = {}, {}
-    for name, x, positive in (("repetition", repetition, True), ("presence", presence, False),
-                              ("frequency", frequency, False), ("temperature", temperature, True)):
+    num, arr = [], []
+    for name, x in zip(("repetition", "presence", "frequency", "temperature"), numbers):
         if isinstance(x, torch.Tensor):
             if x.numel() != B or not x.is_floating_point():
                 raise RuntimeError(f"{who}: {name} must be a number or a float tensor [{B}]")
-            num[name], arr[name] = 0.0, _f32(x)
+            num.append(0.0)
+            arr.append(_f32(x))
         else:
+            positive = name == "repetition" or name == "temperature"
             if not math.isfinite(x) or (positive and x <= 0):
                 raise ValueError(f"{who}: {name} must be finite{' and positive' if positive else ''}, got {x}")
-            num[name], arr[name] = float(x), None
-    if isinstance(lens, torch.Tensor) and lens.dtype == torch.int64 and lens.numel() == B and lens.is_contiguous():
-        lens64 = 1
-    else:
-        lens, lens64 = _ints(who, "lens", lens, B, dev), 0
+            num.append(x)
+            arr.append(None)
+    lens64 = isinstance(lens, torch.Tensor) and lens.dtype == torch.int64 and lens.numel() == B and lens.is_contiguous()
+    if not lens64:
+        lens = _ints(who, "lens", lens, B, dev)
     first, n_prompt = _ints(who, "first", first, B, dev), _ints(who, "n_prompt", n_prompt, B, dev)
-    prm = _lib.PenaltyParams(B, _PAGED_TYPES[logits.dtype], int(tokens.dtype == torch.int64), lens64, V, tokens.shape[-1],
-                             row_stride(logits), row_stride(out), row_stride(tokens),
-                             row_stride(bias) if bias is not None else 0, row_stride(mask) if mask is not None else 0, **num)
-    _call_on(dev, "scope_logit_penalties", C.byref(prm), _p(logits), _p(tokens), _p(lens), _p(first), _p(n_prompt),
-             *(_p(x) for x in arr.values()), _p(bias), _p(mask), _p(out), _stream(dev))
+    prm = _lib.PenaltyParams(B, _PAGED_TYPES[dtype], tokens.dtype == torch.int64, lens64, V, T,
+                             logits.stride(0) if zd == 2 else 0, out.stride(0) if zd == 2 else 0,
+                             tokens.stride(0) if td == 2 else 0, bias.stride(0) if bias is not None and bias.dim() == 2 else 0,
+                             mask.stride(0) if mask is not None and mask.dim() == 2 else 0, *num)
+    _call_on(dev, "scope_logit_penalties", C.byref(prm), logits.data_ptr(), tokens.data_ptr(), lens.data_ptr(),
+             _ptr(first), _ptr(n_prompt), _ptr(arr[0]), _ptr(arr[1]), _ptr(arr[2]), _ptr(arr[3]), _ptr(bias), _ptr(mask),
+             out.data_ptr(), _stream(dev))
     return out
 
 

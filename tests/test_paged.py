@@ -173,7 +173,7 @@ def test_library_refuses_before_any_launch():
                      ("null pages", dict(pages=None)), ("multiple", dict(Hq=3)), ("multiple", dict(Hq=0)),
                      ("multiple", dict(Hq=65536)), ("kv_num", dict(num=one)), ("kv_num", dict(idx=one, maxkv=3)),
                      ("kv_num", dict(num=one, idx=one)), ("kv_num", dict(maxkv=3)), ("kv_num", dict(num=one, idx=one, maxkv=2 ** 26)),
-                     ("null pointer", dict(q=None)), ("null pointer", dict(work=None)), ("aligned", dict(q_sb=516)),
+                     ("null pointer", dict(q=None)), ("null pointer", dict(work=None, MP=4096)), ("aligned", dict(q_sb=516)),
                      ("aligned", dict(q=C.c_void_p(24))), ("aligned", dict(work=C.c_void_p(8)))):
         attn(word, **kw)
 
