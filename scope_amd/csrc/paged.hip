@@ -146,8 +146,15 @@ struct PagedAttnArgs {
 // blockIdx.x, (key head, group of 16 query heads) blockIdx.y.
 constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = 64 * kAttnWaves;
-constexpr int kPieces = 1024;     // workgroups aimed at
-constexpr int kPieceTiles = 16;   // a piece's least tiles: 4 a wavefront
+constexpr int kPieceTiles = 2;  // a piece's least tiles
+
+// Workgroups aimed at.  One sequence's pieces are equal and 1024 fill the device
+// evenly (131k positions, 8 heads: 103 us; 1536: 107, 768: 112).  The pieces of a
+// ragged batch are not, and smaller ones even out its end (64 query heads over 24
+// sequences of 9k to 65k: 1536 269 us, 1024 280), except at D = 256, whose partial
+// rows are longer (16 sequences to 16k: 1024 120 us, 1536 123).
+constexpr int kMostPieces = 1536;
+constexpr int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
 
 struct AttnSplit {
   int pieces, slots;   // pieces aimed at and slots of a (key head, group); with lists: pieces of every list
@@ -155,7 +162,7 @@ struct AttnSplit {
   float* po;           // [slots][Hq][D] partial P·V, unnormalised
   float* pml;          // [slots][Hq][2] their maxima (log2 units) and sums
   int2* plan;          // [B] (pieces, first slot) of each sequence
-  float* lse2;         // [B][Hq] log2 of the whole sums, for the mass
+  float* lse2;         // [B][Hq] log2 of the whole sums of rows in one piece, for the mass
   float* tile_lse;     // [B][Hq][tiles_cap][halves] log2 of each tile's (half tile's) sum, for the mass
 };
 
@@ -244,6 +251,21 @@ struct Words {
   uint32_t w[N];
 };
 
+// N words that are read once: they are not kept in the caches in front of others
+template <int N>
+__device__ __forceinline__ Words<N> load_once(const char* p) {
+  Words<N> x;
+  if constexpr (N == 1) {
+    x.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  } else {
+    typedef uint32_t words_t __attribute__((ext_vector_type(N), aligned(4)));
+    const words_t v = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(p));
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.w[i] = v[i];
+  }
+  return x;
+}
+
 // The attention of one new token.  For a tile of 32 keys and 16 query heads of
 // one key head (those past the group are zero), with lane l, g = l / 16, c = l % 16:
 //   S^T = K·Q^T   two products; operand A's row m is key 8(m/4) + 4t + m%4 of
@@ -277,14 +299,13 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
   Piece p;
   int n_list = 0;
   if (lists) {
+    // pieces of one length for every list, so that the list is read without waiting for its number
     p.b = blockIdx.x / s.pieces;
     p.i = blockIdx.x % s.pieces;
     p.n = s.pieces;
     p.slot = p.b * s.pieces;
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
-    // pieces of one length for every list, so that the join knows which there are
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
-    p.t1 = min(p.t1, static_cast<int>((static_cast<int64_t>(n_list) * c.bs + kTileKeys - 1) / kTileKeys));
   } else if (!find_piece(c, a, s, blockIdx.x, p)) {
     return;
   }
@@ -322,14 +343,10 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
   int pg0 = -1, pg1 = -1, lb0 = 0, lb1 = 0;
   const auto resolve = [&](int t) {
     const auto one = [&](int64_t e, int& lb) -> int {  // entry e of the list, or block e
-      int64_t blk = e;
-      if (lists) {
-        if (e >= n_list) return -1;
-        blk = list[e];
-      }
+      const int64_t blk = !lists ? e : e < a.maxkv ? list[e] : -1;
       const int64_t page = block_page(row, c.MP, blk, c.P);
       lb = page < 0 ? 0 : static_cast<int>(blk);
-      return static_cast<int>(page);
+      return lists && e >= n_list ? -1 : static_cast<int>(page);
     };
     pg0 = pg1 = -1;
     lb0 = lb1 = 0;
@@ -340,16 +357,21 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
     }
   };
 
-  int u = 64;
+  resolve(p.t0 + wave + lane * kAttnWaves);
+  if (lists) p.t1 = min(p.t1, static_cast<int>((static_cast<int64_t>(n_list) * c.bs + kTileKeys - 1) / kTileKeys));
+  int u = 0;
   for (int t = p.t0 + wave; t < p.t1; t += kAttnWaves, ++u) {
     if (u == 64) {
       resolve(t + lane * kAttnWaves);
       u = 0;
     }
     const int page0 = __builtin_amdgcn_readlane(pg0, u), page1 = small ? __builtin_amdgcn_readlane(pg1, u) : page0;
-    const int64_t stat = s.tile_lse ? (((static_cast<int64_t>(b) * a.Hq + h0 + c16) * s.tiles_cap + t) << small) : 0;
+    const auto put_sum = [&](float x) {  // log2 of the tile's sum (of this lane's half of it)
+      if (c16 < nq && (g4 & (small ? 1 : 3)) == 0)
+        s.tile_lse[(((static_cast<int64_t>(b) * a.Hq + h0 + c16) * s.tiles_cap + t) << small) + (small ? g4 >> 1 : 0)] = x;
+    };
     if (page0 < 0 && page1 < 0) {  // nothing to see
-      if (s.tile_lse && c16 < nq && (g4 & (small ? 1 : 3)) == 0) s.tile_lse[stat + (small ? g4 >> 1 : 0)] = -INFINITY;
+      if (s.tile_lse) put_sum(-INFINITY);
       continue;
     }
     const int r0 = small ? 0 : (t * kTileKeys) & (c.bs - 1);  // the tile's first row in its page
@@ -363,10 +385,12 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
 #pragma unroll
       for (int j = 0; j < KV; ++j) kf[i][j] = *reinterpret_cast<const uint4*>(kr + 4 * i * c.k_sr * ES + j * 64);
     Words<VW> vf[NH][8];
+    const auto load_v = [&](int h) {
 #pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vf[h][i] = *reinterpret_cast<const Words<VW>*>(vr + (i * c.v_sr + h * 128) * ES);
+      for (int i = 0; i < 8; ++i) vf[h][i] = load_once<VW>(vr + (i * c.v_sr + h * 128) * ES);
+    };
+    load_v(0);
+    __builtin_amdgcn_sched_barrier(0);  // all loads are under way before the first is waited for
 
     // scores
     f32x4_t sc[2];
@@ -384,6 +408,10 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
           sc[i] = mfma_16<TYPE>(kf[i][j], qf[j], sc[i]);
         }
       }
+    }
+    if constexpr (NH > 1) {  // D = 256: into K's registers, which are free by now
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(1);
     }
     float x[8];
 #pragma unroll
@@ -428,7 +456,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
     if (s.tile_lse) {
       lt += __shfl_xor(lt, 16, kWave);
       if (!small) lt += __shfl_xor(lt, 32, kWave);
-      if (c16 < nq && (g4 & (small ? 1 : 3)) == 0) s.tile_lse[stat + (small ? g4 >> 1 : 0)] = ref + __builtin_amdgcn_logf(lt);
+      put_sum(ref + __builtin_amdgcn_logf(lt));
     }
     const uint4 pf = make_uint4(round2<TYPE>(x[0], x[1]), round2<TYPE>(x[2], x[3]), round2<TYPE>(x[4], x[5]),
                                 round2<TYPE>(x[6], x[7]));
@@ -446,11 +474,11 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
         }
 #pragma unroll
       for (int j = 0; j < VE; ++j) {
-        uint32_t o[4];
+        uint32_t op[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-          o[w] = j % 2 ? pack_hi16(v[2 * w][j / 2], v[2 * w + 1][j / 2]) : pack_lo16(v[2 * w][j / 2], v[2 * w + 1][j / 2]);
-        acc[h * VE + j] = mfma_16<TYPE>(make_uint4(o[0], o[1], o[2], o[3]), pf, acc[h * VE + j]);
+          op[w] = j % 2 ? pack_hi16(v[2 * w][j / 2], v[2 * w + 1][j / 2]) : pack_lo16(v[2 * w][j / 2], v[2 * w + 1][j / 2]);
+        acc[h * VE + j] = mfma_16<TYPE>(make_uint4(op[0], op[1], op[2], op[3]), pf, acc[h * VE + j]);
       }
     }
   }
@@ -510,101 +538,131 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
   }
 }
 
-// The pieces of one (sequence, query head) joined: relative to the largest of
-// their maxima, sixteen bytes of the output row a thread, the pieces shared out
-// over the groups of threads.
-template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
-  const int b = blockIdx.x, h = blockIdx.y;
-  const bool lists = a.kv_idx != nullptr;
-  const int2 plan = lists ? make_int2(s.pieces, b * s.pieces) : s.plan[b];
-  const int n = plan.x;
-  if (n == 1) return;  // written by its only piece
-  constexpr int LD = D / 4, NG = 256 / LD;
-  __shared__ float w[kPieces], red[2][4], so[NG][D];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float* ml = s.pml + (static_cast<int64_t>(plan.y) * a.Hq + h) * 2;
-  float M = -INFINITY;
-  for (int i = tid; i < n; i += 256) M = fmaxf(M, ml[static_cast<int64_t>(i) * a.Hq * 2]);
+// (maximum, sum relative to it) of a row from its n pieces' (maximum, sum) pairs,
+// `step` floats apart: by one wavefront, the same in every lane; the first pair
+// of each lane is read once.
+__device__ __forceinline__ float2 join_sums(const float* ml, int n, int64_t step) {
+  const int lane = threadIdx.x & 63;
+  float m0 = -INFINITY, l0 = 0.f;
+  if (lane < n) {
+    m0 = ml[lane * step];
+    l0 = ml[lane * step + 1];
+  }
+  float M = m0;
+  for (int i = lane + 64; i < n; i += 64) M = fmaxf(M, ml[i * step]);
   M = wave_max_f32(M);
-  if (lane == 0) red[0][wave] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  float L = 0.f;
-  for (int i = tid; i < n; i += 256) {
-    const float mi = ml[static_cast<int64_t>(i) * a.Hq * 2], li = ml[static_cast<int64_t>(i) * a.Hq * 2 + 1];
-    const float f = li == 0.f ? 0.f : __builtin_amdgcn_exp2f(mi - M);
-    w[i] = f;
-    L += f * li;
+  float L = l0 == 0.f ? 0.f : __builtin_amdgcn_exp2f(m0 - M) * l0;
+  for (int i = lane + 64; i < n; i += 64) {
+    const float li = ml[i * step + 1];
+    L += li == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i * step] - M) * li;
   }
   for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, kWave);
-  if (lane == 0) red[1][wave] = L;
-  __syncthreads();
-  L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  const int dl = tid % LD, grp = tid / LD;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float* po = s.po + (static_cast<int64_t>(plan.y) * a.Hq + h) * D + 4 * dl;
-  for (int i = grp; i < n; i += NG) {
-    const float4 v = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(i) * a.Hq * D);
-    const float f = w[i];
-    acc.x += f * v.x;
-    acc.y += f * v.y;
-    acc.z += f * v.z;
-    acc.w += f * v.w;
-  }
-  *reinterpret_cast<float4*>(&so[grp][4 * dl]) = acc;
-  __syncthreads();
-  if (tid < D) {
-    float o = 0.f;
-#pragma unroll
-    for (int i = 0; i < NG; ++i) o += so[i][tid];
-    const float y = L == 0.f ? 0.f : o / L * (a.v_scale ? a.v_scale[h / (a.Hq / c.Hkv)] : 1.f);
-    a.out[(static_cast<int64_t>(b) * a.Hq + h) * D + tid] = c.type == SCOPE_FP16 ? f32_to_half(y) : f32_to_bf16(y);
-    if (tid == 0) {
-      const float e = L == 0.f ? -INFINITY : M + __builtin_amdgcn_logf(L);
-      a.lse[static_cast<int64_t>(b) * a.Hq + h] = e * kLn2;
-      if (s.lse2) s.lse2[static_cast<int64_t>(b) * a.Hq + h] = e;
-    }
-  }
+  return make_float2(M, L);
 }
 
-// Every block's probabilities, from its tiles' sums and the rows' whole ones:
-// one thread per listed block (or block of the sequence), its heads and tiles in
-// order.
-__global__ __launch_bounds__(256) void paged_mass_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
-  const int b = blockIdx.x, hk = blockIdx.y, G = a.Hq / c.Hkv;
-  const int64_t e = static_cast<int64_t>(blockIdx.z) * 256 + threadIdx.x, bh = static_cast<int64_t>(b) * c.Hkv + hk;
-  const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
-  int64_t lb = e;
+// What follows the pieces, for (sequence, key head) (blockIdx.z, blockIdx.y).
+// Workgroup x joins the pieces of the group's query head x, sixteen bytes of the
+// output row a thread, the pieces shared out over groups of threads; and with a
+// mass adds 256 blocks' probabilities, formed from their tiles' sums and the
+// rows' whole ones, a block a thread, its heads and tiles in order.  Both in one
+// launch: a second one costs more than the sums joined anew (4.7 us).
+template <int D>
+__global__ __launch_bounds__(256) void paged_finish_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
+  const int b = blockIdx.z, hk = blockIdx.y, x = blockIdx.x, G = a.Hq / c.Hkv;
+  const bool lists = a.kv_idx != nullptr;
+  constexpr int LD = D / 4, NG = 256 / LD;
+  __shared__ float w[kMostPieces], so[NG][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int2 plan = make_int2(1, 0);
+  if (s.po) plan = lists ? make_int2(s.pieces, b * s.pieces) : s.plan[b];
+  const int n = plan.x;
+  const int64_t step = 2ll * a.Hq;
+  const float* ml0 = s.pml + (static_cast<int64_t>(plan.y) * a.Hq + hk * G) * 2;  // of the group's first head
+  if (x < G && n > 1) {  // (a sequence in one piece is written by it)
+    const int h = hk * G + x;
+    const float* ml = ml0 + 2 * x;
+    const int dl = tid % LD, grp = tid / LD;
+    const float* po = s.po + (static_cast<int64_t>(plan.y) * a.Hq + h) * D + 4 * dl;
+    const int64_t row = static_cast<int64_t>(a.Hq) * D;
+    // the first rows of each group are under way while the sums are formed
+    constexpr int EARLY = 4;
+    float4 v[EARLY];
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) v[k] = *reinterpret_cast<const float4*>(po + min(grp + k * NG, n - 1) * row);
+    const float2 ML = join_sums(ml, n, step);
+    for (int i = tid; i < n; i += 256) w[i] = ml[i * step + 1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i * step] - ML.x);
+    __syncthreads();
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](const float4& r, float f) {
+      acc.x += f * r.x;
+      acc.y += f * r.y;
+      acc.z += f * r.z;
+      acc.w += f * r.w;
+    };
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k)
+      if (grp + k * NG < n) add(v[k], w[grp + k * NG]);
+#pragma unroll 4
+    for (int i = grp + EARLY * NG; i < n; i += NG) add(*reinterpret_cast<const float4*>(po + i * row), w[i]);
+    *reinterpret_cast<float4*>(&so[grp][4 * dl]) = acc;
+    __syncthreads();
+    if (tid < D) {
+      float o = 0.f;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) o += so[i][tid];
+      const float y = ML.y == 0.f ? 0.f : o / ML.y * (a.v_scale ? a.v_scale[hk] : 1.f);
+      a.out[(static_cast<int64_t>(b) * a.Hq + h) * D + tid] = c.type == SCOPE_FP16 ? f32_to_half(y) : f32_to_bf16(y);
+      if (tid == 0)
+        a.lse[static_cast<int64_t>(b) * a.Hq + h] = ML.y == 0.f ? -INFINITY : (ML.x + __builtin_amdgcn_logf(ML.y)) * kLn2;
+    }
+  }
+  const int blocks = lists ? a.maxkv : c.MP;
+  if (!a.mass || static_cast<int64_t>(x) * 256 >= blocks) return;
+  const int64_t e = static_cast<int64_t>(x) * 256 + tid, bh = static_cast<int64_t>(b) * c.Hkv + hk;
+  int64_t lb = -1;
   int lo = 0;
   int64_t hi;
-  if (a.kv_idx) {
-    const int n = min(max(a.kv_num[bh], 0), a.maxkv);
-    if (e >= n) return;
-    lb = a.kv_idx[bh * a.maxkv + e];
-    hi = (static_cast<int64_t>(n) * c.bs + kTileKeys - 1) / kTileKeys;
+  if (lists) {
+    const int num = min(max(a.kv_num[bh], 0), a.maxkv);
+    if (e < num) lb = a.kv_idx[bh * a.maxkv + e];
+    hi = (static_cast<int64_t>(num) * c.bs + kTileKeys - 1) / kTileKeys;
   } else {
-    const int tiles = seq_tiles(a.lens[b], a.first ? a.first[b] : 0, cap, &lo);
-    hi = lo + tiles;
+    if (e < blocks) lb = e;
+    hi = seq_tiles(a.lens[b], a.first ? a.first[b] : 0, static_cast<int64_t>(c.MP) * c.bs, &lo);
+    hi += lo;
   }
-  if (lb < 0 || lb >= c.MP) return;
   // the block's tiles (half tiles of blocks of 16) among those that were formed
   const int halves = c.bs == 16 ? 2 : 1, per = c.bs == 16 ? 1 : c.bs / kTileKeys;
   const int64_t u0 = max(e * per, static_cast<int64_t>(lo) * halves), u1 = min((e + 1) * per, hi * halves);
-  if (u0 >= u1) return;
-  float w = 0.f;
-  for (int g = 0; g < G; ++g) {
-    const int64_t h = static_cast<int64_t>(b) * a.Hq + hk * G + g;
-    const float all = s.lse2[h];
-    if (all == -INFINITY) continue;
-    const float* t = s.tile_lse + h * s.tiles_cap * halves;
-    for (int64_t u = u0; u < u1; ++u) w += __builtin_amdgcn_exp2f(t[u] - all);
+  const bool live = lb >= 0 && lb < c.MP && u0 < u1;
+  float sum = 0.f;
+  for (int g0 = 0; g0 < G; g0 += 256) {
+    __syncthreads();
+    const int ng = min(256, G - g0);
+    for (int g = wave; g < ng; g += 4) {  // log2 of the heads' whole sums
+      float all;
+      if (n > 1) {
+        const float2 ML = join_sums(ml0 + 2 * (g0 + g), n, step);
+        all = ML.y == 0.f ? -INFINITY : ML.x + __builtin_amdgcn_logf(ML.y);
+      } else {
+        all = s.lse2[static_cast<int64_t>(b) * a.Hq + hk * G + g0 + g];
+      }
+      if (lane == 0) w[g] = all;
+    }
+    __syncthreads();
+    for (int g = 0; g < ng && live; ++g) {
+      const float all = w[g];
+      if (all == -INFINITY) continue;
+      const float* t = s.tile_lse + (static_cast<int64_t>(b) * a.Hq + hk * G + g0 + g) * s.tiles_cap * halves;
+      for (int64_t u = u0; u < u1; ++u) sum += __builtin_amdgcn_exp2f(t[u] - all);
+    }
   }
+  if (!live) return;
   // (a list may name a block once; an atomic for the lists that break this)
-  if (a.kv_idx)
-    atomicAdd(a.mass + bh * c.MP + lb, w);
+  if (lists)
+    atomicAdd(a.mass + bh * c.MP + lb, sum);
   else
-    a.mass[bh * c.MP + lb] += w;
+    a.mass[bh * c.MP + lb] += sum;
 }
 
 // ---- eviction -----------------------------------------------------------------
@@ -813,7 +871,8 @@ int64_t plan_split(const scope_paged_cache& c, int Hq, int maxkv, bool with_mass
   s.tiles_cap = (keys + kTileKeys - 1) / kTileKeys;
   const int64_t cols = static_cast<int64_t>(c.Hkv) * ng * (maxkv ? c.B : 1);
   const int64_t most = (s.tiles_cap + kPieceTiles - 1) / kPieceTiles;
-  s.pieces = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((kPieces + cols - 1) / cols, maxkv ? most : kPieces)));
+  const int want = pieces_wanted(c.B, c.D);
+  s.pieces = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((want + cols - 1) / cols, maxkv ? most : want)));
   const bool split = most > 1 && s.pieces > 1;
   s.slots = maxkv ? s.pieces * c.B : split ? s.pieces + c.B : c.B;
   if (!split) s.pieces = 1;
@@ -915,22 +974,16 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
     c->fp8 ? launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, true>{})
            : launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, false>{});
   if (int rc = check_launch("paged_attn_kernel")) return rc;
-  if (s.po) {  // some sequence may be in several pieces
-    const dim3 jg(c->B, Hq);
-    if (c->D == 64)
-      hipLaunchKernelGGL(paged_join_kernel<64>, jg, dim3(256), 0, st, *c, a, s);
-    else if (c->D == 128)
-      hipLaunchKernelGGL(paged_join_kernel<128>, jg, dim3(256), 0, st, *c, a, s);
-    else
-      hipLaunchKernelGGL(paged_join_kernel<256>, jg, dim3(256), 0, st, *c, a, s);
-    if (int rc = check_launch("paged_join_kernel")) return rc;
-  }
-  if (mass) {
-    const int blocks = kv_idx ? maxkv : c->MP;
-    hipLaunchKernelGGL(paged_mass_kernel, dim3(c->B, c->Hkv, ceil_div(blocks, 256)), dim3(256), 0, st, *c, a, s);
-    return check_launch("paged_mass_kernel");
-  }
-  return SCOPE_OK;
+  if (!s.po && !mass) return SCOPE_OK;  // every sequence is one piece
+  const int blocks = kv_idx ? maxkv : c->MP;
+  const dim3 fg(std::max(s.po ? G : 1, mass ? ceil_div(blocks, 256) : 1), c->Hkv, c->B);
+  if (c->D == 64)
+    hipLaunchKernelGGL(paged_finish_kernel<64>, fg, dim3(256), 0, st, *c, a, s);
+  else if (c->D == 128)
+    hipLaunchKernelGGL(paged_finish_kernel<128>, fg, dim3(256), 0, st, *c, a, s);
+  else
+    hipLaunchKernelGGL(paged_finish_kernel<256>, fg, dim3(256), 0, st, *c, a, s);
+  return check_launch("paged_finish_kernel");
 }
 
 int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, const int32_t* table, const float* mass,
