@@ -561,14 +561,16 @@ __device__ __forceinline__ float2 join_sums(const float* ml, int n, int64_t step
 }
 
 // What follows the pieces, for (sequence, key head) (blockIdx.z, blockIdx.y).
-// Workgroup x joins the pieces of the group's query head x, sixteen bytes of the
-// output row a thread, the pieces shared out over groups of threads; and with a
-// mass adds 256 blocks' probabilities, formed from their tiles' sums and the
-// rows' whole ones, a block a thread, its heads and tiles in order.  Both in one
-// launch: a second one costs more than the sums joined anew (4.7 us).
+// The first G workgroups join the pieces of a query head of the group each, sixteen
+// bytes of the output row a thread, the pieces shared out over groups of threads.
+// With a mass, the others add 256 blocks' probabilities each, formed from their
+// tiles' sums and the rows' whole ones, a block a thread, its heads and tiles in
+// order.  Both in one launch: a second one costs more than the sums joined anew
+// (4.7 us).
 template <int D>
 __global__ __launch_bounds__(256) void paged_finish_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
-  const int b = blockIdx.z, hk = blockIdx.y, x = blockIdx.x, G = a.Hq / c.Hkv;
+  const int b = blockIdx.z, hk = blockIdx.y, G = a.Hq / c.Hkv;
+  const int x = static_cast<int>(blockIdx.x) - (s.po ? G : 0);  // < 0: joins, else adds blocks
   const bool lists = a.kv_idx != nullptr;
   constexpr int LD = D / 4, NG = 256 / LD;
   __shared__ float w[kMostPieces], so[NG][D];
@@ -578,9 +580,10 @@ __global__ __launch_bounds__(256) void paged_finish_kernel(scope_paged_cache c, 
   const int n = plan.x;
   const int64_t step = 2ll * a.Hq;
   const float* ml0 = s.pml + (static_cast<int64_t>(plan.y) * a.Hq + hk * G) * 2;  // of the group's first head
-  if (x < G && n > 1) {  // (a sequence in one piece is written by it)
-    const int h = hk * G + x;
-    const float* ml = ml0 + 2 * x;
+  if (x < 0) {
+    if (n == 1) return;  // written by its only piece
+    const int g = x + G, h = hk * G + g;
+    const float* ml = ml0 + 2 * g;
     const int dl = tid % LD, grp = tid / LD;
     const float* po = s.po + (static_cast<int64_t>(plan.y) * a.Hq + h) * D + 4 * dl;
     const int64_t row = static_cast<int64_t>(a.Hq) * D;
@@ -615,9 +618,9 @@ __global__ __launch_bounds__(256) void paged_finish_kernel(scope_paged_cache c, 
       if (tid == 0)
         a.lse[static_cast<int64_t>(b) * a.Hq + h] = ML.y == 0.f ? -INFINITY : (ML.x + __builtin_amdgcn_logf(ML.y)) * kLn2;
     }
+    return;
   }
   const int blocks = lists ? a.maxkv : c.MP;
-  if (!a.mass || static_cast<int64_t>(x) * 256 >= blocks) return;
   const int64_t e = static_cast<int64_t>(x) * 256 + tid, bh = static_cast<int64_t>(b) * c.Hkv + hk;
   int64_t lb = -1;
   int lo = 0;
@@ -976,7 +979,7 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
   if (int rc = check_launch("paged_attn_kernel")) return rc;
   if (!s.po && !mass) return SCOPE_OK;  // every sequence is one piece
   const int blocks = kv_idx ? maxkv : c->MP;
-  const dim3 fg(std::max(s.po ? G : 1, mass ? ceil_div(blocks, 256) : 1), c->Hkv, c->B);
+  const dim3 fg((s.po ? G : 0) + (mass ? ceil_div(blocks, 256) : 0), c->Hkv, c->B);
   if (c->D == 64)
     hipLaunchKernelGGL(paged_finish_kernel<64>, fg, dim3(256), 0, st, *c, a, s);
   else if (c->D == 128)
