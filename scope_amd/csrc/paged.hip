@@ -691,10 +691,26 @@ __device__ __forceinline__ uint32_t weight_key(float f) {
 
 // One workgroup per sequence, K blocks a thread (block i = 1024·k + thread) with
 // their keys in registers, so that mass is read once.  The n-th smallest key is
-// found two bits a step: a step counts the keys below three probes (a comparison
-// and a popcount of its mask a key and probe) and costs one barrier.  Blocks with
-// a smaller key go, of those with the same key the first ones.
+// found in three digits of 11, 11 and 10 bits: the keys that agree with the
+// digits found so far are counted by their next one in LDS, and the digit is
+// where the running count passes n.  Blocks with a smaller key go, of those with
+// the same key the first ones.  Bound by latency: one sequence of 1027 blocks and
+// 8 heads 7.0 us (10.8 with the key found two bits at a time by ballots), 64 of
+// 8192 blocks 15.1 us for 17 MB (a workgroup a sequence; 37.6 with the ballots
+// and 16 loads a thread under way instead of 32).
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+
+constexpr int kDigit = 11, kBins = 1 << kDigit;
+
+// inclusive sum over the lanes of a wavefront
+__device__ __forceinline__ int wave_prefix(int v) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(v, o, kWave);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
 
 // counts[k·16 + wavefront] = the set flags before that group of 64 blocks, in the
 // blocks' order; returns the sum of all.  counts: K·16 + 1 ints of LDS.
@@ -716,11 +732,7 @@ __device__ __forceinline__ int prefix_flags(Flag flag, int* counts) {
       v[i] = lane * PER + i < N ? counts[lane * PER + i] : 0;
       sum += v[i];
     }
-    int upto = sum;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += x;
-    }
+    const int upto = wave_prefix(sum);
     int at = upto - sum;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -738,14 +750,15 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(EvictArgs a)
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t base = static_cast<int64_t>(b) * a.MP;
   __shared__ int counts[K * kEvictWaves + 1];
-  __shared__ int4 steps[2][kEvictWaves];
+  __shared__ int bins[kBins], totals[2 * kEvictWaves], found[2];
   const int64_t len = a.lens[b];
   const int n = len <= 0 ? 0 : static_cast<int>(min((len + a.bs - 1) / a.bs, static_cast<int64_t>(a.MP)));
   uint32_t key[K];
   int held = 0, may = 0;  // of the wavefront
-  // KG blocks at a time, so that their loads are under way together (block
-  // indices past the row are cut to it, and left out of the keys)
-  constexpr int KG = K < 8 ? K : 8, UH = KG == 8 ? 2 : 8;
+  // KG blocks and eight heads at a time, so that their loads are under way
+  // together (block indices past the row are cut to it, and left out of the keys)
+  constexpr int KG = K < 4 ? K : 4;
+  const float* mass = a.mass + static_cast<int64_t>(b) * a.Hkv * a.MP;
 #pragma unroll
   for (int g = 0; g < K; g += KG) {
 #pragma unroll
@@ -753,19 +766,28 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(EvictArgs a)
     if (g * kEvictThreads >= n) continue;
     int id[KG];
     double sum[KG];
-    const float* w[KG];
+    uint32_t at[KG];
 #pragma unroll
     for (int k = 0; k < KG; ++k) {
-      const int i = min((g + k) * kEvictThreads + tid, a.MP - 1);
-      id[k] = a.table[base + i];
-      w[k] = a.mass + static_cast<int64_t>(b) * a.Hkv * a.MP + i;
+      at[k] = min((g + k) * kEvictThreads + tid, a.MP - 1);
+      id[k] = a.table[base + at[k]];
       sum[k] = 0.0;
     }
-#pragma unroll UH
-    for (int h = 0; h < a.Hkv; ++h) {
+    int h = 0;
+    for (; h + 8 <= a.Hkv; h += 8) {
+      float f[8][KG];
 #pragma unroll
-      for (int k = 0; k < KG; ++k) sum[k] += w[k][static_cast<int64_t>(h) * a.MP];
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int k = 0; k < KG; ++k) f[j][k] = (mass + static_cast<int64_t>(h + j) * a.MP)[at[k]];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int k = 0; k < KG; ++k) sum[k] += f[j][k];
     }
+    for (; h < a.Hkv; ++h)
+#pragma unroll
+      for (int k = 0; k < KG; ++k) sum[k] += (mass + static_cast<int64_t>(h) * a.MP)[at[k]];
 #pragma unroll
     for (int k = 0; k < KG; ++k) {
       const int i = (g + k) * kEvictThreads + tid;
@@ -775,49 +797,47 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(EvictArgs a)
       if (can) key[g + k] = weight_key(static_cast<float>(sum[k]));
     }
   }
-  if (lane == 0) steps[1][wave] = make_int4(held, may, 0, 0);
+  if (lane == 0) {
+    totals[wave] = held;
+    totals[kEvictWaves + wave] = may;
+  }
   __syncthreads();
   held = may = 0;
 #pragma unroll
   for (int w = 0; w < kEvictWaves; ++w) {
-    held += steps[1][w].x;
-    may += steps[1][w].y;
+    held += totals[w];
+    may += totals[kEvictWaves + w];
   }
   const int n_drop = min(max(held - max(a.budget[b], 0), 0), may);
   uint64_t go = 0;  // bit k: block k of this thread
   if (n_drop > 0) {
-    uint32_t cut = 0;  // the largest value that fewer than n_drop keys lie below
+    uint32_t cut = 0;  // the n_drop-th smallest key, its digits from the top
     int below = 0;     // keys below it
-#pragma unroll 1
-    for (int bit = 30, at = 0; bit >= 0; bit -= 2, at ^= 1) {
-      const uint32_t p1 = cut | 1u << bit, p2 = cut | 2u << bit, p3 = cut | 3u << bit;
-      int n1 = 0, n2 = 0, n3 = 0;
+    static_assert(kBins == 2 * kEvictThreads, "two bins a thread");
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        n1 += __popcll(__ballot(key[k] < p1));
-        n2 += __popcll(__ballot(key[k] < p2));
-        n3 += __popcll(__ballot(key[k] < p3));
-      }
-      if (lane == 0) steps[at][wave] = make_int4(n1, n2, n3, 0);
-      __syncthreads();  // (the other half of steps is written in the next step)
-      n1 = n2 = n3 = 0;
+    for (int digit = 0; digit < 3; ++digit) {
+      const int low = digit == 0 ? 21 : digit == 1 ? 10 : 0, width = digit == 2 ? 10 : kDigit, top = low + width;
+      bins[2 * tid] = bins[2 * tid + 1] = 0;
+      __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kEvictWaves; ++w) {
-        const int4 x = steps[at][w];
-        n1 += x.x;
-        n2 += x.y;
-        n3 += x.z;
+      for (int k = 0; k < K; ++k)
+        if (key[k] != kKeyStays && (digit == 0 || key[k] >> (top & 31) == cut >> (top & 31)))
+          atomicAdd(&bins[key[k] >> low & ((1 << width) - 1)], 1);
+      __syncthreads();
+      const int b0 = bins[2 * tid], b1 = bins[2 * tid + 1], upto = wave_prefix(b0 + b1);
+      if (lane == 63) totals[wave] = upto;
+      __syncthreads();
+      int before = below + upto - b0 - b1;
+#pragma unroll
+      for (int w = 0; w < kEvictWaves; ++w) before += w < wave ? totals[w] : 0;
+      if (before < n_drop && n_drop <= before + b0 + b1) {  // one thread
+        const bool second = n_drop > before + b0;
+        found[0] = 2 * tid + second;
+        found[1] = before + (second ? b0 : 0);
       }
-      if (n3 < n_drop) {
-        cut = p3;
-        below = n3;
-      } else if (n2 < n_drop) {
-        cut = p2;
-        below = n2;
-      } else if (n1 < n_drop) {
-        cut = p1;
-        below = n1;
-      }
+      __syncthreads();
+      cut |= static_cast<uint32_t>(found[0]) << low;
+      below = found[1];
     }
     prefix_flags<K>([&](int k) { return key[k] == cut; }, counts);
 #pragma unroll
@@ -1001,11 +1021,16 @@ int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, 
   const EvictArgs a{B, Hkv, MP, bs, window, n_global, table, mass, lens, budget, table_out, freed, n_freed};
   const dim3 grid(B), block(kEvictThreads);
   hipStream_t st = as_stream(stream);
-  if (MP <= kEvictThreads)
+  const int k = ceil_div(MP, kEvictThreads);
+  if (k <= 1)
     hipLaunchKernelGGL(paged_evict_kernel<1>, grid, block, 0, st, a);
-  else if (MP <= 4 * kEvictThreads)
+  else if (k <= 2)
+    hipLaunchKernelGGL(paged_evict_kernel<2>, grid, block, 0, st, a);
+  else if (k <= 4)
     hipLaunchKernelGGL(paged_evict_kernel<4>, grid, block, 0, st, a);
-  else if (MP <= 16 * kEvictThreads)
+  else if (k <= 8)
+    hipLaunchKernelGGL(paged_evict_kernel<8>, grid, block, 0, st, a);
+  else if (k <= 16)
     hipLaunchKernelGGL(paged_evict_kernel<16>, grid, block, 0, st, a);
   else
     hipLaunchKernelGGL(paged_evict_kernel<64>, grid, block, 0, st, a);
