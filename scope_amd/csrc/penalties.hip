@@ -15,9 +15,15 @@
 namespace scope {
 
 namespace {
-constexpr int kPenThreads = 1024;
 constexpr int kPenWords = 8;  // of a thread
-constexpr int kPenTile = kPenThreads * kPenWords;
+constexpr int kXcds = 8;
+// Histories of up to this many tokens take 512 threads (4096 words) a workgroup,
+// whose waits are shorter (128 rows of 50304 words, histories to 8192: 16.3 us;
+// with 1024 threads 17.4).  Longer ones are read by fewer workgroups with 1024,
+// and those of a row follow each other on one XCD, so that its history comes into
+// one L2 (16 rows of 100003 words, histories of 60k to 131k: 19.0 us; on all XCDs
+// 22.1, with 512 threads 25.0).
+constexpr int64_t kLongHistory = 16384;
 }  // namespace
 
 struct PenaltyArgs {
@@ -60,18 +66,24 @@ __device__ __forceinline__ auto logit_out(float f) {
 // A workgroup holds the counters of its words in LDS (bit 31: seen, the rest: c)
 // and reads the whole history, its tokens 16 bytes a load and four loads under
 // way; its logits, bias and bits are loaded before that, so one latency covers
-// both.  8192 words a workgroup: with fewer, more workgroups read the same
-// history, which is what bounds long ones.
-template <int TYPE, class Token>
-__global__ __launch_bounds__(kPenThreads) void logit_penalties_kernel(scope_penalty_params p, PenaltyArgs a) {
+// both.
+template <int TYPE, class Token, int THREADS>
+__global__ __launch_bounds__(THREADS, 2048 / THREADS) void logit_penalties_kernel(scope_penalty_params p, PenaltyArgs a) {
   using Logit = typename std::conditional<TYPE == SCOPE_FP32, uint32_t, uint16_t>::type;
-  constexpr int PT = 16 / sizeof(Token), UNR = 4;
-  __shared__ __attribute__((aligned(16))) uint32_t count[kPenTile];
+  constexpr int PT = 16 / sizeof(Token), UNR = 4, TILE = THREADS * kPenWords, XCDS = THREADS == 1024 ? kXcds : 1;
+  __shared__ __attribute__((aligned(16))) uint32_t count[TILE + kWave];  // (and a place a lane for words of other tiles)
   const int tid = threadIdx.x;
-  const int64_t b = blockIdx.y, v0 = static_cast<int64_t>(blockIdx.x) * kPenTile;
-  const int nv = static_cast<int>(min(static_cast<int64_t>(kPenTile), p.V - v0));
+  // (workgroups go round the XCDs)
+  const int tiles = static_cast<int>((p.V + TILE - 1) / TILE), slot = blockIdx.x / XCDS;
+  const int64_t b = static_cast<int64_t>(slot / tiles) * XCDS + blockIdx.x % XCDS;
+  const int64_t v0 = static_cast<int64_t>(slot % tiles) * TILE;
+  if (b >= p.B) return;
+  const int nv = static_cast<int>(min(static_cast<int64_t>(TILE), p.V - v0));
   const int w0 = tid * kPenWords, mine = min(max(nv - w0, 0), kPenWords);  // this thread's words
   const int64_t len = p.lens64 ? static_cast<const int64_t*>(a.lens)[b] : static_cast<const int32_t*>(a.lens)[b];
+  const int64_t end = min(len, p.T), from = a.first ? max(a.first[b], 0) : 0, cut = a.n_prompt ? a.n_prompt[b] : 0;
+  const float r = a.repetition ? a.repetition[b] : p.repetition, f = a.frequency ? a.frequency[b] : p.frequency;
+  const float pr = a.presence ? a.presence[b] : p.presence, te = a.temperature ? a.temperature[b] : p.temperature;
   const Logit* zin = static_cast<const Logit*>(a.logits) + b * p.z_sb + v0 + w0;
   const float* bin = a.bias ? a.bias + b * p.bias_sb + v0 + w0 : nullptr;
   Packed<Logit, kPenWords> z;
@@ -89,41 +101,62 @@ __global__ __launch_bounds__(kPenThreads) void logit_penalties_kernel(scope_pena
   }
   if (a.mask && mine > 0) bits = static_cast<uint32_t>(a.mask[b * p.mask_sb + (v0 + w0) / 32]) >> (w0 % 32);
 #pragma unroll
-  for (int i = 0; i < kPenWords; i += 4) *reinterpret_cast<uint4*>(&count[i * kPenThreads + 4 * tid]) = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kPenWords; i += 4) *reinterpret_cast<uint4*>(&count[i * THREADS + 4 * tid]) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  const int64_t end = min(len, p.T), from = a.first ? max(a.first[b], 0) : 0, cut = a.n_prompt ? a.n_prompt[b] : 0;
   const Token* tokens = static_cast<const Token*>(a.tokens) + b * p.tok_sb;
-  for (int64_t j0 = from + tid * PT; j0 - tid * PT < end; j0 += static_cast<int64_t>(kPenThreads) * PT * UNR) {
-    Packed<Token, PT> t[UNR];
+  // A token's counter, or the lane's own place past them: a token of another tile
+  // or outside the vocabulary costs no branch.  (Words past V in the last tile
+  // have counters that nothing reads.)
+  const auto counter = [&](Token token) {
+    const uint32_t w = static_cast<uint32_t>(token) - static_cast<uint32_t>(v0);
+    return min(sizeof(Token) == 8 && static_cast<uint64_t>(token) >> 32 ? ~0u : w, static_cast<uint32_t>(TILE + tid % kWave));
+  };
+  const auto add = [&](Token token, bool counts) {
+    if (counts)
+      atomicAdd(&count[counter(token)], 1u);
+    else
+      atomicOr(&count[counter(token)], 0x80000000u);
+  };
+  constexpr int STEP = THREADS * PT;
+  const auto within = [](int64_t x) { return static_cast<int>(max(min(x, static_cast<int64_t>(1) << 30), static_cast<int64_t>(-1) << 30)); };
+  if (end - from >= PT) {
+    for (int64_t base = from; base < end; base += UNR * STEP) {
+      // places relative to base: the history's last load, and the first token that counts
+      const int last = within(end - base) - PT, first_new = within(cut - base);
+      Packed<Token, PT> t[UNR];
+      // (loads past the history's last are moved back to it, and only their new
+      // tokens count; no load under a branch, which would wait for those before it)
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) {
-      const int64_t j = j0 + static_cast<int64_t>(u) * kPenThreads * PT;
-      if (j + PT <= end) {
-        t[u] = *reinterpret_cast<const Packed<Token, PT>*>(tokens + j);
-      } else {
+      for (int u = 0; u < UNR; ++u) t[u] = *reinterpret_cast<const Packed<Token, PT>*>(tokens + base + min(u * STEP + tid * PT, last));
+      if (last + PT >= UNR * STEP && (first_new <= 0 || first_new >= UNR * STEP)) {
+        // within the history, and on one side of n_prompt
+        if (first_new <= 0) {
 #pragma unroll
-        for (int k = 0; k < PT; ++k) t[u].x[k] = j + k < end ? tokens[j + k] : Token{-1};
+          for (int u = 0; u < UNR; ++u)
+#pragma unroll
+            for (int k = 0; k < PT; ++k) atomicAdd(&count[counter(t[u].x[k])], 1u);
+        } else {
+#pragma unroll
+          for (int u = 0; u < UNR; ++u)
+#pragma unroll
+            for (int k = 0; k < PT; ++k) atomicOr(&count[counter(t[u].x[k])], 0x80000000u);
+        }
+        continue;
       }
-    }
 #pragma unroll
-    for (int u = 0; u < UNR; ++u) {
-      const int64_t j = j0 + static_cast<int64_t>(u) * kPenThreads * PT;
+      for (int u = 0; u < UNR; ++u)
+        if (u * STEP < last + PT) {
+          const int j = u * STEP + tid * PT, at = min(j, last);
 #pragma unroll
-      for (int k = 0; k < PT; ++k) {
-        // (a token outside the vocabulary, and a place past the history, are no words of any tile)
-        const uint64_t w = static_cast<uint64_t>(static_cast<int64_t>(t[u].x[k]) - v0);
-        if (w >= static_cast<uint64_t>(nv)) continue;
-        if (j + k >= cut)
-          atomicAdd(&count[w], 1u);
-        else
-          atomicOr(&count[w], 0x80000000u);
-      }
+          for (int k = 0; k < PT; ++k)
+            if (at + k >= j) add(t[u].x[k], at + k >= first_new);
+        }
     }
+  } else if (from + tid < end) {
+    add(tokens[from + tid], from + tid >= cut);
   }
   __syncthreads();
   if (mine == 0) return;
-  const float r = a.repetition ? a.repetition[b] : p.repetition, f = a.frequency ? a.frequency[b] : p.frequency;
-  const float pr = a.presence ? a.presence[b] : p.presence, te = a.temperature ? a.temperature[b] : p.temperature;
   uint32_t n[kPenWords];
 #pragma unroll
   for (int i = 0; i < kPenWords; i += 4) {
@@ -173,13 +206,22 @@ extern "C" int scope_logit_penalties(const scope_penalty_params* p, const void* 
   SCOPE_REQUIRE(p->type == SCOPE_BF16 || p->type == SCOPE_FP16 || p->type == SCOPE_FP32, "%s: unknown type %d", fn, p->type);
   SCOPE_REQUIRE(logits && out && lens && (tokens || p->T == 0), "%s: null pointer", fn);
   const PenaltyArgs a{logits, tokens, lens, first, n_prompt, repetition, presence, frequency, temperature, bias, mask, out};
-  const dim3 grid(ceil_div(p->V, kPenTile), p->B), block(kPenThreads);
+  const bool lng = p->T > kLongHistory;
+  const int threads = lng ? 1024 : 512, rows = lng ? ceil_div(p->B, kXcds) * kXcds : p->B;
+  const int64_t groups = static_cast<int64_t>(rows) * ceil_div(p->V, threads * kPenWords);
+  SCOPE_REQUIRE(groups <= INT32_MAX, "%s: %d rows of %lld words are more than one launch holds", fn, p->B, (long long)p->V);
+  const dim3 grid(static_cast<uint32_t>(groups)), block(threads);
+  hipStream_t st = as_stream(stream);
   const auto launch = [&](auto type) {
     constexpr int T = decltype(type)::value;
-    if (p->tokens64)
-      hipLaunchKernelGGL((logit_penalties_kernel<T, int64_t>), grid, block, 0, as_stream(stream), *p, a);
+    if (p->tokens64 && lng)
+      hipLaunchKernelGGL((logit_penalties_kernel<T, int64_t, 1024>), grid, block, 0, st, *p, a);
+    else if (p->tokens64)
+      hipLaunchKernelGGL((logit_penalties_kernel<T, int64_t, 512>), grid, block, 0, st, *p, a);
+    else if (lng)
+      hipLaunchKernelGGL((logit_penalties_kernel<T, int32_t, 1024>), grid, block, 0, st, *p, a);
     else
-      hipLaunchKernelGGL((logit_penalties_kernel<T, int32_t>), grid, block, 0, as_stream(stream), *p, a);
+      hipLaunchKernelGGL((logit_penalties_kernel<T, int32_t, 512>), grid, block, 0, st, *p, a);
   };
   if (p->type == SCOPE_FP32)
     launch(std::integral_constant<int, SCOPE_FP32>{});

@@ -60,7 +60,8 @@ def full(B, V, T, seed):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("B,V,T", [(1, 1, 1), (1, 33, 5), (2, 300, 40), (3, 4096, 100), (2, 4097, 2000), (2, 9001, 77), (3, 12295, 1500)])
+@pytest.mark.parametrize("B,V,T", [(1, 1, 1), (1, 33, 5), (2, 300, 40), (3, 4096, 100), (2, 4097, 2000), (2, 9001, 77), (3, 12295, 1500),
+                                   (1, 8193, 16384), (9, 8200, 16385), (17, 130, 20001)])
 def test_everything_at_once(ops, dtype, B, V, T):
     print(f"penalties {dtype} B={B} V={V} T={T}", flush=True)
     logits = (torch.randn((B, V), generator=torch.Generator().manual_seed(V)) * 5).to(dtype)
@@ -76,6 +77,19 @@ def test_one_at_a_time(ops, name, value):
     if name in ("first", "n_prompt"):
         kw["frequency"] = 0.5
     check(ops, logits, tokens, torch.tensor([60, 25]), **kw)
+
+
+@pytest.mark.parametrize("T", [16384, 40000])
+@pytest.mark.parametrize("token", [torch.int32, torch.int64])
+def test_token_types_and_edges_of_the_history(ops, T, token):
+    """Histories that start and end at every place of a 16-byte load, and of one to nine tokens."""
+    g = torch.Generator().manual_seed(T)
+    tokens = torch.randint(0, 300, (9, T), generator=g).to(token)
+    logits = torch.randn((9, 300), generator=g)
+    for first in (0, 1, 2, 3):
+        for n in (1, 2, 3, 4, 5, 8, 9, 4096, 8193):
+            lens = torch.full((9,), first + n) + torch.arange(9) % 2
+            check(ops, logits, tokens, lens, first=first, n_prompt=first + n // 2, frequency=0.25, repetition=1.5, presence=0.5)
 
 
 def test_nothing_asked_is_the_logits(ops):
