@@ -482,15 +482,28 @@ class ScopeDecoder(nn.Module):
         return self._g_out.clone()
 
     @torch.no_grad()
-    def generate(self, n_steps: int, first: int | torch.Tensor) -> torch.Tensor:
+    def generate(self, n_steps: int, first: int | torch.Tensor, *, penalties: dict | None = None) -> torch.Tensor:
         """Greedy decoding: feeds ``first``, then each argmax, for n_steps.
         With the one-launch step it returns when the tokens are there: a step
-        whose waits expired has no other step after it to say so."""
+        whose waits expired has no other step after it to say so.
+
+        ``penalties``: keywords of ``ops.logit_penalties`` (repetition, presence,
+        frequency, temperature, bias, mask, first, n_prompt), taken to every
+        step's logits over the tokens held so far; presence and frequency count
+        those of this call unless n_prompt says otherwise."""
+        V = self.cfg.vocab_size
         out = torch.empty(n_steps, dtype=torch.int64, device=self.device)
         tok = torch.as_tensor(first, device=self.device)
+        if penalties is not None:
+            penalties = {"n_prompt": self.t, **penalties}
+            for name in ("first", "n_prompt"):  # on the device once, not every step
+                if isinstance(penalties.get(name), int):
+                    penalties[name] = torch.tensor([penalties[name]], dtype=torch.int32, device=self.device)
         for s in range(n_steps):
-            logits = self.step(tok)
-            tok = ops.argmax(logits[:self.cfg.vocab_size], out=out[s:s + 1])  # written in place
+            logits = self.step(tok)[:V]
+            if penalties is not None:
+                ops.logit_penalties(logits, self.tokens, self._t_dev, out=logits, **penalties)
+            tok = ops.argmax(logits, out=out[s:s + 1])  # written in place
         if self._step_status is not None:
             torch.cuda.current_stream(self.device).synchronize()
             self._check_waits("generate")

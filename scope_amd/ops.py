@@ -1178,6 +1178,10 @@ def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: 
     vp, vh, vr, vd = v_pages.stride()
     if kd != 1 or vd != 1:
         raise RuntimeError(f"{who}: the pages' last dimension must be contiguous")
+    if P == 1:  # (the stride of a dimension of one is never taken)
+        kp = vp = 0
+    if Hkv == 1:
+        kh = vh = 0
     B, MP = table.shape
     return _lib.PagedCache(B, Hkv, D, bs, MP, _PAGED_TYPES[dtype], fp8, P, kp, kh, kr, vp, vh, vr)
 
@@ -1208,8 +1212,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                 raise RuntimeError(f"{who}: the pages are an expanded tensor: their rows share memory")
     lens = _ints(who, "lens", lens, c.B, dev)
     cu = _ints(who, "cu", cu, c.B + 1, dev)
-    _call_on(dev, "scope_paged_append", C.byref(c), shape[0], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-             _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(),
+    N, one = shape[0], c.Hkv == 1
+    _call_on(dev, "scope_paged_append", C.byref(c), N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1],
+             v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1], _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(),
              v_pages.data_ptr(), _stream(dev))
 
 
@@ -1257,7 +1262,8 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
     need = _paged_work_bytes(B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, scale, q.data_ptr(), qs[0], qs[1], k_pages.data_ptr(),
+    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, scale, q.data_ptr(), qs[0] if B > 1 else 0,
+             qs[1] if Hq > 1 else 0, k_pages.data_ptr(),
              v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _ptr(first),
              _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr(), _stream(dev))
     return out, lse

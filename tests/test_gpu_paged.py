@@ -45,6 +45,38 @@ def test_attn_head_groups(ops, Hq, Hkv):
     check_attn(ops, c, DEV, scale=0.12, mass=torch.zeros((2, Hkv, c["table"].shape[1])))
 
 
+@pytest.mark.parametrize("G", [15, 16, 17, 33])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_attn_wide_groups_of_wide_heads(ops, G, fp8):
+    """D = 256 with a full group of sixteen columns and more: the largest share of LDS."""
+    print(f"paged attn D=256 G={G} fp8={fp8}", flush=True)
+    c = cache([900, 65], Hq=G, Hkv=1, D=256, bs=64, fp8=fp8, seed=G)
+    check_attn(ops, c, DEV, scale=0.06, mass=torch.zeros((2, 1, c["table"].shape[1])))
+
+
+def test_strides_of_dimensions_of_one(ops):
+    """One sequence, one key head and one page as odd views: their strides are never taken."""
+    c = cache([13], Hq=2, Hkv=1, D=64, bs=16, MP=1, seed=4)
+    odd = lambda x: x.contiguous().as_strided(x.shape, (5,) + x.stride()[1:])  # noqa: E731
+
+    def strided(d):
+        d = dict(d, q=odd(d["q"]))
+        page = int(d["table"][0, 0])
+        for n in ("k_pages", "v_pages"):
+            one = d[n][page:page + 1].contiguous()
+            d[n] = one.as_strided(one.shape, (3, 7, 64, 1))
+        return d
+
+    d = strided({k: (x.to(DEV) if isinstance(x, torch.Tensor) else x) for k, x in c.items()})
+    zero = torch.zeros((1, 1), dtype=torch.int32, device=DEV)
+    out, lse = ops.paged_decode_attn(d["q"], d["k_pages"], d["v_pages"], zero, d["lens"], scale=0.12)
+    want, wl = check_attn(ops, c, DEV, scale=0.12)
+    assert torch.equal(out, want) and torch.equal(lse, wl)
+    row = torch.randn((1, 1, 64), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    ops.paged_append(row.as_strided((1, 1, 64), (3, 5, 1)), row, d["k_pages"], d["v_pages"], zero, d["lens"])
+    assert torch.equal(d["k_pages"][0, 0, 13], row[0, 0]) and torch.equal(d["v_pages"][0, 0, 13], row[0, 0])
+
+
 @pytest.mark.parametrize("B,hi", [(1, 9000), (3, 5000), (70, 400), (200, 130)])
 def test_attn_ragged_batches(ops, B, hi):
     """Long sequences beside short and empty ones: the split over the length and its join."""

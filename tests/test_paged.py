@@ -344,3 +344,37 @@ def test_struct_layouts_match_the_header(tmp_path):
     for cls in structs.values():
         want += [C.sizeof(cls)] + [getattr(cls, f).offset for f, _ in cls._fields_]
     assert got == want
+
+
+# ---- the cache's bookkeeping -------------------------------------------------------------
+def test_cache_takes_and_returns_pages():
+    from scope_amd import PagedKVCache
+
+    c = PagedKVCache(pages=6, sequences=2, max_len=80, kv_heads=1, head_dim=64, page_size=16, device="cpu")
+    assert c.table.shape == (2, 5) and c.free_pages == 6
+    c.reserve([17, 0])
+    assert c.table.tolist() == [[0, 1, -1, -1, -1], [-1] * 5] and c.free_pages == 4
+    c._len[0] = 17
+    c.reserve([15, 1])  # to the end of its second page: only the other sequence needs one
+    assert c.table.tolist() == [[0, 1, -1, -1, -1], [2, -1, -1, -1, -1]]
+    c._len = [32, 1]
+    with pytest.raises(RuntimeError, match="5 pages needed, 3 free"):
+        c.reserve([48, 32])
+    assert c.free_pages == 3 and c.table.tolist()[0] == [0, 1, -1, -1, -1]  # nothing was taken
+    with pytest.raises(RuntimeError, match="81 positions of 80"):
+        c.reserve([49, 0])
+    with pytest.raises(ValueError, match="rows"):
+        c.reserve([1])
+    with pytest.raises(ValueError, match="rows"):
+        c.reserve([1, -1])
+    c.mass.fill_(1.0)
+    c.release(0)
+    assert c.free_pages == 5 and c.length(0) == 0 and c.table.tolist()[0] == [-1] * 5 and c.mass[0].sum() == 0 and c.mass[1].sum() > 0
+    c.reserve([1, 0])
+    assert c.table[0, 0] == 0  # the lowest of its own first
+    with pytest.raises(ValueError, match="announced"):
+        c.append(torch.zeros(2, 1, 64).bfloat16(), torch.zeros(2, 1, 64).bfloat16(), rows=[1, 0])
+    with pytest.raises(RuntimeError, match="GPU"):
+        c.append(torch.zeros(2, 1, 64).bfloat16(), torch.zeros(2, 1, 64).bfloat16())
+    with pytest.raises(ValueError, match="at least 1"):
+        PagedKVCache(pages=0, sequences=1, max_len=1, kv_heads=1, head_dim=64, device="cpu")
