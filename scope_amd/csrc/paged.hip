@@ -251,6 +251,16 @@ __device__ __forceinline__ uint32_t round2(float lo, float hi) {
   }
 }
 
+// the halves of a word of two 16-bit values
+template <int TYPE>
+__device__ __forceinline__ float low_half(uint32_t w) {
+  return TYPE == SCOPE_BF16 ? __uint_as_float(w << 16) : half_to_f32(static_cast<uint16_t>(w));
+}
+template <int TYPE>
+__device__ __forceinline__ float high_half(uint32_t w) {
+  return TYPE == SCOPE_BF16 ? __uint_as_float(w & 0xffff0000u) : half_to_f32(static_cast<uint16_t>(w >> 16));
+}
+
 // two e4m3 bytes as 16-bit values (exact)
 template <int TYPE, bool HI>
 __device__ __forceinline__ uint32_t widen2(uint32_t w) {
@@ -293,11 +303,24 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // query's maximum, sum and outputs stay in the lanes of its column.  Scores are
 // scaled into log2 units in fp32; the maximum that the probabilities are taken
 // relative to moves only when a score passes it by more than 8 (p <= 256 until
-// then, no loss in floating point); they are rounded to the 16-bit type for the
-// product with V, as the type's own matrix instruction takes them, and summed
-// before that rounding.
+// then, no loss in floating point).  For the product with V, whose instruction
+// takes 16-bit operands, a probability is the sum of two 16-bit values (off by
+// 2^-17 of it, fp16 2^-23 or 2^-25 in all); one value alone, off by 2^-9, was 1.5
+// times as far from the exact output after its own rounding, and 0.3% faster.
+// Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
+// 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
+// GB) 5.6 TB/s with the launch behind it.  Only V passes the caches:
+// 103 us with the join and weights of the time, both through them 112, both past
+// them 106.  More in flight (two tiles at once, the next one's loads ahead)
+// changed nothing.
+constexpr int attn_waves(int D, bool fp8) {  // wavefronts a SIMD that the registers are cut to
+  // (D = 256 needs 256 registers and a few more in 16 bits: one wavefront 109 us, two
+  // that spill 113; in e4m3 two 59, one 78)
+  return D == 64 ? 4 : D == 128 ? 3 : fp8 ? 2 : 1;
+}
+
 template <int TYPE, bool FP8, int D>
-__global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void paged_attn_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
+__global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
   constexpr int NJ = D / 32;                     // products over D
   constexpr int VE = D / 16 < 8 ? D / 16 : 8;    // features of a lane in a row of V
   constexpr int NH = D / (16 * VE);              // rows of V in halves
@@ -472,8 +495,14 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
       if (!small) lt += __shfl_xor(lt, 32, kWave);
       put_sum(ref + __builtin_amdgcn_logf(lt));
     }
-    const uint4 pf = make_uint4(round2<TYPE>(x[0], x[1]), round2<TYPE>(x[2], x[3]), round2<TYPE>(x[4], x[5]),
-                                round2<TYPE>(x[6], x[7]));
+    // the probabilities as a sum of two 16-bit values each
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ph[i] = round2<TYPE>(x[2 * i], x[2 * i + 1]);
+      pl[i] = round2<TYPE>(x[2 * i] - low_half<TYPE>(ph[i]), x[2 * i + 1] - high_half<TYPE>(ph[i]));
+    }
+    const uint4 pf = make_uint4(ph[0], ph[1], ph[2], ph[3]), pg = make_uint4(pl[0], pl[1], pl[2], pl[3]);
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       uint32_t v[8][VE / 2];  // the eight rows as 16-bit pairs of neighbouring features
@@ -492,7 +521,8 @@ __global__ __launch_bounds__(kAttnThreads, D == 64 ? 4 : D == 128 ? 3 : 2) void 
 #pragma unroll
         for (int w = 0; w < 4; ++w)
           op[w] = j % 2 ? pack_hi16(v[2 * w][j / 2], v[2 * w + 1][j / 2]) : pack_lo16(v[2 * w][j / 2], v[2 * w + 1][j / 2]);
-        acc[h * VE + j] = mfma_16<TYPE>(make_uint4(op[0], op[1], op[2], op[3]), pf, acc[h * VE + j]);
+        const uint4 vt = make_uint4(op[0], op[1], op[2], op[3]);
+        acc[h * VE + j] = mfma_16<TYPE>(vt, pg, mfma_16<TYPE>(vt, pf, acc[h * VE + j]));
       }
     }
   }

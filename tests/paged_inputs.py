@@ -42,11 +42,11 @@ def cache(lens, *, Hq, Hkv, D, bs, dtype="bf16", fp8=False, MP=None, seed=0, amp
 def attn_bounds(dtype: torch.dtype, D: int, r: dict):
     """Bounds of (out, lse, weights), element by element, against fp64 (r: the oracle's).
 
-    u: half a step of the 16-bit type.  The kernel rounds each probability to
-    that type before its product with V (u·Σp|v|) and the result (u·|out|).  In
-    fp16 a probability below the normal range, taken relative to a maximum
-    whose own is at least 1, is off by up to 2^-25 (2^-25·Σ|v|), and so may be
-    the result.  Scores are fp32 sums of D exact products, one scaling and one
+    u: half a step of the 16-bit type.  The result is rounded to it (u·|out|).
+    The kernel takes each probability into its product with V as a sum of two
+    such values (u²·Σp|v|; in fp16 one below the normal range is off by up to
+    2^-25 relative to a maximum of at least 1: 2^-25·Σ|v|, and so may be the
+    result).  Scores are fp32 sums of D exact products, one scaling and one
     difference: off by at most δ = ((D + 2)·2^-24 + 3·2^-23)·max scale·Σ|q_d k_d|
     (+ 2^-22 for the exponential's and logarithm's own error), so that p is off
     by 2δ relative.  Sums of positive terms are formed as a few hundred partial
@@ -57,7 +57,7 @@ def attn_bounds(dtype: torch.dtype, D: int, r: dict):
     delta = ((D + 2) * 2.0 ** -24 + 3 * 2.0 ** -23) * r["size"] + 2.0 ** -22
     rel = 2 * delta + 2.0 ** -16
     low = 2.0 ** -25 * (1 + r["total"]) if dtype == torch.float16 else 0.0
-    b_out = u * r["out"].abs() + (u * (1 + u) + rel)[..., None] * r["spread"] + low
+    b_out = u * r["out"].abs() + (u * u + rel)[..., None] * r["spread"] + low
     b_lse = delta + 2.0 ** -16 + 2.0 ** -23 * r["lse"].abs().nan_to_num(posinf=0.0)
     b_w = (rel.max() + 2.0 ** -23) * r["weights"] + 2.0 ** -110
     return b_out, b_lse, b_w

@@ -142,8 +142,8 @@ def test_attn_equals_the_contiguous_decode_attention(ops):
     want, wl = ops.decode_attn(c["q"][0].to(DEV), k, v, kv_num.to(DEV), kv_idx.to(DEV), torch.zeros(T, dtype=torch.int32, device=DEV),
                                T - 1, bs=bs, scale=0.12)
     out, lse = check_attn(ops, c, DEV, scale=0.12, kv_num=kv_num[None], kv_idx=kv_idx[None])
-    # both round one result to bf16, this one its probabilities too: 2^-8 each of values below 1
-    assert (out[0].float() - want.float()).abs().max() <= 3 * 2.0 ** -8
+    # both round one result to bf16: half a step each of values below 1
+    assert (out[0].float() - want.float()).abs().max() <= 2 * 2.0 ** -8
     assert (lse[0] - wl).abs().max() <= 2.0 ** -15
 
 
