@@ -160,7 +160,11 @@ struct PagedAttnArgs {
 // blockIdx.x, (key head, group of 16 query heads) blockIdx.y.
 constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = 64 * kAttnWaves;
-constexpr int kPieceTiles = 2;  // a piece's least tiles
+
+// A piece's least tiles: short rows wait less in more pieces (1100 positions of 8
+// heads 11.5 us with 2, 12.7 with 4; lists of nine blocks of 128 8.9, 9.1, and 11.4
+// with 16).
+constexpr int kPieceTiles = 2;
 
 // Workgroups aimed at.  One sequence's pieces are equal and 1024 fill the device
 // evenly (131k positions, 8 heads: 103 us; 1536: 107, 768: 112).  The pieces of a

@@ -1252,6 +1252,8 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
             raise RuntimeError(f"{who}: kv_num and kv_idx come together")
         if kv_idx.dim() != 3 or kv_idx.shape[2] < 1 or kv_idx.shape[:2] != (B, Hkv) or kv_num.shape != (B, Hkv):
             raise RuntimeError(f"{who}: kv_num must be [{B}, {Hkv}] and kv_idx [{B}, {Hkv}, maxkv]")
+        if kv_num.is_floating_point() or kv_idx.is_floating_point():
+            raise RuntimeError(f"{who}: kv_num and kv_idx must be integers (got {kv_num.dtype} and {kv_idx.dtype})")
         maxkv = kv_idx.shape[2]
         kv_num, kv_idx = _i32(kv_num), _i32(kv_idx)
     if mass is not None and (mass.dtype != torch.float32 or mass.shape != (B, Hkv, MP) or not mass.is_contiguous()):
@@ -1262,7 +1264,7 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
     need = _paged_work_bytes(B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, scale, q.data_ptr(), qs[0] if B > 1 else 0,
+    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0,
              qs[1] if Hq > 1 else 0, k_pages.data_ptr(),
              v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _ptr(first),
              _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr(), _stream(dev))
@@ -1298,7 +1300,7 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     budget = _ints(who, "budget", budget, B, dev)
     freed = torch.empty((B, MP), dtype=torch.int32, device=dev)
     n_freed = torch.empty(B, dtype=torch.int32, device=dev)
-    _call_on(dev, "scope_paged_evict", B, ms[1], MP, bs, window, n_global, table.data_ptr(), mass.data_ptr(),
+    _call_on(dev, "scope_paged_evict", B, ms[1], MP, int(bs), int(window), int(n_global), table.data_ptr(), mass.data_ptr(),
              lens.data_ptr(), budget.data_ptr(), out.data_ptr(), freed.data_ptr(), n_freed.data_ptr(), _stream(dev))
     return out, freed, n_freed
 
@@ -1357,7 +1359,7 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
             positive = name == "repetition" or name == "temperature"
             if not math.isfinite(x) or (positive and x <= 0):
                 raise ValueError(f"{who}: {name} must be finite{' and positive' if positive else ''}, got {x}")
-            num.append(x)
+            num.append(float(x))
             arr.append(None)
     lens64 = isinstance(lens, torch.Tensor) and lens.dtype == torch.int64 and lens.numel() == B and lens.is_contiguous()
     if not lens64:

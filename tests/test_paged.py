@@ -263,7 +263,7 @@ def test_attention_wrapper_refusals(on_cpu):
                      (f8, dict(v_scale=torch.ones(2).half())), (c, dict(table=c["table"].long())), (c, dict(table=c["table"][:, ::2])),
                      (c, dict(table=c["table"][0])), (c, dict(lens=torch.ones(3, dtype=torch.int32))), (c, dict(lens=torch.ones(2))),
                      (c, dict(first=torch.ones(1, dtype=torch.int32))), (c, dict(kv_num=num)), (c, dict(kv_idx=idx)),
-                     (c, dict(kv_num=num[:1], kv_idx=idx)), (c, dict(kv_num=num, kv_idx=idx[0])), (c, dict(kv_num=num, kv_idx=idx[..., :0])),
+                     (c, dict(kv_num=num[:1], kv_idx=idx)), (c, dict(kv_num=num, kv_idx=idx.float())), (c, dict(kv_num=num.float(), kv_idx=idx)), (c, dict(kv_num=num, kv_idx=idx[0])), (c, dict(kv_num=num, kv_idx=idx[..., :0])),
                      (c, dict(mass=torch.zeros(2, 2, MP + 1))), (c, dict(mass=torch.zeros(2, 2, MP).double())),
                      (c, dict(mass=torch.zeros(2, 2, 2 * MP)[..., ::2]))):
         with pytest.raises(RuntimeError, match="paged_decode_attn"):
