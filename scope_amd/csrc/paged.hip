@@ -999,7 +999,7 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
 }
 
 int64_t scope_paged_attn_workspace_bytes(const scope_paged_cache* c, int Hq, int maxkv, int with_mass) {
-  if (!c || c->Hkv < 1 || Hq < 1 || Hq % c->Hkv) return 0;
+  if (!c || c->B < 1 || c->MP < 1 || c->bs < 1 || c->D < 1 || c->Hkv < 1 || Hq < 1 || Hq % c->Hkv || maxkv < 0) return 0;
   return plan_split(*c, Hq, maxkv, with_mass != 0, nullptr, nullptr);
 }
 

@@ -1129,14 +1129,17 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """``call`` with ``dev`` as the current device (a launch takes the current
-    device's kernels, whatever device its stream is on)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        call(name, *args)
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """``_lib.call`` on the current stream of ``dev``, which becomes the last
+    argument, with ``dev`` as the current device (a launch takes the current
+    device's kernels, whatever device its stream is on).  The tensors behind
+    the arguments' addresses are held by the caller."""
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            call(name, *args)
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _ints(who: str, name: str, x, n: int, dev: torch.device) -> torch.Tensor | None:
@@ -1213,9 +1216,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     lens = _ints(who, "lens", lens, c.B, dev)
     cu = _ints(who, "cu", cu, c.B + 1, dev)
     N, one = shape[0], c.Hkv == 1
-    _call_on(dev, "scope_paged_append", C.byref(c), N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1],
+    _launch(dev, "scope_paged_append", C.byref(c), N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1],
              v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1], _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(),
-             v_pages.data_ptr(), _stream(dev))
+             v_pages.data_ptr())
 
 
 def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -1260,14 +1263,14 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
         raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, {Hkv}, {MP}]")
     lens = _ints(who, "lens", lens, B, dev)
     first = _ints(who, "first", first, B, dev)
-    out = torch.empty(shape, dtype=dtype, device=dev)
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=dev)
     lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
     need = _paged_work_bytes(B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call_on(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0,
+    _launch(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0,
              qs[1] if Hq > 1 else 0, k_pages.data_ptr(),
              v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _ptr(first),
-             _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr(), _stream(dev))
+             _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr())
     return out, lse
 
 
@@ -1293,15 +1296,15 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     if mass.dtype != torch.float32 or len(ms) != 3 or ms[0] != B or ms[2] != MP or not mass.is_contiguous():
         raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, Hkv, {MP}]")
     if out is None:
-        out = torch.empty((B, MP), dtype=torch.int32, device=dev)
+        out = torch.empty_like(table)  # (less host work than empty)
     elif out.dtype != torch.int32 or out.shape != table.shape or not out.is_contiguous():
         raise RuntimeError(f"{who}: out must be a contiguous int32 [{B}, {MP}]")
     lens = _ints(who, "lens", lens, B, dev)
     budget = _ints(who, "budget", budget, B, dev)
-    freed = torch.empty((B, MP), dtype=torch.int32, device=dev)
+    freed = torch.empty_like(table)
     n_freed = torch.empty(B, dtype=torch.int32, device=dev)
-    _call_on(dev, "scope_paged_evict", B, ms[1], MP, int(bs), int(window), int(n_global), table.data_ptr(), mass.data_ptr(),
-             lens.data_ptr(), budget.data_ptr(), out.data_ptr(), freed.data_ptr(), n_freed.data_ptr(), _stream(dev))
+    _launch(dev, "scope_paged_evict", B, ms[1], MP, int(bs), int(window), int(n_global), table.data_ptr(), mass.data_ptr(),
+             lens.data_ptr(), budget.data_ptr(), out.data_ptr(), freed.data_ptr(), n_freed.data_ptr())
     return out, freed, n_freed
 
 
@@ -1329,7 +1332,7 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
     who = "logit_penalties"
     numbers = (repetition, presence, frequency, temperature)
     dev = _device(who, logits, tokens, bias, mask, out,
-                  *(x for x in (lens, first, n_prompt, *numbers) if isinstance(x, torch.Tensor)))
+                  *[x for x in (lens, first, n_prompt, *numbers) if isinstance(x, torch.Tensor)])
     zd, shape, dtype = logits.dim(), logits.shape, logits.dtype
     if dtype not in _PAGED_TYPES or not 1 <= zd <= 2 or logits.stride(-1) != 1 or logits.numel() < 1:
         raise RuntimeError(f"{who}: logits must be fp32, bf16 or fp16 [B, V] or [V] with contiguous rows")
@@ -1344,23 +1347,20 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
     if mask is not None and (mask.dtype != torch.int32 or mask.shape not in ((W,), (B, W)) or mask.stride(-1) != 1):
         raise RuntimeError(f"{who}: mask must be int32 [{W}] or [{B}, {W}] with contiguous rows")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty(shape, dtype=dtype, device=dev)
     elif out.dtype != dtype or out.shape != shape or out.stride(-1) != 1 or (B > 1 and out.stride(0) < V) \
             or (out.data_ptr() == logits.data_ptr() and B > 1 and out.stride(0) != logits.stride(0)):
         raise RuntimeError(f"{who}: out must have the logits' shape and type, rows of its own, and their strides if it is them")
-    num, arr = [], []
-    for name, x in zip(("repetition", "presence", "frequency", "temperature"), numbers):
-        if isinstance(x, torch.Tensor):
-            if x.numel() != B or not x.is_floating_point():
+    num, arr = numbers, (None, None, None, None)
+    if not all([type(x) is float for x in numbers]):
+        arr = [_f32(x) if isinstance(x, torch.Tensor) else None for x in numbers]
+        num = [1.0 if isinstance(x, torch.Tensor) else float(x) for x in numbers]
+        for name, x in zip(("repetition", "presence", "frequency", "temperature"), numbers):
+            if isinstance(x, torch.Tensor) and (x.numel() != B or not x.is_floating_point()):
                 raise RuntimeError(f"{who}: {name} must be a number or a float tensor [{B}]")
-            num.append(0.0)
-            arr.append(_f32(x))
-        else:
-            positive = name == "repetition" or name == "temperature"
-            if not math.isfinite(x) or (positive and x <= 0):
-                raise ValueError(f"{who}: {name} must be finite{' and positive' if positive else ''}, got {x}")
-            num.append(float(x))
-            arr.append(None)
+    if not (0.0 < num[0] < math.inf and 0.0 < num[3] < math.inf and math.isfinite(num[1]) and math.isfinite(num[2])):
+        raise ValueError(f"{who}: repetition and temperature must be finite and positive, presence and frequency finite (got "
+                         f"{num[0]}, {num[3]}, {num[1]} and {num[2]})")
     lens64 = isinstance(lens, torch.Tensor) and lens.dtype == torch.int64 and lens.numel() == B and lens.is_contiguous()
     if not lens64:
         lens = _ints(who, "lens", lens, B, dev)
@@ -1369,9 +1369,9 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
                              logits.stride(0) if zd == 2 else 0, out.stride(0) if zd == 2 else 0,
                              tokens.stride(0) if td == 2 else 0, bias.stride(0) if bias is not None and bias.dim() == 2 else 0,
                              mask.stride(0) if mask is not None and mask.dim() == 2 else 0, *num)
-    _call_on(dev, "scope_logit_penalties", C.byref(prm), logits.data_ptr(), tokens.data_ptr(), lens.data_ptr(),
+    _launch(dev, "scope_logit_penalties", C.byref(prm), logits.data_ptr(), tokens.data_ptr(), lens.data_ptr(),
              _ptr(first), _ptr(n_prompt), _ptr(arr[0]), _ptr(arr[1]), _ptr(arr[2]), _ptr(arr[3]), _ptr(bias), _ptr(mask),
-             out.data_ptr(), _stream(dev))
+             out.data_ptr())
     return out
 
 

@@ -13,7 +13,8 @@ The reference has no decode path and no cache.  Pages are taken from the pool
 when a sequence grows into them, on the host, whose copy of the lengths needs no
 reading back; ``evict`` reads the table back to know what it freed.  ``append``
 and ``attend`` never wait for the GPU, except where ``append`` takes pages: the
-new table entries are copied from pageable host memory.
+new table entries are copied from pageable host memory.  A cache is used on one
+stream at a time: a page goes from one sequence to another in stream order.
 """
 from __future__ import annotations
 

@@ -131,6 +131,27 @@ def test_attn_lists(ops, bs, maxkv):
     check_attn(ops, c, DEV, scale=0.12, kv_num=kv_num, kv_idx=kv_idx, first=torch.tensor([bs * 3 + 1, 5, 0], dtype=torch.int32))
 
 
+def test_attn_a_block_listed_twice_counts_twice(ops):
+    c = cache([200], Hq=2, Hkv=1, D=64, bs=32, seed=2)
+    kv_idx = torch.tensor([[[3, 0, 3, 6, 3]]], dtype=torch.int32)
+    check_attn(ops, c, DEV, scale=0.12, kv_num=torch.tensor([[5]], dtype=torch.int32), kv_idx=kv_idx)
+
+
+def test_no_sequences_and_no_rows(ops):
+    """Nothing to append is nothing done; a batch of none is refused, lists or not."""
+    c = cache([20], Hq=2, Hkv=1, D=64, bs=16)
+    d = {k: x.to(DEV) for k, x in c.items() if isinstance(x, torch.Tensor)}
+    before = d["k_pages"].clone()
+    none = torch.empty((0, 1, 64), dtype=torch.bfloat16, device=DEV)
+    ops.paged_append(none, none, d["k_pages"], d["v_pages"], d["table"], d["lens"], cu=torch.zeros(2, dtype=torch.int32, device=DEV))
+    ops.paged_append(none, none, d["k_pages"], d["v_pages"], d["table"], d["lens"])
+    assert torch.equal(d["k_pages"], before)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    for kw in ({}, dict(kv_num=torch.empty((0, 1), **i32), kv_idx=torch.empty((0, 1, 3), **i32))):
+        with pytest.raises(RuntimeError, match="bad sizes"):
+            ops.paged_decode_attn(d["q"][:0], d["k_pages"], d["v_pages"], d["table"][:0], d["lens"][:0], scale=0.1, **kw)
+
+
 def test_attn_equals_the_contiguous_decode_attention(ops):
     """One sequence whose pages lie in order, over the pointer mask's lists: the framework's contiguous call."""
     H, bs, T = 8, 128, 1152

@@ -204,7 +204,14 @@ def test_library_refuses_before_any_launch():
     for word, kw in (("sizes", dict(B=0)), ("sizes", dict(B=70000)), ("sizes", dict(V=0)), ("sizes", dict(T=-1)),
                      ("sizes", dict(V=2 ** 31)), ("type", dict(type=3)), ("null pointer", dict(logits=None))):
         penalise(word, **kw)
+    # the workspace of sizes that no call takes: none, and no division by them
     assert lib.scope_paged_attn_workspace_bytes(None, 4, 0, 0) == 0
+    for bad in (dict(B=0), dict(MP=0), dict(bs=0), dict(D=0), dict(Hkv=0), dict(Hkv=3), dict(B=-1), dict(MP=-2)):
+        c = _lib.PagedCache(**{**good, **bad})
+        assert lib.scope_paged_attn_workspace_bytes(C.byref(c), 4, 9, 1) == 0
+    c = _lib.PagedCache(**good)
+    assert lib.scope_paged_attn_workspace_bytes(C.byref(c), 0, 9, 1) == lib.scope_paged_attn_workspace_bytes(C.byref(c), 4, -1, 1) == 0
+    assert lib.scope_paged_attn_workspace_bytes(C.byref(c), 4, 9, 1) > 0
 
 
 @pytest.fixture()
@@ -220,8 +227,7 @@ def on_cpu(monkeypatch):
         raise Reached
 
     monkeypatch.setattr(ops, "_gpu", lambda who, *ts: torch.device("cpu"))
-    monkeypatch.setattr(ops, "_call_on", reached)
-    monkeypatch.setattr(ops, "_stream", lambda dev: None)
+    monkeypatch.setattr(ops, "_launch", reached)
     monkeypatch.setattr(ops, "query", lambda *a: 16)
     return ops, Reached
 
