@@ -47,18 +47,19 @@ struct AppendArgs {
   void* v_pages;
 };
 
-// 1 / s where the quotient x / s may be formed by it (quotient below), else 0
+// 1 / s where the quotient x / s may be formed by it (quotient below), else 0: for
+// scales in 2^-60 .. 2^60 whose significand is not all ones
 __device__ __forceinline__ float quotient_factor(float s) {
-  return s >= 0x1p-60f && s <= 0x1p60f ? 1.f / s : 0.f;
+  return s >= 0x1p-60f && s <= 0x1p60f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu ? 1.f / s : 0.f;
 }
 
 // The fp32 quotient x / s of a 16-bit x, rounded to nearest as a division rounds
-// it, as far as e4m3 can tell.  With r = 1 / s to nearest, q = x·r is off by at
-// most two steps, and one residual step q + r·(x - q·s) is the quotient to
-// nearest (the residual is exact while it does not fall below 2^-126: with s in
-// 2^-60 .. 2^60 that is only where |q| < 2^-20, which is 0 in e4m3 either way).
-// Quotients past every finite e4m3, infinities and NaN need no residual.  Three
-// instructions for the division's ten.
+// it, as far as e4m3 can tell.  With r = 1 / s to nearest, q = x·r is next to the
+// quotient, and one residual step q + r·(x - q·s) gives it to nearest (Markstein's
+// division; the residual is exact while it does not fall below 2^-126, as for
+// |q| >= 2^-20 and these scales it does not).  Quotients below that are 0 in e4m3
+// and keep their sign without the step; those past every finite e4m3, infinities
+// and NaN need none.  A few instructions for the division's ten.
 __device__ __forceinline__ float quotient(float x, float s, float r) {
   if (r == 0.f) return x / s;
   const float q = x * r;

@@ -332,6 +332,28 @@ def test_append_e4m3_rounding(ops):
         assert torch.equal(torch.signbit(got[~nan]), torch.signbit(want.float()[~nan]))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_append_e4m3_of_every_value(ops, dtype):
+    """All 65536 values of the type over scales of every kind, the ones that take a plain division among
+    them, as torch divides, cuts and rounds."""
+    t = TYPES[dtype]
+    x = torch.arange(-2 ** 15, 2 ** 15).to(torch.int16).view(t).reshape(1024, 1, 64).to(DEV)
+    table, zero = torch.arange(64, dtype=torch.int32, device=DEV)[None], torch.zeros(1, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 1024], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    scales = [1.0, 0.0, -1.0, math.inf, math.nan, 1e-30, 1e30, 2.0 ** -60, 2.0 ** 61, 2.0 ** -140, 2 - 2.0 ** -23, 0.1, 1 / 3, 448.0]
+    scales += torch.exp(torch.randn(12, generator=g) * 4).tolist()
+    kp, vp = (torch.zeros((64, 1, 16, 64), dtype=torch.float8_e4m3fn, device=DEV) for _ in range(2))
+    for s in scales:
+        s = torch.tensor([s], device=DEV)
+        ops.paged_append(x, x, kp, vp, table, zero, cu=cu, k_scale=s)
+        want = (x.float() / s).clamp(-448, 448).to(torch.float8_e4m3fn).reshape(64, 16, 64)
+        got = kp[:, 0].view(torch.uint8)
+        nan = torch.isnan(want.float())
+        assert torch.equal(torch.isnan(kp[:, 0].float()), nan), f"scale {s.item()}"
+        assert torch.equal(got[~nan], want.view(torch.uint8)[~nan]), f"scale {s.item()}"
+
+
 # ---- eviction -------------------------------------------------------------------------
 @pytest.mark.parametrize("B,Hkv,MP", [(1, 1, 1), (3, 8, 7), (5, 2, 64), (4, 3, 1027), (2, 8, 4099), (1, 1, 20000), (2, 1, 65536)])
 @pytest.mark.parametrize("window,n_global", [(1, 0), (4, 2)])
