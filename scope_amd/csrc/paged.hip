@@ -22,6 +22,38 @@ __device__ __forceinline__ uint16_t f32_to_half(float f) { return __builtin_bit_
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// op over a wavefront in six steps on neighbouring lanes' registers (row shifts by
+// 1, 2, 4, 8, then the rows' last lanes to the rows behind them): lane l gets the
+// result over lanes 0 .. l.  A step costs a few cycles, one through LDS some sixty.
+template <int CTRL, int ROWS, class Op>
+__device__ __forceinline__ uint32_t lane_step(uint32_t v, uint32_t none, Op op) {
+  return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(v), CTRL, ROWS, 0xf, false)));
+}
+template <class Op>
+__device__ __forceinline__ uint32_t lane_prefix(uint32_t v, uint32_t none, Op op) {
+  v = lane_step<0x111, 0xf>(v, none, op);
+  v = lane_step<0x112, 0xf>(v, none, op);
+  v = lane_step<0x114, 0xf>(v, none, op);
+  v = lane_step<0x118, 0xf>(v, none, op);
+  v = lane_step<0x142, 0xa>(v, none, op);
+  return lane_step<0x143, 0xc>(v, none, op);
+}
+__device__ __forceinline__ uint32_t add_u32(uint32_t a, uint32_t b) { return a + b; }
+__device__ __forceinline__ uint32_t add_f32(uint32_t a, uint32_t b) {
+  return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+__device__ __forceinline__ uint32_t max_f32(uint32_t a, uint32_t b) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+// the sums over lanes 0 .. l of a count, and over all lanes
+__device__ __forceinline__ int prefix_of(int v) { return static_cast<int>(lane_prefix(static_cast<uint32_t>(v), 0u, add_u32)); }
+__device__ __forceinline__ float sum_of(float v) {
+  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0u, add_f32), 63));
+}
+__device__ __forceinline__ float max_of(float v) {
+  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0xff800000u, max_f32), 63));
+}
 }  // namespace
 
 // ---- append ------------------------------------------------------------------
@@ -202,23 +234,19 @@ __device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const Pag
   };
   int lo0;
   const int tiles0 = tiles_of(lane, &lo0);
-  int64_t total = tiles0;
-  for (int b = 64 + lane; b < c.B; b += 64) {
+  // (64 sequences of less than 2^26 tiles: their sum fits 32 bits)
+  int64_t total = static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles0), 63));
+  for (int b0 = 64; b0 < c.B; b0 += 64) {
     int lo;
-    total += tiles_of(b, &lo);
+    total += static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles_of(b0 + lane, &lo)), 63));
   }
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, kWave);
   const int64_t piece = piece_tiles(total, s.pieces, kPieceTiles);
   int before = 0;
   for (int b0 = 0; b0 < c.B; b0 += 64) {
     int lo = lo0;
     const int tiles = b0 ? tiles_of(b0 + lane, &lo) : tiles0;
     const int n = b0 + lane < c.B ? seq_pieces(tiles, piece) : 0;
-    int upto = n;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += v;
-    }
+    const int upto = prefix_of(n);
     const uint64_t hit = __ballot(x < before + upto);
     if (hit) {
       const int at = __ffsll(static_cast<unsigned long long>(hit)) - 1;
@@ -599,14 +627,13 @@ __device__ __forceinline__ float2 join_sums(const float* ml, int n, int64_t step
   }
   float M = m0;
   for (int i = lane + 64; i < n; i += 64) M = fmaxf(M, ml[i * step]);
-  M = wave_max_f32(M);
+  M = max_of(M);
   float L = l0 == 0.f ? 0.f : __builtin_amdgcn_exp2f(m0 - M) * l0;
   for (int i = lane + 64; i < n; i += 64) {
     const float li = ml[i * step + 1];
     L += li == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[i * step] - M) * li;
   }
-  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, kWave);
-  return make_float2(M, L);
+  return make_float2(M, sum_of(L));
 }
 
 // What follows the pieces, for (sequence, key head) (blockIdx.z, blockIdx.y).
@@ -751,16 +778,6 @@ constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 
 constexpr int kDigit = 11, kBins = 1 << kDigit;
 
-// inclusive sum over the lanes of a wavefront
-__device__ __forceinline__ int wave_prefix(int v) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(v, o, kWave);
-    if (lane >= o) v += x;
-  }
-  return v;
-}
-
 // counts[k·16 + wavefront] = the set flags before that group of 64 blocks, in the
 // blocks' order; returns the sum of all.  counts: K·16 + 1 ints of LDS.
 template <int K, class Flag>
@@ -781,7 +798,7 @@ __device__ __forceinline__ int prefix_flags(Flag flag, int* counts) {
       v[i] = lane * PER + i < N ? counts[lane * PER + i] : 0;
       sum += v[i];
     }
-    const int upto = wave_prefix(sum);
+    const int upto = prefix_of(sum);
     int at = upto - sum;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -873,7 +890,7 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(EvictArgs a)
         if (key[k] != kKeyStays && (digit == 0 || key[k] >> (top & 31) == cut >> (top & 31)))
           atomicAdd(&bins[key[k] >> low & ((1 << width) - 1)], 1);
       __syncthreads();
-      const int b0 = bins[2 * tid], b1 = bins[2 * tid + 1], upto = wave_prefix(b0 + b1);
+      const int b0 = bins[2 * tid], b1 = bins[2 * tid + 1], upto = prefix_of(b0 + b1);
       if (lane == 63) totals[wave] = upto;
       __syncthreads();
       int before = below + upto - b0 - b1;
