@@ -46,6 +46,19 @@ __device__ __forceinline__ uint32_t add_f32(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t max_f32(uint32_t a, uint32_t b) {
   return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
 }
+// op over the four lanes l % 16 + 16 k, or over two of them (k = 0, 1 and 2, 3): rows
+// of 16 lanes and halves of 32 exchanged between two copies
+template <class Op>
+__device__ __forceinline__ float over_rows2(float v, Op op) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(op(r[0], r[1]));
+}
+template <class Op>
+__device__ __forceinline__ float over_rows(float v, Op op) {
+  const uint32_t x = __float_as_uint(over_rows2(v, op));
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __uint_as_float(op(r[0], r[1]));
+}
 // the sums over lanes 0 .. l of a count, and over all lanes
 __device__ __forceinline__ int prefix_of(int v) { return static_cast<int>(lane_prefix(static_cast<uint32_t>(v), 0u, add_u32)); }
 __device__ __forceinline__ float sum_of(float v) {
@@ -507,8 +520,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
     if (__any(top > m + 8.f)) {
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      top = over_rows(top, max_f32);
       const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
@@ -524,8 +536,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     }
     l += lt;
     if (s.tile_lse) {
-      lt += __shfl_xor(lt, 16, kWave);
-      if (!small) lt += __shfl_xor(lt, 32, kWave);
+      lt = small ? over_rows2(lt, add_f32) : over_rows(lt, add_f32);
       put_sum(ref + __builtin_amdgcn_logf(lt));
     }
     // the probabilities as a sum of two 16-bit values each
@@ -561,8 +572,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
   }
 
   // the wavefronts' shares: maxima and sums, then the outputs of the group's queries
-  l += __shfl_xor(l, 16, kWave);
-  l += __shfl_xor(l, 32, kWave);
+  l = over_rows(l, add_f32);
   float* sm = lds;                       // [waves][16]
   float* sl = lds + kAttnWaves * 16;     // [waves][16]
   float* so = lds + kAttnWaves * 32;     // [waves][nq][D]
