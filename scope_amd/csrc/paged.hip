@@ -208,15 +208,15 @@ constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = 64 * kAttnWaves;
 
 // A piece's least tiles: short rows wait less in more pieces (1100 positions of 8
-// heads 11.5 us with 2, 12.7 with 4; lists of nine blocks of 128 8.9, 9.1, and 11.4
-// with 16).
+// heads 10.0 us with 2, 12.2 with 4, 15.2 with 16; lists of nine blocks of 128 8.2,
+// 8.6 and 11.3).
 constexpr int kPieceTiles = 2;
 
-// Workgroups aimed at.  One sequence's pieces are equal and 1024 fill the device
-// evenly (131k positions, 8 heads: 103 us; 1536: 107, 768: 112).  The pieces of a
-// ragged batch are not, and smaller ones even out its end (64 query heads over 24
-// sequences of 9k to 65k: 1536 269 us, 1024 280), except at D = 256, whose partial
-// rows are longer (16 sequences to 16k: 1024 120 us, 1536 123).
+// Workgroups aimed at.  The pieces of a ragged batch are not equal, and smaller ones
+// even out its end (64 query heads over 24 sequences of 9k to 65k: 1536 270 us, 1024
+// 280, 768 313); one sequence's are (131k positions: 1024 96 us, 1536 98), and at D =
+// 256 the partial rows are longer (16 sequences to 16k: 1024 107 us, 1536 114; in
+// whole turns of the wavefronts, which change nothing elsewhere, 102).
 constexpr int kMostPieces = 1536;
 constexpr int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
 
@@ -238,7 +238,7 @@ struct Piece {
 // The piece of this workgroup, found by every wavefront for itself: the batch's
 // tiles are summed, then the sequences' numbers of pieces.  false: there is none.
 __device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const PagedAttnArgs& a, const AttnSplit& s, int x,
-                                           Piece& p) {
+                                           int turn, Piece& p) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
   const auto tiles_of = [&](int b, int* lo) {
@@ -253,7 +253,7 @@ __device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const Pag
     int lo;
     total += static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles_of(b0 + lane, &lo)), 63));
   }
-  const int64_t piece = piece_tiles(total, s.pieces, kPieceTiles);
+  const int64_t piece = piece_tiles(total, s.pieces, kPieceTiles, turn);
   int before = 0;
   for (int b0 = 0; b0 < c.B; b0 += 64) {
     int lo = lo0;
@@ -355,13 +355,13 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // times as far from the exact output after its own rounding, and 0.3% faster.
 // Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
 // 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
-// GB) 5.6 TB/s with the launch behind it.  Only V passes the caches:
-// 103 us with the join and weights of the time, both through them 112, both past
-// them 106.  More in flight (two tiles at once, the next one's loads ahead)
-// changed nothing.
+// GB) 5.6 TB/s with the launch behind it.  V passes the caches (131k
+// positions with the launch behind it 96 us, through them 105); K does not (the same
+// 96 past them, but 1100 positions 10.0 -> 10.7 us).  More in flight (two tiles at
+// once, the next one's loads ahead) changed nothing.
 constexpr int attn_waves(int D, bool fp8) {  // wavefronts a SIMD that the registers are cut to
-  // (D = 256 needs 256 registers and a few more in 16 bits: one wavefront 109 us, two
-  // that spill 113; in e4m3 two 59, one 78)
+  // (D = 256 needs 256 registers and a few more in 16 bits: one wavefront 107 us, two
+  // that spill 113; in e4m3 two 58, one 75)
   return D == 64 ? 4 : D == 128 ? 3 : fp8 ? 2 : 1;
 }
 
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     p.slot = p.b * s.pieces;
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
-  } else if (!find_piece(c, a, s, blockIdx.x, p)) {
+  } else if (!find_piece(c, a, s, blockIdx.x, D == 256 ? kAttnWaves : 1, p)) {
     return;
   }
   const int b = p.b;
@@ -973,7 +973,10 @@ int64_t plan_split(const scope_paged_cache& c, int Hq, int maxkv, bool with_mass
   const int want = pieces_wanted(c.B, c.D);
   s.pieces = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((want + cols - 1) / cols, maxkv ? most : want)));
   const bool split = most > 1 && s.pieces > 1;
-  s.slots = maxkv ? s.pieces * c.B : split ? s.pieces + c.B : c.B;
+  // (the pieces of a batch are no more than those aimed at and one a sequence, nor
+  // than the shortest ones that a table row holds)
+  s.slots = static_cast<int>(maxkv ? static_cast<int64_t>(s.pieces) * c.B
+                                   : split ? std::min<int64_t>(s.pieces + c.B, most * c.B) : c.B);
   if (!split) s.pieces = 1;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {

@@ -33,10 +33,11 @@ SCOPE_HD int seq_tiles(int64_t len, int64_t first, int64_t cap, int* lo) {
   return static_cast<int>((end + kTileKeys - 1) / kTileKeys) - *lo;
 }
 
-// tiles of a piece, for a batch of `total` tiles and about `pieces` of them
-SCOPE_HD int64_t piece_tiles(int64_t total, int pieces, int least) {
-  const int64_t c = (total + pieces - 1) / pieces;
-  return c > least ? c : least;
+// tiles of a piece, for a batch of `total` tiles and about `pieces` of them: a
+// multiple of `turn`, `least` at least
+SCOPE_HD int64_t piece_tiles(int64_t total, int pieces, int least, int turn) {
+  const int64_t c = (total + pieces - 1) / pieces, d = (c + turn - 1) / turn * turn;
+  return c > least ? d : least;
 }
 
 // pieces of a sequence (one at least: it writes the zeros of an empty row).

@@ -24,7 +24,7 @@ PLAN = r'''
 using namespace scope;
 extern "C" {
 int tiles(int64_t len, int64_t first, int64_t cap, int* lo) { return seq_tiles(len, first, cap, lo); }
-int64_t piece(int64_t total, int pieces, int least) { return piece_tiles(total, pieces, least); }
+int64_t piece(int64_t total, int pieces, int least, int turn) { return piece_tiles(total, pieces, least, turn); }
 int pieces(int tiles, int64_t piece) { return seq_pieces(tiles, piece); }
 void range(int lo, int tiles, int n, int i, int* t) { piece_range(lo, tiles, n, i, t, t + 1); }
 int64_t page(const int32_t* row, int MP, int64_t lb, int64_t P) { return block_page(row, MP, lb, P); }
@@ -41,7 +41,7 @@ def plan(tmp_path_factory):
                     str(d / "plan.cpp"), "-o", str(d / "plan.so")], check=True)
     lib = C.CDLL(str(d / "plan.so"))
     i64, p = C.c_int64, C.c_void_p
-    for name, res, args in (("tiles", C.c_int, [i64, i64, i64, p]), ("piece", i64, [i64, C.c_int, C.c_int]),
+    for name, res, args in (("tiles", C.c_int, [i64, i64, i64, p]), ("piece", i64, [i64, C.c_int, C.c_int, C.c_int]),
                             ("pieces", C.c_int, [C.c_int, i64]), ("range", None, [C.c_int] * 4 + [p]),
                             ("page", i64, [p, C.c_int, i64, i64]), ("position", i64, [p, p, C.c_int, i64, p])):
         getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
@@ -70,8 +70,9 @@ def test_every_tile_is_in_one_piece(plan, seed):
             assert lo.value * 32 <= first < lo.value * 32 + 32 and (lo.value + t - 1) * 32 < end <= (lo.value + t) * 32
         seqs.append((lo.value, t))
     total = sum(t for _, t in seqs)
-    c = plan.piece(total, want, least)
-    assert c >= least
+    turn = r.choice([1, 4])
+    c = plan.piece(total, want, least, turn)
+    assert c >= least and (c == least or c % turn == 0)
     slots = 0
     for lo, t in seqs:
         n = plan.pieces(t, c)
@@ -84,7 +85,7 @@ def test_every_tile_is_in_one_piece(plan, seed):
             at = got[1]
         assert at == lo + t
         slots += n
-    assert slots <= want + B
+    assert slots <= want + B and slots <= B * -(-(-(-cap // 32)) // least)
 
 
 def test_list_pieces_cover_every_list(plan):
