@@ -662,7 +662,7 @@ int scope_argmax_f32(const float* x, int64_t n, int64_t* out, void* stream);
  *   table [B][MP]     int32 page of each block of bs positions; an entry
  *                     outside [0, P) is a block without a page
  *   lens [B]          int32 positions of each sequence; kept to [0, MP·bs]
- * D in {64, 128, 256}, bs in {16, 32, 64, 128, 256}, MP·bs < 2^31.
+ * D in {64, 128, 256}, bs in {16, 32, 64, 128, 256}, MP·bs <= 2^31 - 32.
  * ---------------------------------------------------------------------- */
 enum { SCOPE_BF16 = 0, SCOPE_FP16 = 1, SCOPE_FP32 = 2 };
 typedef struct {

@@ -951,8 +951,9 @@ int check_cache(const scope_paged_cache* c, const void* k_pages, const void* v_p
   SCOPE_REQUIRE(c->type == SCOPE_BF16 || c->type == SCOPE_FP16, "%s: unknown type %d", fn, c->type);
   SCOPE_REQUIRE(c->B >= 1 && c->B <= 65535 && c->Hkv >= 1 && c->Hkv <= 4096 && c->P >= 1,
                 "%s: bad sizes B=%d (1 .. 65535), Hkv=%d (1 .. 4096), P=%lld (at least 1)", fn, c->B, c->Hkv, (long long)c->P);
-  SCOPE_REQUIRE(c->MP >= 1 && static_cast<int64_t>(c->MP) * c->bs <= INT32_MAX,
-                "%s: a table row of %d pages of %d positions (1 .. 2^31 - 1 positions)", fn, c->MP, c->bs);
+  // (less than 2^26 tiles a row: the plan sums 64 rows in 32 bits)
+  SCOPE_REQUIRE(c->MP >= 1 && static_cast<int64_t>(c->MP) * c->bs <= INT32_MAX - (kTileKeys - 1),
+                "%s: a table row of %d pages of %d positions (1 .. 2^31 - 32 positions)", fn, c->MP, c->bs);
   const int al = c->fp8 ? 16 : 8;  // elements of 16 bytes
   SCOPE_REQUIRE(k_pages && v_pages, "%s: null pages", fn);
   SCOPE_REQUIRE(c->k_sp % al == 0 && c->k_sh % al == 0 && c->k_sr % al == 0 && c->v_sp % al == 0 && c->v_sh % al == 0 &&

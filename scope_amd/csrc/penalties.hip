@@ -118,7 +118,7 @@ __global__ __launch_bounds__(THREADS, 2048 / THREADS) void logit_penalties_kerne
       atomicOr(&count[counter(token)], 0x80000000u);
   };
   constexpr int STEP = THREADS * PT;
-  const auto within = [](int64_t x) { return static_cast<int>(max(min(x, static_cast<int64_t>(1) << 30), static_cast<int64_t>(-1) << 30)); };
+  const auto within = [](int64_t x) { return static_cast<int>(max(min(x, static_cast<int64_t>(1) << 30), -(static_cast<int64_t>(1) << 30))); };
   if (end - from >= PT) {
     for (int64_t base = from; base < end; base += UNR * STEP) {
       // places relative to base: the history's last load, and the first token that counts

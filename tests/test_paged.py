@@ -170,6 +170,7 @@ def test_library_refuses_before_any_launch():
     for word, kw in (("head dim", dict(D=96)), ("page size", dict(bs=48)), ("page size", dict(bs=512)), ("type", dict(type=2)),
                      ("bad sizes", dict(B=0)), ("bad sizes", dict(B=65536)), ("bad sizes", dict(Hkv=0)), ("bad sizes", dict(P=0)),
                      ("table row", dict(MP=0)), ("table row", dict(MP=2 ** 25)), ("aligned", dict(k_sr=132)),
+                     ("table row", dict(MP=2 ** 27 - 1, bs=16)),  # 2^26 tiles, 64 of which pass 32 bits
                      ("aligned", dict(v_sp=4)), ("aligned", dict(fp8=1, k_sr=136)), ("aligned", dict(pages=C.c_void_p(8))),
                      ("null pages", dict(pages=None)), ("multiple", dict(Hq=3)), ("multiple", dict(Hq=0)),
                      ("multiple", dict(Hq=65536)), ("kv_num", dict(num=one)), ("kv_num", dict(idx=one, maxkv=3)),
