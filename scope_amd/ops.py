@@ -1142,6 +1142,14 @@ def _launch(dev: torch.device, name: str, *args) -> None:
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def _sat32(x: torch.Tensor) -> torch.Tensor:
+    """Integers as contiguous int32; those past 32 bits as the nearest one, on the
+    same side of every length and index."""
+    if x.dtype == torch.int32:
+        return x.contiguous()
+    return (x.clamp(-2 ** 31, 2 ** 31 - 1) if x.dtype == torch.int64 else x).to(torch.int32).contiguous()
+
+
 def _ints(who: str, name: str, x, n: int, dev: torch.device) -> torch.Tensor | None:
     """n int32 numbers on dev: of an integer tensor of n elements, or one number for all."""
     if x is None:
@@ -1151,7 +1159,7 @@ def _ints(who: str, name: str, x, n: int, dev: torch.device) -> torch.Tensor | N
     dt = x.dtype
     if x.numel() != n or (dt != torch.int32 and dt != torch.int64):
         raise RuntimeError(f"{who}: {name} must be int32 or int64 [{n}] (got {x.dtype} {tuple(x.shape)})")
-    return x if dt == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+    return x if dt == torch.int32 and x.is_contiguous() else _sat32(x)
 
 
 @functools.lru_cache(maxsize=256)
@@ -1258,7 +1266,7 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
         if kv_num.is_floating_point() or kv_idx.is_floating_point():
             raise RuntimeError(f"{who}: kv_num and kv_idx must be integers (got {kv_num.dtype} and {kv_idx.dtype})")
         maxkv = kv_idx.shape[2]
-        kv_num, kv_idx = _i32(kv_num), _i32(kv_idx)
+        kv_num, kv_idx = _sat32(kv_num), _sat32(kv_idx)
     if mass is not None and (mass.dtype != torch.float32 or mass.shape != (B, Hkv, MP) or not mass.is_contiguous()):
         raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, {Hkv}, {MP}]")
     lens = _ints(who, "lens", lens, B, dev)

@@ -388,6 +388,27 @@ def test_evict_in_place_and_by_budgets(ops):
     assert out is d and torch.equal(d.cpu(), want[0]) and torch.equal(freed.cpu(), want[1]) and torch.equal(n.cpu(), want[2])
 
 
+def test_integers_past_32_bits(ops):
+    """int64 budgets, lengths, first positions and list entries that no int32 holds: as the number says."""
+    none = 2 ** 63 - 1
+    table = torch.arange(2 * 40, dtype=torch.int32, device=DEV).reshape(2, 40)
+    out, _, n = ops.paged_evict(table, torch.rand((2, 1, 40), device=DEV), torch.tensor([2 ** 33, 640], device=DEV),
+                                torch.tensor([none, 2 ** 32 + 30], device=DEV), bs=16)
+    assert torch.equal(out, table) and n.tolist() == [0, 0]
+    c = {k: x.to(DEV) if torch.is_tensor(x) else x for k, x in cache([200, 90], Hq=2, Hkv=1, D=64, bs=32, seed=21).items()}
+    args = [c[k] for k in ("q", "k_pages", "v_pages", "table")]
+    want = ops.paged_decode_attn(*args, c["lens"], scale=0.1)
+    for first, seen in ((2 ** 32, False), (-2 ** 32 - 1, True)):
+        got, lse = ops.paged_decode_attn(*args, c["lens"], scale=0.1, first=torch.tensor([first, 0], device=DEV))
+        assert torch.equal(got[1], want[0][1])
+        assert torch.equal(got[0], want[0][0]) if seen else bool((got[0] == 0).all()) and bool((lse[0] == -math.inf).all())
+    idx = torch.tensor([1, 2 ** 32, 0], device=DEV).repeat(2, 1, 1)
+    got = ops.paged_decode_attn(*args, c["lens"], scale=0.1, kv_num=torch.full((2, 1), 2 ** 40, device=DEV), kv_idx=idx)
+    ref = ops.paged_decode_attn(*args, c["lens"], scale=0.1, kv_num=torch.full((2, 1), 3, device=DEV),
+                                kv_idx=torch.tensor([1, -1, 0], device=DEV).repeat(2, 1, 1))
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
 # ---- together ---------------------------------------------------------------------------
 @pytest.mark.parametrize("fp8", [False, True])
 def test_prompts_steps_and_evictions_together(ops, fp8):

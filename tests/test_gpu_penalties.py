@@ -111,6 +111,13 @@ def test_tokens_outside_the_vocabulary_and_lengths_outside_the_history(ops):
           repetition=1.5, frequency=0.5, first=torch.tensor([-5, 29, 0, 40]), n_prompt=torch.tensor([-1, 500, 0, 3]))
 
 
+def test_nothing_counts_from_the_largest_position_on(ops):
+    g = torch.Generator().manual_seed(4)
+    logits, tokens = torch.randn((2, 100), generator=g).to(DEV), torch.randint(0, 100, (2, 30), generator=g).to(DEV)
+    got = ops.logit_penalties(logits, tokens, 30, n_prompt=torch.tensor([2 ** 63 - 1, 2 ** 32], device=DEV), frequency=1.0, presence=1.0)
+    assert torch.equal(got, logits)
+
+
 def test_infinite_logits_and_rows_without_a_word(ops):
     """-inf and the type's lowest value stay, NaN stays, a mask of zeros leaves -inf everywhere."""
     logits = torch.tensor([[0.0, -math.inf, math.inf, math.nan, -0.0, 1.0, torch.finfo(torch.float32).min, 5.0]])

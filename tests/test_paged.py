@@ -278,6 +278,18 @@ def test_attention_wrapper_refusals(on_cpu):
             call(src, **bad)
 
 
+def test_integers_past_32_bits_stay_on_their_side(on_cpu):
+    """A limit of 2^40 or the largest int64 for "none": not the 0 or -1 of its low 32 bits."""
+    ops, _ = on_cpu
+    x = torch.tensor([2 ** 40, -2 ** 40, 2 ** 63 - 1, -2 ** 63, 2 ** 31, -2 ** 31 - 1, 7, -7])
+    want = [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, -2 ** 31, 7, -7]
+    assert ops._ints("x", "x", x, 8, x.device).tolist() == ops._sat32(x[None])[0].tolist() == want
+    y = torch.stack((x, x), 1)[:, 0]  # a column
+    assert ops._ints("x", "y", y, 8, x.device).tolist() == want
+    z = torch.arange(16, dtype=torch.int32)[::2]
+    assert ops._ints("x", "z", z, 8, z.device).is_contiguous() and ops._sat32(z).tolist() == list(range(0, 16, 2))
+
+
 def test_append_and_evict_wrapper_refusals(on_cpu):
     ops, Reached = on_cpu
     c = cache([20, 5], Hq=4, Hkv=2, D=64, bs=16)
