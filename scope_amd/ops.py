@@ -1311,7 +1311,10 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     budget = _ints(who, "budget", budget, B, dev)
     freed = torch.empty_like(table)
     n_freed = torch.empty(B, dtype=torch.int32, device=dev)
-    _launch(dev, "scope_paged_evict", B, ms[1], MP, int(bs), int(window), int(n_global), table.data_ptr(), mass.data_ptr(),
+    window, n_global = min(int(window), MP), min(int(n_global), MP)  # (a C int each; MP keeps every block)
+    if window < 1 or n_global < 0:
+        raise RuntimeError(f"{who}: window={window} must be at least 1 (the page being written stays), n_global={n_global} at least 0")
+    _launch(dev, "scope_paged_evict", B, ms[1], MP, int(bs), window, n_global, table.data_ptr(), mass.data_ptr(),
              lens.data_ptr(), budget.data_ptr(), out.data_ptr(), freed.data_ptr(), n_freed.data_ptr())
     return out, freed, n_freed
 

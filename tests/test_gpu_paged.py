@@ -395,6 +395,9 @@ def test_integers_past_32_bits(ops):
     out, _, n = ops.paged_evict(table, torch.rand((2, 1, 40), device=DEV), torch.tensor([2 ** 33, 640], device=DEV),
                                 torch.tensor([none, 2 ** 32 + 30], device=DEV), bs=16)
     assert torch.equal(out, table) and n.tolist() == [0, 0]
+    for kw in (dict(window=2 ** 32 + 1), dict(n_global=2 ** 32)):
+        out, _, n = ops.paged_evict(table, torch.rand((2, 1, 40), device=DEV), torch.tensor([640, 640], device=DEV), 1, bs=16, **kw)
+        assert torch.equal(out, table) and n.tolist() == [0, 0]
     c = {k: x.to(DEV) if torch.is_tensor(x) else x for k, x in cache([200, 90], Hq=2, Hkv=1, D=64, bs=32, seed=21).items()}
     args = [c[k] for k in ("q", "k_pages", "v_pages", "table")]
     want = ops.paged_decode_attn(*args, c["lens"], scale=0.1)

@@ -319,7 +319,7 @@ def test_append_and_evict_wrapper_refusals(on_cpu):
             evict(**ok)
     for bad in (dict(table=c["table"].long()), dict(mass=mass[..., :1]), dict(mass=mass.half()), dict(mass=mass[0]), dict(mass=mass.transpose(0, 1)[:, :, :]
                 .contiguous().transpose(0, 1)), dict(lens=c["lens"][:1]), dict(budget=torch.tensor([1])), dict(out=c["table"].long()),
-                dict(out=c["table"][:1])):
+                dict(out=c["table"][:1]), dict(window=0), dict(window=-2 ** 32 + 5), dict(n_global=-1), dict(n_global=-2 ** 32)):
         with pytest.raises(RuntimeError, match="paged_evict"):
             evict(**bad)
 
