@@ -15,6 +15,8 @@ reading back; ``evict`` reads the table back to know what it freed.  ``append``
 and ``attend`` never wait for the GPU, except where ``append`` takes pages: the
 new table entries are copied from pageable host memory.  A cache is used on one
 stream at a time: a page goes from one sequence to another in stream order.
+``attend`` may be captured into a graph; the calls that also change the host's
+copy, which a replay would not, raise there.
 """
 from __future__ import annotations
 
@@ -59,9 +61,15 @@ class PagedKVCache:
     def length(self, sequence: int) -> int:
         return self._len[sequence]
 
+    def _on_host(self, what: str) -> None:
+        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"PagedKVCache: {what} changes lengths or pages on the host, which a replayed graph would not; "
+                               "capture the operators of scope_amd.ops instead")
+
     def reserve(self, rows) -> None:
         """Takes the pages that rows[b] more positions of each sequence b need;
         raises before it takes any if the pool or a sequence's table is too short."""
+        self._on_host("reserve")
         if len(rows) != len(self._len) or any(n < 0 for n in rows):
             raise ValueError(f"PagedKVCache: rows must be {len(self._len)} numbers of at least 0, got {list(rows)}")
         want = []
@@ -85,6 +93,7 @@ class PagedKVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, rows=None) -> None:
         """Appends k, v [N, kv_heads, head_dim]: rows[b] of them, in order, to each
         sequence b (their sum is N), or without ``rows`` one to every sequence."""
+        self._on_host("append")
         B = len(self._len)
         one_each = rows is None
         rows = [1] * B if one_each else [int(n) for n in rows]
@@ -114,6 +123,7 @@ class PagedKVCache:
         """Brings every sequence back to ``budget`` pages (a number or int [sequences])
         by ``ops.paged_evict`` on the accumulated weights; returns how many pages
         went back to the pool.  Waits for the GPU."""
+        self._on_host("evict")
         ops.paged_evict(self.table, self.mass, self.lens, budget, bs=self.page_size, window=window, n_global=n_global,
                         out=self.table)
         count = 0
@@ -125,6 +135,7 @@ class PagedKVCache:
 
     def release(self, sequence: int) -> None:
         """Ends a sequence: its pages go back to the pool, its length and weights to 0."""
+        self._on_host("release")
         held = self._pages[sequence]
         self._free += [held[i] for i in sorted(held, reverse=True)]
         held.clear()

@@ -80,6 +80,20 @@ def test_cache_in_use(dtype):
         c.append(torch.zeros((160, Hkv, D), dtype=rows_t, device=DEV), torch.zeros((160, Hkv, D), dtype=rows_t, device=DEV), [160, 0, 0])
 
 
+def test_calls_that_a_replay_would_not_repeat_are_refused(monkeypatch):
+    from scope_amd import PagedKVCache
+
+    c = PagedKVCache(pages=4, sequences=1, max_len=64, kv_heads=1, head_dim=64, page_size=16)
+    x = torch.zeros((1, 1, 64), dtype=torch.bfloat16, device=DEV)
+    c.append(x, x)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        for call in (lambda: c.append(x, x), lambda: c.append(x, x, [1]), lambda: c.reserve([3]), lambda: c.evict(1), lambda: c.release(0)):
+            with pytest.raises(RuntimeError, match="on the host"):
+                call()
+    assert c.length(0) == 1 and c.free_pages == 3 and c.lens.tolist() == [1]
+
+
 def test_pointer_lists_over_pages():
     """The pointer selection's lists of each sequence's newest block, attended to over shuffled pages; a page
     that eviction took is not seen though its block is listed."""
