@@ -690,7 +690,8 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
  * has a page and, with lists, j / bs is among kv_idx [B][Hkv][maxkv] up to
  * kv_num [B][Hkv] (entries outside [0, MP) are skipped, kv_num is kept to
  * [0, maxkv]; an entry listed twice counts twice).
- *   out [B][Hq][D]     softmax(scale · q·k) · v; zeros where nothing is seen
+ *   out [B][Hq][D]     softmax(scale · q·k) · v; zeros where nothing is seen; an
+ *                      infinite value of v in a seen row gives inf or NaN
  *   lse [B][Hq]        natural logarithm of the sum; -inf there
  *   mass [B][Hkv][MP]  or NULL: each block's probabilities, summed over its
  *                      positions and the group's query heads, are added (lists

@@ -352,7 +352,8 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // then, no loss in floating point).  For the product with V, whose instruction
 // takes 16-bit operands, a probability is the sum of two 16-bit values (off by
 // 2^-17 of it, fp16 2^-23 or 2^-25 in all); one value alone, off by 2^-9, was 1.5
-// times as far from the exact output after its own rounding, and 0.3% faster.
+// times as far from the exact output after its own rounding, and 0.3% faster.  (The
+// second value may be 0 or negative: an infinite value of V can come out as NaN.)
 // Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
 // 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
 // GB) 5.6 TB/s with the launch behind it.  V passes the caches (131k
