@@ -351,8 +351,17 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // relative to moves only when a score passes it by more than 8 (p <= 256 until
 // then, no loss in floating point).  For the product with V, whose instruction
 // takes 16-bit operands, a probability is the sum of two 16-bit values (off by
-// 2^-17 of it, fp16 2^-23 or 2^-25 in all); one value alone, off by 2^-9, was 1.5
-// times as far from the exact output after its own rounding, and 0.3% faster.  (The
+// 2^-17 of it, fp16 2^-23); one value alone, off by 2^-9, was 1.5
+// times as far from the exact output after its own rounding, and 0.3% faster.
+// fp16 has no exponents for the small weights of a long cache (below 2^-25 a key
+// would count in the sum and not in the output: behind one key that takes nearly all
+// of the weight, 131k others 17.4 nats lower came out as 0).  There the
+// probabilities are taken relative to each tile's own largest, which becomes 2^14,
+// and sums and outputs follow by powers of two: a key is off by no more than 2^-39
+// of its tile's largest (half of fp16's smallest step), all of them by 2^-34 of the
+// sum.  That costs up to 1% (48 windows of 4096 at D = 64 53.8 us either way, 32
+// sequences to 16k at D = 128 58.8 -> 59.1); a tile's product of its own, joined by an
+// fp32 factor, spills at D = 128 (79.7).  (The
 // second value may be 0 or negative: an infinite value of V can come out as NaN.)
 // Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
 // 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
@@ -365,6 +374,11 @@ constexpr int attn_waves(int D, bool fp8) {  // wavefronts a SIMD that the regis
   // that spill 113; in e4m3 two 58, one 75)
   return D == 64 ? 4 : D == 128 ? 3 : fp8 ? 2 : 1;
 }
+
+// fp16: log2 of a tile's largest probability, and how far below the largest so far
+// a tile is taken as it is (deeper, its keys are off by up to 2^-99 of the sum; the
+// sums stay below 2^(14 + 60 + 31), the outputs 2^16 times that)
+constexpr float kTopBits = 14.f, kMostBelow = 60.f;
 
 template <int TYPE, bool FP8, int D>
 __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
@@ -415,7 +429,8 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
   f32x4_t acc[NH * VE];
 #pragma unroll
   for (int i = 0; i < NH * VE; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  // the maximum so far, what the probabilities are taken relative to, their sum
+  float m = -INFINITY, ref = 0.f, l = 0.f;
 
   const char* kbase = static_cast<const char*>(a.k_pages) + hk * c.k_sh * ES;
   const char* vbase = static_cast<const char*>(a.v_pages) + hk * c.v_sh * ES;
@@ -520,15 +535,26 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-    if (__any(top > m + 8.f)) {
-      top = over_rows(top, max_f32);
-      const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
+    const auto rescale = [&](float f) {
       l *= f;
 #pragma unroll
       for (int i = 0; i < NH * VE; ++i) acc[i] *= f;
+    };
+    if constexpr (TYPE == SCOPE_FP16) {
+      top = over_rows(top, max_f32);
+      const float mn = fmaxf(m, top), to = rintf(fmaxf(top, mn - kMostBelow)) - kTopBits;
+      if (mn != -INFINITY) {
+        rescale(m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - to));
+        ref = to;
+        m = mn;
+      }
+    } else if (__any(top > m + 8.f)) {
+      top = over_rows(top, max_f32);
+      const float mn = fmaxf(m, top);
+      rescale(mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn));
+      m = mn;
+      ref = m == -INFINITY ? 0.f : m;
     }
-    const float ref = m == -INFINITY ? 0.f : m;
     float lt = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -578,7 +604,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
   float* sl = lds + kAttnWaves * 16;     // [waves][16]
   float* so = lds + kAttnWaves * 32;     // [waves][nq][D]
   if (g4 == 0) {
-    sm[wave * 16 + c16] = m;
+    sm[wave * 16 + c16] = m == -INFINITY ? m : ref;
     sl[wave * 16 + c16] = l;
   }
   if (c16 < nq) {
