@@ -356,8 +356,8 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // fp16 has no exponents for the small weights of a long cache (below 2^-25 a key
 // would count in the sum and not in the output: behind one key that takes nearly all
 // of the weight, 131k others 17.4 nats lower came out as 0).  There the
-// probabilities are taken relative to each tile's own largest, which becomes 2^14,
-// and sums and outputs follow by powers of two: a key is off by no more than 2^-39
+// probabilities are taken relative to each tile's own largest, which becomes 2^14 to
+// 2^15, and sums and outputs follow by powers of two: a key is off by no more than 2^-39
 // of its tile's largest (half of fp16's smallest step), all of them by 2^-34 of the
 // sum.  That costs up to 1% (48 windows of 4096 at D = 64 53.8 us either way, 32
 // sequences to 16k at D = 128 58.8 -> 59.1); a tile's product of its own, joined by an
@@ -375,9 +375,9 @@ constexpr int attn_waves(int D, bool fp8) {  // wavefronts a SIMD that the regis
   return D == 64 ? 4 : D == 128 ? 3 : fp8 ? 2 : 1;
 }
 
-// fp16: log2 of a tile's largest probability, and how far below the largest so far
+// fp16: log2 of a tile's largest probability (2^15 at most), and how far below the largest so far
 // a tile is taken as it is (deeper, its keys are off by up to 2^-99 of the sum; the
-// sums stay below 2^(14 + 60 + 31), the outputs 2^16 times that)
+// sums stay below 2^(15 + 60 + 31), the outputs 2^16 times that)
 constexpr float kTopBits = 14.f, kMostBelow = 60.f;
 
 template <int TYPE, bool FP8, int D>
@@ -542,7 +542,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     };
     if constexpr (TYPE == SCOPE_FP16) {
       top = over_rows(top, max_f32);
-      const float mn = fmaxf(m, top), to = rintf(fmaxf(top, mn - kMostBelow)) - kTopBits;
+      const float mn = fmaxf(m, top), to = floorf(fmaxf(top, mn - kMostBelow)) - kTopBits;
       if (mn != -INFINITY) {
         rescale(m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref - to));
         ref = to;

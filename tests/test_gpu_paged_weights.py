@@ -4,7 +4,7 @@
 The kernel takes a probability into its product with V as a sum of two 16-bit
 parts, off by at most 2^-17 (bf16) or 2^-23 (fp16) of it, in fp16 by 2^-39 of the
 largest among the 32 keys of its tile where that is more (half of fp16's smallest
-step, the largest scaled to 2^13.5 or more).  The tiles' largest sum to no more
+step, the largest scaled to 2^14 or more).  The tiles' largest sum to no more
 than all probabilities do, so fp16 loses at most 32·2^-39 = 2^-34 of the largest
 |v| of the output, however long the cache is."""
 from __future__ import annotations
@@ -71,6 +71,6 @@ def test_small_weights_add_up(ops, dtype, fp8, D, bs, T, sink):
     rel = (2.0 ** -23 if dtype == "fp16" else 2.0 ** -17) + 105 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -16
     bound = (half_step(t) + rel) * want
     if dtype == "fp16":
-        bound = bound + 2.0 ** -25 + 2.0 ** -34 * 1.5
+        bound = bound + 2.0 ** -25 + 2.0 ** -34 * 1.5  # (|v| <= 1.5)
     over = (out[0].double() - want).abs() - bound
     assert over.max() <= 0, f"gap {gaps[int(over.amax(1).argmax())].item()}: {over.max().item():.3e} over its bound"
