@@ -350,9 +350,9 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // scaled into log2 units in fp32; the maximum that the probabilities are taken
 // relative to moves only when a score passes it by more than 8 (p <= 256 until
 // then, no loss in floating point).  For the product with V, whose instruction
-// takes 16-bit operands, a probability is the sum of two 16-bit values (off by
-// 2^-17 of it, fp16 2^-23); one value alone, off by 2^-9, was 1.5
-// times as far from the exact output after its own rounding, and 0.3% faster.
+// takes 16-bit operands, a probability is the sum of 16-bit values: three in bf16
+// (off by 2^-27 of it, less than fp32 itself; two, off by 2^-17, were 1% faster in
+// e4m3 and no faster in bf16), two in fp16 (2^-23).
 // fp16 has no exponents for the small weights of a long cache (below 2^-25 a key
 // would count in the sum and not in the output: behind one key that takes nearly all
 // of the weight, 131k others 17.4 nats lower came out as 0).  There the
@@ -362,7 +362,7 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // sum.  That costs up to 1% (48 windows of 4096 at D = 64 53.8 us either way, 32
 // sequences to 16k at D = 128 58.8 -> 59.1); a tile's product of its own, joined by an
 // fp32 factor, spills at D = 128 (79.7).  (The
-// second value may be 0 or negative: an infinite value of V can come out as NaN.)
+// later values may be 0 or negative: an infinite value of V can come out as NaN.)
 // Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
 // 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
 // GB) 5.6 TB/s with the launch behind it.  V passes the caches (131k
@@ -379,6 +379,9 @@ constexpr int attn_waves(int D, bool fp8) {  // wavefronts a SIMD that the regis
 // a tile is taken as it is (deeper, its keys are off by up to 2^-99 of the sum; the
 // sums stay below 2^(15 + 60 + 31), the outputs 2^16 times that)
 constexpr float kTopBits = 14.f, kMostBelow = 60.f;
+
+// 16-bit values whose sum is a probability in the product with V
+constexpr int prob_parts(int type) { return type == SCOPE_FP16 ? 2 : 3; }
 
 template <int TYPE, bool FP8, int D>
 __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_kernel(scope_paged_cache c, PagedAttnArgs a, AttnSplit s) {
@@ -566,16 +569,23 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
       lt = small ? over_rows2(lt, add_f32) : over_rows(lt, add_f32);
       put_sum(ref + __builtin_amdgcn_logf(lt));
     }
-    // the probabilities as a sum of two 16-bit values each
-    uint32_t ph[4], pl[4];
+    // the probabilities as a sum of 16-bit values each
+    constexpr int NP = prob_parts(TYPE);
+    uint4 pf[NP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ph[i] = round2<TYPE>(x[2 * i], x[2 * i + 1]);
-      pl[i] = round2<TYPE>(x[2 * i] - low_half<TYPE>(ph[i]), x[2 * i + 1] - high_half<TYPE>(ph[i]));
+    for (int k = 0; k < NP; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = round2<TYPE>(x[2 * i], x[2 * i + 1]);
+        x[2 * i] -= low_half<TYPE>(w[i]);
+        x[2 * i + 1] -= high_half<TYPE>(w[i]);
+      }
+      pf[k] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    const uint4 pf = make_uint4(ph[0], ph[1], ph[2], ph[3]), pg = make_uint4(pl[0], pl[1], pl[2], pl[3]);
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
+      if constexpr (NH > 1) __builtin_amdgcn_sched_barrier(0);  // (or registers spill: e4m3 59 us, this way 55.5)
       uint32_t v[8][VE / 2];  // the eight rows as 16-bit pairs of neighbouring features
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -593,7 +603,8 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
         for (int w = 0; w < 4; ++w)
           op[w] = j % 2 ? pack_hi16(v[2 * w][j / 2], v[2 * w + 1][j / 2]) : pack_lo16(v[2 * w][j / 2], v[2 * w + 1][j / 2]);
         const uint4 vt = make_uint4(op[0], op[1], op[2], op[3]);
-        acc[h * VE + j] = mfma_16<TYPE>(vt, pg, mfma_16<TYPE>(vt, pf, acc[h * VE + j]));
+#pragma unroll
+        for (int k = 0; k < NP; ++k) acc[h * VE + j] = mfma_16<TYPE>(vt, pf[k], acc[h * VE + j]);
       }
     }
   }

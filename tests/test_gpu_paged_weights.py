@@ -1,12 +1,12 @@
-"""Small weights in the paged decode attention, on the GPU against closed forms in
-64 bits.
+"""Small and cancelling weights in the paged decode attention, on the GPU against
+closed forms in 64 bits.
 
-The kernel takes a probability into its product with V as a sum of two 16-bit
-parts, off by at most 2^-17 (bf16) or 2^-23 (fp16) of it, in fp16 by 2^-39 of the
-largest among the 32 keys of its tile where that is more (half of fp16's smallest
-step, the largest scaled to 2^14 or more).  The tiles' largest sum to no more
-than all probabilities do, so fp16 loses at most 32·2^-39 = 2^-34 of the largest
-|v| of the output, however long the cache is."""
+The kernel takes a probability into its product with V as a sum of 16-bit parts:
+three in bf16, off by at most 2^-27 of it; two in fp16, off by at most 2^-23 of
+it, or by 2^-39 of the largest among the 32 keys of its tile where that is more
+(half of fp16's smallest step, the largest scaled to 2^14 or more).  The tiles'
+largest sum to no more than all probabilities do, so fp16 loses at most
+32·2^-39 = 2^-34 of the largest |v| of the output, however long the cache is."""
 from __future__ import annotations
 
 import pytest
@@ -68,9 +68,39 @@ def test_small_weights_add_up(ops, dtype, fp8, D, bs, T, sink):
     assert ((lse[0].double() - (gaps.double() + torch.log(whole))).abs() <= 2.0 ** -16 + 2.0 ** -22 * gaps).all()
     # (the result's rounding: half a step of it, or of the smallest number; scores up to 24 in log2 units of 35, three
     # roundings of 2^-24 each, and the exponential's: 35·3·2^-24 + 2^-22 of a weight; sums of partial sums 2^-16)
-    rel = (2.0 ** -23 if dtype == "fp16" else 2.0 ** -17) + 105 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -16
+    rel = 2.0 ** -23 + 105 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -16
     bound = (half_step(t) + rel) * want
     if dtype == "fp16":
         bound = bound + 2.0 ** -25 + 2.0 ** -34 * 1.5  # (|v| <= 1.5)
     over = (out[0].double() - want).abs() - bound
     assert over.max() <= 0, f"gap {gaps[int(over.amax(1).argmax())].item()}: {over.max().item():.3e} over its bound"
+
+
+@pytest.mark.parametrize("dtype,fp8", [("fp16", False), ("fp16", True), ("bf16", False), ("bf16", True)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_weights_that_cancel(ops, dtype, fp8, D):
+    """Two keys whose weighted values cancel but for the rounding of one of them: what is left shows
+    a weight's error."""
+    t, B, H = TYPES[dtype], 32, 4
+    page_t = torch.float8_e4m3fn if fp8 else t
+    g = torch.Generator(device=DEV).manual_seed(D)
+    gap = (0.01 + 0.09 * torch.rand((B, H), generator=g, device=DEV)).to(t)
+    q = torch.zeros((B, H, D), dtype=t, device=DEV)
+    q[:, :, 0] = gap
+    w = torch.exp(-gap.double())
+    a = (0.5 + torch.rand((B, H, D), generator=g, device=DEV)).to(page_t).double()
+    k, v = (torch.zeros((B, 2, H, D), device=DEV) for _ in range(2))
+    k[:, 0, :, 0] = 1.0
+    v[:, 0] = a.float()
+    v[:, 1] = -(a / w[..., None]).float().to(page_t).float()
+    kp, table = paged(k, 16, 2)
+    vp, _ = paged(v, 16, 2)
+    out, _ = ops.paged_decode_attn(q, kp.to(page_t), vp.to(page_t), table, torch.full((B,), 2, device=DEV), scale=1.0)
+    b = v[:, 1].double()
+    want = (a + w[..., None] * b) / (1 + w[..., None])
+    spread = (a.abs() + w[..., None] * b.abs()) / (1 + w[..., None])
+    # parts at most 2^-23; the exponential 2^-22 and its argument, a difference of numbers up to 0.15, 2^-25;
+    # a few fp32 additions and the division, 2^-21 in all
+    bound = half_step(t) * want.abs() + 2.0 ** -20 * spread + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    over = (out.double() - want).abs() - bound
+    assert over.max() <= 0, f"{over.max().item():.3e} over its bound, {(over > 0).double().mean().item():.3f} of the outputs"
