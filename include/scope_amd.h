@@ -691,7 +691,9 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
  * kv_num [B][Hkv] (entries outside [0, MP) are skipped, kv_num is kept to
  * [0, maxkv]; an entry listed twice counts twice).
  *   out [B][Hq][D]     softmax(scale · q·k) · v; zeros where nothing is seen; an
- *                      infinite value of v in a seen row gives inf or NaN
+ *                      infinite value of v in a seen row gives that infinity (or
+ *                      NaN, where the row's weight is below 2^-15 in fp16, 2^-100
+ *                      in bf16, of the largest among the 32 positions around it)
  *   lse [B][Hq]        natural logarithm of the sum; -inf there
  *   mass [B][Hkv][MP]  or NULL: each block's probabilities, summed over its
  *                      positions and the group's query heads, are added (lists

@@ -297,6 +297,16 @@ __device__ __forceinline__ uint32_t round2(float lo, float hi) {
   }
 }
 
+// the largest 16-bit values below two positive numbers (0 below 0)
+template <int TYPE>
+__device__ __forceinline__ uint32_t below2(float lo, float hi) {
+  const uint32_t a = __builtin_elementwise_sub_sat(__float_as_uint(lo), 1u), b = __builtin_elementwise_sub_sat(__float_as_uint(hi), 1u);
+  if constexpr (TYPE == SCOPE_BF16)
+    return pack_hi16(a, b);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(a), __uint_as_float(b)));
+}
+
 // the halves of a word of two 16-bit values
 template <int TYPE>
 __device__ __forceinline__ float low_half(uint32_t w) {
@@ -351,8 +361,12 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // relative to moves only when a score passes it by more than 8 (p <= 256 until
 // then, no loss in floating point).  For the product with V, whose instruction
 // takes 16-bit operands, a probability is the sum of 16-bit values: three in bf16
-// (off by 2^-27 of it, less than fp32 itself; two, off by 2^-17, were 1% faster in
-// e4m3 and no faster in bf16), two in fp16 (2^-23).
+// (two, off by 2^-17 of it, were 1% faster in e4m3 and no faster in bf16), two in
+// fp16.  All but the last are the largest below what is left, so that none is
+// negative, nor 0 unless the probability is small (bf16 2^-100, fp16 2^-15 of its
+// tile's largest): an infinite value of V stays one.  That leaves an error of 2^-23
+// (bf16), 2^-21 (fp16) of a probability.  e4m3 has no infinities: rounded to nearest,
+// 2^-27 and 2^-23.
 // fp16 has no exponents for the small weights of a long cache (below 2^-25 a key
 // would count in the sum and not in the output: behind one key that takes nearly all
 // of the weight, 131k others 17.4 nats lower came out as 0).  There the
@@ -361,8 +375,7 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // of its tile's largest (half of fp16's smallest step), all of them by 2^-34 of the
 // sum.  That costs up to 1% (48 windows of 4096 at D = 64 53.8 us either way, 32
 // sequences to 16k at D = 128 58.8 -> 59.1); a tile's product of its own, joined by an
-// fp32 factor, spills at D = 128 (79.7).  (The
-// later values may be 0 or negative: an infinite value of V can come out as NaN.)
+// fp32 factor, spills at D = 128 (79.7).
 // Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
 // 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
 // GB) 5.6 TB/s with the launch behind it.  V passes the caches (131k
@@ -577,7 +590,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = round2<TYPE>(x[2 * i], x[2 * i + 1]);
+        w[i] = k + 1 < NP && !FP8 ? below2<TYPE>(x[2 * i], x[2 * i + 1]) : round2<TYPE>(x[2 * i], x[2 * i + 1]);
         x[2 * i] -= low_half<TYPE>(w[i]);
         x[2 * i + 1] -= high_half<TYPE>(w[i]);
       }

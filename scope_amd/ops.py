@@ -1244,7 +1244,9 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     its block has a page, and with lists where its block is among kv_idx [B,
     Hkv, maxkv] up to kv_num [B, Hkv] (blocks of bs positions; those outside
     the table are skipped).  A row that sees nothing gives 0 and lse -inf; an
-    infinite value of v in a seen row gives inf or NaN.
+    infinite value of v in a seen row gives that infinity (or NaN, where the
+    row's weight is below 2^-15 in fp16, 2^-100 in bf16, of the largest among
+    the 32 positions around it).
     ``mass`` [B, Hkv, MP] fp32 contiguous gets each block's probabilities,
     summed over its positions and the group's query heads, added in place
     (lists without repeats then; not two calls on one mass at a time).
