@@ -1163,10 +1163,11 @@ def _ints(who: str, name: str, x, n: int, dev: torch.device) -> torch.Tensor | N
 
 
 @functools.lru_cache(maxsize=256)
-def _paged_work_bytes(B: int, Hkv: int, D: int, bs: int, MP: int, Hq: int, maxkv: int, with_mass: bool) -> int:
-    """The attention's workspace, a function of these sizes alone."""
+def _paged_work_bytes(ask, B: int, Hkv: int, D: int, bs: int, MP: int, Hq: int, maxkv: int, with_mass: bool) -> int:
+    """The attention's workspace, a function of these sizes alone (and of ``ask``, the
+    call to the library: what another one answered is not kept for this one)."""
     c = _lib.PagedCache(B, Hkv, D, bs, MP)
-    return query("scope_paged_attn_workspace_bytes", C.byref(c), Hq, maxkv, int(with_mass))
+    return ask("scope_paged_attn_workspace_bytes", C.byref(c), Hq, maxkv, int(with_mass))
 
 
 def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, dtype: torch.dtype,
@@ -1276,7 +1277,7 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     first = _ints(who, "first", first, B, dev)
     out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=dev)
     lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
-    need = _paged_work_bytes(B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
+    need = _paged_work_bytes(query, B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _launch(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0,
              qs[1] if Hq > 1 else 0, k_pages.data_ptr(),
