@@ -204,21 +204,7 @@ struct PagedAttnArgs {
 
 // Workgroups of kAttnWaves wavefronts; piece i of the batch (paged_plan.h) is
 // blockIdx.x, (key head, group of 16 query heads) blockIdx.y.
-constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = 64 * kAttnWaves;
-
-// A piece's least tiles: short rows wait less in more pieces (1100 positions of 8
-// heads 10.0 us with 2, 12.2 with 4, 15.2 with 16; lists of nine blocks of 128 8.2,
-// 8.6 and 11.3).
-constexpr int kPieceTiles = 2;
-
-// Workgroups aimed at.  The pieces of a ragged batch are not equal, and smaller ones
-// even out its end (64 query heads over 24 sequences of 9k to 65k: 1536 270 us, 1024
-// 280, 768 313); one sequence's are (131k positions: 1024 96 us, 1536 98), and at D =
-// 256 the partial rows are longer (16 sequences to 16k: 1024 107 us, 1536 114; in
-// whole turns of the wavefronts, which change nothing elsewhere, 102).
-constexpr int kMostPieces = 1536;
-constexpr int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
 
 struct AttnSplit {
   int pieces, slots;   // pieces aimed at and slots of a (key head, group); with lists: pieces of every list
@@ -420,7 +406,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     p.slot = p.b * s.pieces;
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
-  } else if (!find_piece(c, a, s, blockIdx.x, D == 256 ? kAttnWaves : 1, p)) {
+  } else if (!find_piece(c, a, s, blockIdx.x, piece_turn(D), p)) {
     return;
   }
   const int b = p.b;
@@ -1016,27 +1002,18 @@ int check_cache(const scope_paged_cache* c, const void* k_pages, const void* v_p
 // The pieces of a call and its workspace (laid out in `work` where s is given);
 // returns its bytes.
 int64_t plan_split(const scope_paged_cache& c, int Hq, int maxkv, bool with_mass, AttnSplit* out, void* work) {
-  const int G = Hq / c.Hkv, ng = (G + 15) / 16;
-  const int64_t keys = static_cast<int64_t>(maxkv ? maxkv : c.MP) * c.bs;
+  const SplitSizes z = split_sizes(c.B, c.Hkv, c.D, c.bs, c.MP, Hq, maxkv);
   AttnSplit s{};
-  s.tiles_cap = (keys + kTileKeys - 1) / kTileKeys;
-  const int64_t cols = static_cast<int64_t>(c.Hkv) * ng * (maxkv ? c.B : 1);
-  const int64_t most = (s.tiles_cap + kPieceTiles - 1) / kPieceTiles;
-  const int want = pieces_wanted(c.B, c.D);
-  s.pieces = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((want + cols - 1) / cols, maxkv ? most : want)));
-  const bool split = most > 1 && s.pieces > 1;
-  // (the pieces of a batch are no more than those aimed at and one a sequence, nor
-  // than the shortest ones that a table row holds)
-  s.slots = static_cast<int>(maxkv ? static_cast<int64_t>(s.pieces) * c.B
-                                   : split ? std::min<int64_t>(s.pieces + c.B, most * c.B) : c.B);
-  if (!split) s.pieces = 1;
+  s.pieces = z.pieces;
+  s.slots = z.slots;
+  s.tiles_cap = z.tiles_cap;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     char* p = work ? static_cast<char*>(work) + at : nullptr;
     at += (bytes + 15) & ~static_cast<int64_t>(15);
     return p;
   };
-  if (split) {
+  if (z.split) {
     s.po = reinterpret_cast<float*>(take(4ll * s.slots * Hq * c.D));
     s.pml = reinterpret_cast<float*>(take(8ll * s.slots * Hq));
     s.plan = reinterpret_cast<int2*>(take(8ll * c.B));

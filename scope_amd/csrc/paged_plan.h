@@ -20,6 +20,23 @@ namespace scope {
 
 constexpr int kTileKeys = 32;
 
+// wavefronts of a piece's workgroup, which take its tiles in turn
+constexpr int kAttnWaves = 4;
+
+// A piece's least tiles: short rows wait less in more pieces (1100 positions of 8
+// heads 10.0 us with 2, 12.2 with 4, 15.2 with 16; lists of nine blocks of 128 8.2,
+// 8.6 and 11.3).
+constexpr int kPieceTiles = 2;
+
+// Workgroups aimed at.  The pieces of a ragged batch are not equal, and smaller ones
+// even out its end (64 query heads over 24 sequences of 9k to 65k: 1536 270 us, 1024
+// 280, 768 313); one sequence's are (131k positions: 1024 96 us, 1536 98), and at D =
+// 256 the partial rows are longer (16 sequences to 16k: 1024 107 us, 1536 114; in
+// whole turns of the wavefronts, which change nothing elsewhere, 102).
+constexpr int kMostPieces = 1536;
+SCOPE_HD int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
+SCOPE_HD int piece_turn(int D) { return D == 256 ? kAttnWaves : 1; }
+
 // positions that a sequence of `len` holds in a table row of `cap`
 SCOPE_HD int64_t seq_end(int64_t len, int64_t cap) { return len < 0 ? 0 : len < cap ? len : cap; }
 
@@ -33,8 +50,8 @@ SCOPE_HD int seq_tiles(int64_t len, int64_t first, int64_t cap, int* lo) {
   return static_cast<int>((end + kTileKeys - 1) / kTileKeys) - *lo;
 }
 
-// tiles of a piece, for a batch of `total` tiles and about `pieces` of them: a
-// multiple of `turn`, `least` at least
+// tiles of a piece at most, for a batch of `total` tiles and about `pieces` of them:
+// `least`, or a multiple of `turn` above it (piece_range evens out a sequence's)
 SCOPE_HD int64_t piece_tiles(int64_t total, int pieces, int least, int turn) {
   const int64_t c = (total + pieces - 1) / pieces, d = (c + turn - 1) / turn * turn;
   return c > least ? d : least;
@@ -46,6 +63,30 @@ SCOPE_HD int64_t piece_tiles(int64_t total, int pieces, int least, int turn) {
 SCOPE_HD int seq_pieces(int tiles, int64_t piece) {
   const int n = tiles <= piece ? 1 : static_cast<int>((tiles + piece - 1) / piece);
   return n;
+}
+
+// The pieces aimed at and the slots of a (key head, group of 16 query heads): what
+// the grid and the workspace are made for.  With lists (of maxkv entries; 0: none)
+// every list is cut into `pieces`.
+struct SplitSizes {
+  int pieces, slots;
+  int64_t tiles_cap;  // tiles of a full table row (list)
+  bool split;         // some sequence may take more than one piece
+};
+SCOPE_HD SplitSizes split_sizes(int B, int Hkv, int D, int bs, int MP, int Hq, int maxkv) {
+  SplitSizes s;
+  const int G = Hq / Hkv, ng = (G + 15) / 16, want = pieces_wanted(B, D);
+  s.tiles_cap = (static_cast<int64_t>(maxkv ? maxkv : MP) * bs + kTileKeys - 1) / kTileKeys;
+  const int64_t cols = static_cast<int64_t>(Hkv) * ng * (maxkv ? B : 1);
+  const int64_t most = (s.tiles_cap + kPieceTiles - 1) / kPieceTiles;  // the shortest pieces of a full row
+  const int64_t share = (want + cols - 1) / cols, pieces = maxkv && most < share ? most : share;
+  s.split = most > 1 && pieces > 1;
+  s.pieces = s.split ? static_cast<int>(pieces) : 1;
+  // (the pieces of a batch are no more than those aimed at and one a sequence, nor
+  // than the shortest ones that its table rows hold)
+  const int64_t ragged = s.pieces + B < most * B ? s.pieces + B : most * B;
+  s.slots = maxkv ? s.pieces * B : s.split ? static_cast<int>(ragged) : B;
+  return s;
 }
 
 // tiles [*t0, *t1) of piece i of n
