@@ -1045,7 +1045,7 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
   SCOPE_REQUIRE(k && v && table && lens, "%s: null pointer", fn);
   SCOPE_REQUIRE(aligned16(k) && aligned16(v) && k_sn % 8 == 0 && k_sh % 8 == 0 && v_sn % 8 == 0 && v_sh % 8 == 0,
                 "%s: the rows of k and v must be 16-byte aligned", fn);
-  const int rows = N >= 8192 ? 2 : 1;  // (one row a wavefront while that leaves the device wavefronts to spare)
+  const int rows = append_rows(N);
   const AppendArgs a{N, k_sn, k_sh, v_sn, v_sh, rows, k, v, cu, table, lens, k_scale, v_scale, k_pages, v_pages};
   const dim3 grid(ceil_div(N, 4 * rows)), block(256);
   hipStream_t st = as_stream(stream);

@@ -103,6 +103,18 @@ SCOPE_HD int64_t block_page(const int32_t* row, int MP, int64_t lb, int64_t P) {
   return page >= 0 && page < P ? page : -1;
 }
 
+// work-items that one dimension of a grid holds
+constexpr int64_t kGridItems = (static_cast<int64_t>(1) << 32) - 1;
+
+// rows of a wavefront that appends N of them, four wavefronts a workgroup: one while
+// that leaves the device wavefronts to spare, two from 8192 on, and as many as the
+// grid needs (up to 64, for 2^31 - 1)
+SCOPE_HD int append_rows(int64_t N) {
+  int rows = N >= 8192 ? 2 : 1;
+  while ((N + 4 * rows - 1) / (4 * rows) * 256 > kGridItems) rows *= 2;
+  return rows;
+}
+
 // where row i of the new ones goes: its sequence in *b and its position, -1 for
 // a row of no sequence.  cu [B + 1] or null (row i to sequence i); whatever cu
 // holds, *b stays in [0, B).

@@ -44,6 +44,7 @@ int64_t found(int B, int D, int64_t cap, const int32_t* lens, const int32_t* fir
   }
   return n_all;
 }
+int rows_each(int64_t N) { return append_rows(N); }
 int list_range(int tiles_cap, int pieces) {
   int at = 0;
   for (int i = 0; i < pieces; ++i) {
@@ -66,6 +67,7 @@ def plan(tmp_path_factory):
                     str(d / "plan.cpp"), "-o", str(d / "plan.so")], check=True)
     lib = C.CDLL(str(d / "plan.so"))
     lib.found.restype, lib.found.argtypes = C.c_int64, [C.c_int, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
+    lib.rows_each.restype, lib.rows_each.argtypes = C.c_int, [C.c_int64]
     lib.sizes.restype, lib.sizes.argtypes = None, [C.c_int] * 7 + [C.c_void_p]
     return lib
 
@@ -127,3 +129,12 @@ def test_the_workspace_holds_the_slots(plan, seed):
         assert lib.scope_paged_attn_workspace_bytes(C.byref(c), Hq, maxkv, 0) == want
         want += up(4 * B * Hq) + up(4 * B * Hq * cap * (2 if bs == 16 else 1))
         assert lib.scope_paged_attn_workspace_bytes(C.byref(c), Hq, maxkv, 1) == want
+
+
+def test_appended_rows_fit_a_grid(plan):
+    """A launch holds less than 2^32 work-items; a wavefront places up to 64 rows."""
+    edges = [1, 8191, 8192, 2 ** 27 - 8, 2 ** 27 - 7, 2 ** 27, 2 ** 28, 2 ** 29 - 1, 2 ** 30 + 1, 2 ** 31 - 1]
+    for n in edges + [random.Random(i).randint(1, 2 ** 31 - 1) for i in range(200)]:
+        rows = plan.rows_each(n)
+        assert 1 <= rows <= 64 and -(-n // (4 * rows)) * 256 < 2 ** 32
+    assert [plan.rows_each(n) for n in (8191, 8192, 2 ** 27 - 8, 2 ** 27 - 7)] == [1, 2, 2, 4]
