@@ -729,6 +729,8 @@ int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, 
  *   then z - presence;  z + bias[b][v] (row stride bias_sb, 0 for one row);
  *   z / temperature;  -inf where bit v % 32 of mask[b][v / 32] (row stride
  *   mask_sb) is 0.
+ * One launch: about 2^35 logits at most (2^32 threads of 8 words, rows rounded up
+ * to whole workgroups), others are refused.
  * repetition, presence, frequency and temperature are [B] arrays, or NULL for
  * the parameters' numbers; repetition and temperature are positive. */
 typedef struct {

@@ -209,7 +209,9 @@ extern "C" int scope_logit_penalties(const scope_penalty_params* p, const void* 
   const bool lng = p->T > kLongHistory;
   const int threads = lng ? 1024 : 512, rows = lng ? ceil_div(p->B, kXcds) * kXcds : p->B;
   const int64_t groups = static_cast<int64_t>(rows) * ceil_div(p->V, threads * kPenWords);
-  SCOPE_REQUIRE(groups <= INT32_MAX, "%s: %d rows of %lld words are more than one launch holds", fn, p->B, (long long)p->V);
+  // (a grid holds less than 2^32 work-items)
+  SCOPE_REQUIRE(groups * threads <= UINT32_MAX, "%s: %d rows of %lld words are more than one launch holds (about 2^35 in all)", fn,
+                p->B, (long long)p->V);
   const dim3 grid(static_cast<uint32_t>(groups)), block(threads);
   hipStream_t st = as_stream(stream);
   const auto launch = [&](auto type) {

@@ -60,3 +60,16 @@ def test_a_workspace_size_is_the_librarys_own(on_cpu, monkeypatch):
         call()
     p = _lib.PagedCache(2, 2, 64, 16, MP)
     assert sizes == [_lib.load().scope_paged_attn_workspace_bytes(C.byref(p), 4, 3, 1)] and sizes[0] > 16
+
+
+@needs_lib
+def test_more_logits_than_a_launch_holds_are_refused():
+    """2^32 work-items or more: the stated refusal, before the launch (the pointers are never followed)."""
+    from scope_amd import _lib
+
+    lib, one = _lib.load(), C.c_void_p(16)
+    # (512 threads of 8 words, and 1024 with rows in eights where the history is long)
+    for B, V, T in ((65535, 2 ** 19 + 1, 5), (65535, 2 ** 31 - 1, 5), (32768, 2 ** 20, 5), (65529, 524289, 20000), (32761, 2 ** 20, 20000)):
+        p = _lib.PenaltyParams(B=B, type=2, V=V, T=T, repetition=1.0, temperature=1.0)
+        rc = lib.scope_logit_penalties(C.byref(p), one, one, one, *[None] * 8, one, None)
+        assert rc == -1 and "more than one launch holds" in lib.scope_last_error().decode(), lib.scope_last_error()
