@@ -1151,11 +1151,12 @@ def _sat32(x: torch.Tensor) -> torch.Tensor:
 
 
 def _ints(who: str, name: str, x, n: int, dev: torch.device) -> torch.Tensor | None:
-    """n int32 numbers on dev: of an integer tensor of n elements, or one number for all."""
+    """n int32 numbers on dev: of an integer tensor of n elements, or one number for all;
+    those past 32 bits as ``_sat32`` takes them."""
     if x is None:
         return None
     if not isinstance(x, torch.Tensor):
-        return torch.full((n,), int(x), dtype=torch.int32, device=dev)
+        return torch.full((n,), max(-2 ** 31, min(int(x), 2 ** 31 - 1)), dtype=torch.int32, device=dev)
     dt = x.dtype
     if x.numel() != n or (dt != torch.int32 and dt != torch.int64):
         raise RuntimeError(f"{who}: {name} must be int32 or int64 [{n}] (got {x.dtype} {tuple(x.shape)})")

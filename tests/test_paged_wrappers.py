@@ -73,3 +73,25 @@ def test_more_logits_than_a_launch_holds_are_refused():
         p = _lib.PenaltyParams(B=B, type=2, V=V, T=T, repetition=1.0, temperature=1.0)
         rc = lib.scope_logit_penalties(C.byref(p), one, one, one, *[None] * 8, one, None)
         assert rc == -1 and "more than one launch holds" in lib.scope_last_error().decode(), lib.scope_last_error()
+
+
+@pytest.mark.parametrize("x,want", [(2 ** 63 - 1, 2 ** 31 - 1), (2 ** 40, 2 ** 31 - 1), (-2 ** 40, -2 ** 31), (2 ** 31, 2 ** 31 - 1), (10 ** 30, 2 ** 31 - 1),
+                                    (2 ** 31 - 1, 2 ** 31 - 1), (-2 ** 31, -2 ** 31), (7, 7), (-1, -1), (True, 1)])
+def test_numbers_past_32_bits_stay_on_their_side(on_cpu, x, want):
+    """A number counts as a tensor of it does."""
+    ops = on_cpu
+    dev = torch.device("cpu")
+    assert ops._ints("x", "x", x, 3, dev).tolist() == [want] * 3
+    if -2 ** 63 <= x < 2 ** 63 and not isinstance(x, bool):
+        assert ops._ints("x", "x", torch.tensor([x] * 3), 3, dev).tolist() == [want] * 3
+
+
+def test_calls_with_numbers_past_32_bits_are_made(on_cpu):
+    ops = on_cpu
+    table, mass, lens = torch.zeros((2, 5), dtype=torch.int32), torch.zeros((2, 1, 5)), torch.tensor([80, 3])
+    with pytest.raises(Reached):
+        ops.paged_evict(table, mass, lens, 2 ** 63 - 1, bs=16)
+    z, t = torch.zeros(2, 70), torch.zeros(2, 9, dtype=torch.int64)
+    for kw in (dict(n_prompt=2 ** 63 - 1), dict(first=2 ** 40), dict(first=-2 ** 40)):
+        with pytest.raises(Reached):
+            ops.logit_penalties(z, t, 2 ** 40, **kw)
