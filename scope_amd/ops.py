@@ -1109,7 +1109,7 @@ def decoder_step(prm, table: torch.Tensor, work: torch.Tensor, tok: torch.Tensor
 # ---- the paged cache of a decode loop over several sequences --------------------
 _PAGED_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _FP8 = torch.float8_e4m3fn
-EVICT_MAX_PAGES = 65536  # include/scope_amd.h SCOPE_PAGED_EVICT_MAX_PAGES
+_INT_MAX = 2 ** 31 - 1  # (a C int takes the low 32 bits of what is larger)
 
 
 def _device(who: str, first: torch.Tensor, *ts: torch.Tensor | None) -> torch.device:
@@ -1181,8 +1181,8 @@ def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: 
     if (dtype != torch.bfloat16 and dtype != torch.float16) or not (fp8 or pt == dtype):
         raise RuntimeError(f"{who}: bfloat16 or float16 rows with pages of their type or float8_e4m3fn "
                            f"(got {dtype} and {pt})")
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
-        raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP]")
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.numel() > _INT_MAX:
+        raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP] of less than 2^31 entries")
     P, Hkv, bs, D = shape
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
         if t is not None and (not fp8 or t.dtype != torch.float32 or t.numel() != Hkv or not t.is_contiguous()):
@@ -1266,7 +1266,7 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     if kv_num is not None or kv_idx is not None:
         if kv_num is None or kv_idx is None:
             raise RuntimeError(f"{who}: kv_num and kv_idx come together")
-        if kv_idx.dim() != 3 or kv_idx.shape[2] < 1 or kv_idx.shape[:2] != (B, Hkv) or kv_num.shape != (B, Hkv):
+        if kv_idx.dim() != 3 or not 1 <= kv_idx.shape[2] <= _INT_MAX or kv_idx.shape[:2] != (B, Hkv) or kv_num.shape != (B, Hkv):
             raise RuntimeError(f"{who}: kv_num must be [{B}, {Hkv}] and kv_idx [{B}, {Hkv}, maxkv]")
         if kv_num.is_floating_point() or kv_idx.is_floating_point():
             raise RuntimeError(f"{who}: kv_num and kv_idx must be integers (got {kv_num.dtype} and {kv_idx.dtype})")
@@ -1302,8 +1302,8 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     table itself); freed holds their pages in the blocks' order, then -1."""
     who = "paged_evict"
     dev = _device(who, table, mass, lens, budget if isinstance(budget, torch.Tensor) else None, out)
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
-        raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP]")
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.numel() > _INT_MAX:
+        raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP] of less than 2^31 entries")
     B, MP = table.shape
     ms = mass.shape
     if mass.dtype != torch.float32 or len(ms) != 3 or ms[0] != B or ms[2] != MP or not mass.is_contiguous():
@@ -1317,6 +1317,8 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     freed = torch.empty_like(table)
     n_freed = torch.empty(B, dtype=torch.int32, device=dev)
     window, n_global = min(int(window), MP), min(int(n_global), MP)  # (a C int each; MP keeps every block)
+    if not 1 <= bs <= _INT_MAX:
+        raise RuntimeError(f"{who}: bs={bs} must be 1 .. 2^31 - 1")
     if window < 1 or n_global < 0:
         raise RuntimeError(f"{who}: window={window} must be at least 1 (the page being written stays), n_global={n_global} at least 0")
     _launch(dev, "scope_paged_evict", B, ms[1], MP, int(bs), window, n_global, table.data_ptr(), mass.data_ptr(),

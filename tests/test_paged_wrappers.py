@@ -95,3 +95,17 @@ def test_calls_with_numbers_past_32_bits_are_made(on_cpu):
     for kw in (dict(n_prompt=2 ** 63 - 1), dict(first=2 ** 40), dict(first=-2 ** 40)):
         with pytest.raises(Reached):
             ops.logit_penalties(z, t, 2 ** 40, **kw)
+
+
+def test_sizes_past_a_c_int_are_refused(on_cpu):
+    """Not the page size or the table of their low 32 bits (the expanded tensors hold no memory)."""
+    ops = on_cpu
+    table, mass, lens = torch.zeros((2, 5), dtype=torch.int32), torch.zeros((2, 1, 5)), torch.tensor([80, 3])
+    for bs in (2 ** 32 + 16, 2 ** 31, 0, -16, 2 ** 32):
+        with pytest.raises(RuntimeError, match="paged_evict: bs="):
+            ops.paged_evict(table, mass, lens, 1, bs=bs)
+    c = cache([20, 5], Hq=4, Hkv=2, D=64, bs=16)
+    args = [c[k] for k in ("q", "k_pages", "v_pages", "table", "lens")]
+    idx = torch.zeros(1, dtype=torch.int32).expand(2, 2, 2 ** 32 + 3)
+    with pytest.raises(RuntimeError, match="kv_idx"):
+        ops.paged_decode_attn(*args, scale=0.1, kv_num=torch.ones(2, 2, dtype=torch.int32), kv_idx=idx)
