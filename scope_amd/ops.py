@@ -1109,6 +1109,7 @@ def decoder_step(prm, table: torch.Tensor, work: torch.Tensor, tok: torch.Tensor
 # ---- the paged cache of a decode loop over several sequences --------------------
 _PAGED_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _FP8 = torch.float8_e4m3fn
+_F32_MIN, _F32_MAX = 2.0 ** -126, (2 - 2.0 ** -23) * 2.0 ** 127
 _INT_MAX = 2 ** 31 - 1  # (a C int takes the low 32 bits of what is larger)
 
 
@@ -1376,9 +1377,9 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
         for name, x in zip(("repetition", "presence", "frequency", "temperature"), numbers):
             if isinstance(x, torch.Tensor) and (x.numel() != B or not x.is_floating_point()):
                 raise RuntimeError(f"{who}: {name} must be a number or a float tensor [{B}]")
-    if not (0.0 < num[0] < math.inf and 0.0 < num[3] < math.inf and math.isfinite(num[1]) and math.isfinite(num[2])):
-        raise ValueError(f"{who}: repetition and temperature must be finite and positive, presence and frequency finite (got "
-                         f"{num[0]}, {num[3]}, {num[1]} and {num[2]})")
+    if not (_F32_MIN <= num[0] <= _F32_MAX and _F32_MIN <= num[3] <= _F32_MAX and abs(num[1]) <= _F32_MAX and abs(num[2]) <= _F32_MAX):
+        raise ValueError(f"{who}: repetition and temperature must be finite and positive, presence and frequency finite, as fp32 "
+                         f"numbers (got {num[0]}, {num[3]}, {num[1]} and {num[2]})")
     lens64 = isinstance(lens, torch.Tensor) and lens.dtype == torch.int64 and lens.numel() == B and lens.is_contiguous()
     if not lens64:
         lens = _ints(who, "lens", lens, B, dev)

@@ -109,3 +109,17 @@ def test_sizes_past_a_c_int_are_refused(on_cpu):
     idx = torch.zeros(1, dtype=torch.int32).expand(2, 2, 2 ** 32 + 3)
     with pytest.raises(RuntimeError, match="kv_idx"):
         ops.paged_decode_attn(*args, scale=0.1, kv_num=torch.ones(2, 2, dtype=torch.int32), kv_idx=idx)
+
+
+def test_penalties_that_fp32_does_not_hold_are_refused(on_cpu):
+    """1e-50 and 1e50 are 0 and infinity to the kernel: a quotient by 0, a product of infinity and 0."""
+    ops = on_cpu
+    z, t = torch.zeros(2, 70), torch.zeros(2, 9, dtype=torch.int64)
+    for name in ("repetition", "temperature", "presence", "frequency"):
+        for x in (1e50, -1e50) + ((1e-50, 0.0, -1.0) if name in ("repetition", "temperature") else (float("nan"),)):
+            with pytest.raises(ValueError, match="logit_penalties"):
+                ops.logit_penalties(z, t, 3, **{name: x})
+        with pytest.raises(Reached):
+            ops.logit_penalties(z, t, 3, **{name: 2.0 ** -126})
+        with pytest.raises(Reached):
+            ops.logit_penalties(z, t, 3, **{name: 3.4e38})
