@@ -498,7 +498,9 @@ class ScopeDecoder(nn.Module):
             penalties = {"n_prompt": self.t, **penalties}
             for name in ("first", "n_prompt"):  # on the device once, not every step
                 if isinstance(penalties.get(name), int):
-                    penalties[name] = torch.tensor([penalties[name]], dtype=torch.int32, device=self.device)
+                    penalties[name] = ops._ints("generate", name, penalties[name], 1, self.device)
+            # what it refuses it refuses here, before a step has moved the position
+            ops.logit_penalties(torch.zeros(V, device=self.device), self.tokens, self._t_dev, **penalties)
         for s in range(n_steps):
             logits = self.step(tok)[:V]
             if penalties is not None:
