@@ -1143,6 +1143,20 @@ def _launch(dev: torch.device, name: str, *args) -> None:
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+class _NoGradient(torch.autograd.Function):
+    """Node of a call that has no backward: a gradient that reaches one of its
+    results is an error, not a silent zero."""
+
+    @staticmethod
+    def forward(ctx, who, call, *wanted):
+        ctx.who = who
+        return call()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.who} is not differentiable: detach its inputs or its results")
+
+
 def _sat32(x: torch.Tensor) -> torch.Tensor:
     """Integers as contiguous int32; those past 32 bits as the nearest one, on the
     same side of every length and index."""
@@ -1213,7 +1227,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing; without it N <= B
     and row i to sequence i), position lens[b] + i - cu[b].  Rows of no
     sequence, past the table, or of a block whose entry is outside [0, P) are
-    not written; no two rows may share a slot."""
+    not written; no two rows may share a slot.  The pages hold values: no
+    gradient passes through them to k and v."""
     who = "paged_append"
     dev = _device(who, k, v, k_pages, v_pages, table, lens, cu, k_scale, v_scale)
     dtype, shape, ks, vs = k.dtype, k.shape, k.stride(), v.stride()
@@ -1254,8 +1269,13 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     summed over its positions and the group's query heads, added in place
     (lists without repeats then; not two calls on one mass at a time).
     Nothing of it waits for the GPU or reads a length on the host, so a call
-    can be captured and replayed while the lengths and the table change."""
+    can be captured and replayed while the lengths and the table change.  It has
+    no backward: a gradient that reaches its results raises."""
     who = "paged_decode_attn"
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        return _NoGradient.apply(who, functools.partial(paged_decode_attn, q, k_pages, v_pages, table, lens, scale=scale, first=first,
+                                                        kv_num=kv_num, kv_idx=kv_idx, mass=mass, k_scale=k_scale, v_scale=v_scale),
+                                 q, k_pages, v_pages)
     dev = _device(who, q, k_pages, v_pages, table, lens, first, kv_num, kv_idx, mass, k_scale, v_scale)
     shape, qs, dtype = q.shape, q.stride(), q.dtype
     c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)
@@ -1347,8 +1367,13 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
     ``mask`` [W] or [B, W] int32 holds word v's bit at v % 32 of entry v // 32.
     repetition, presence, frequency and temperature are numbers or fp32 [B];
     repetition and temperature must be positive (numbers are checked).
-    ``out`` may be the logits themselves."""
+    ``out`` may be the logits themselves.  There is no backward: a gradient that
+    reaches the result raises (what is written to ``out`` leaves the graph)."""
     who = "logit_penalties"
+    if torch.is_grad_enabled() and out is None and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        return _NoGradient.apply(who, functools.partial(logit_penalties, logits, tokens, lens, first=first, n_prompt=n_prompt,
+                                                        repetition=repetition, presence=presence, frequency=frequency,
+                                                        temperature=temperature, bias=bias, mask=mask), logits, bias)
     numbers = (repetition, presence, frequency, temperature)
     dev = _device(who, logits, tokens, bias, mask, out,
                   *[x for x in (lens, first, n_prompt, *numbers) if isinstance(x, torch.Tensor)])

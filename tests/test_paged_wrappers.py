@@ -123,3 +123,30 @@ def test_penalties_that_fp32_does_not_hold_are_refused(on_cpu):
             ops.logit_penalties(z, t, 3, **{name: 2.0 ** -126})
         with pytest.raises(Reached):
             ops.logit_penalties(z, t, 3, **{name: 3.4e38})
+
+
+def test_a_gradient_that_reaches_the_results_raises(on_cpu, monkeypatch):
+    """Not a silent zero; without gradients, or with none asked for, nothing is recorded."""
+    ops = on_cpu
+    monkeypatch.setattr(ops, "_launch", lambda *a: None)
+    monkeypatch.setattr(ops, "query", lambda *a: 16)
+    c = cache([20, 5], Hq=4, Hkv=2, D=64, bs=16)
+    rest = [c[k] for k in ("k_pages", "v_pages", "table", "lens")]
+    q, mass = c["q"].clone().requires_grad_(), torch.zeros(2, 2, c["table"].shape[1])
+    out, lse = ops.paged_decode_attn(q, *rest, scale=0.1, mass=mass)
+    for y in (out, lse):
+        with pytest.raises(RuntimeError, match="paged_decode_attn is not differentiable"):
+            y.float().sum().backward()
+    z, t = torch.zeros(2, 70, requires_grad=True), torch.zeros(2, 9, dtype=torch.int64)
+    bias = torch.zeros(70, requires_grad=True)
+    for got in (ops.logit_penalties(z, t, 3, bias=bias.detach()), ops.logit_penalties(z.detach(), t, 3, bias=bias)):
+        assert got.shape == z.shape
+        with pytest.raises(RuntimeError, match="logit_penalties is not differentiable"):
+            got.sum().backward()
+    with torch.no_grad():
+        quiet = [*ops.paged_decode_attn(q, *rest, scale=0.1), ops.logit_penalties(z, t, 3, bias=bias)]
+    quiet += [*ops.paged_decode_attn(q.detach(), *rest, scale=0.1), ops.logit_penalties(z.detach(), t, 3)]
+    assert not any(y.requires_grad for y in quiet)
+    assert ops.logit_penalties(z.detach(), t, 3, out=z.detach()).requires_grad is False
+    with pytest.raises(RuntimeError, match="kv_num and kv_idx"):
+        ops.paged_decode_attn(q, *rest, scale=0.1, kv_num=torch.ones(2, 2, dtype=torch.int32))
