@@ -29,10 +29,13 @@ constexpr int kAttnWaves = 4;
 constexpr int kPieceTiles = 2;
 
 // Workgroups aimed at.  The pieces of a ragged batch are not equal, and smaller ones
-// even out its end (64 query heads over 24 sequences of 9k to 65k: 1536 270 us, 1024
-// 280, 768 313); one sequence's are (131k positions: 1024 96 us, 1536 98), and at D =
-// 256 the partial rows are longer (16 sequences to 16k: 1024 107 us, 1536 114; in
-// whole turns of the wavefronts, which change nothing elsewhere, 102).
+// even out its end (64 query heads over 24 sequences of 9k to 65k: 1536 272 us, 1024
+// 281, 768 313; 48 windows of 4096 at D = 64 54.1 and 57.3; 32 sequences to 16k 58.9
+// and 59.7; two to eight sequences of one length, which the host cannot tell, the
+// other way by 0.5 to 3%).  One sequence's are equal (131k positions: 1024 93.5 us,
+// 1536 96.0; 16k 22.8 and 23.9), and at D = 256 the partial rows are longer (16
+// sequences to 16k: 1024 107 us, 1536 114; in whole turns of the wavefronts, which
+// change nothing elsewhere, 102).
 constexpr int kMostPieces = 1536;
 SCOPE_HD int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
 SCOPE_HD int piece_turn(int D) { return D == 256 ? kAttnWaves : 1; }

@@ -17,12 +17,17 @@ namespace scope {
 namespace {
 constexpr int kPenWords = 8;  // of a thread
 constexpr int kXcds = 8;
-// Histories of up to this many tokens take 512 threads (4096 words) a workgroup,
-// whose waits are shorter (128 rows of 50304 words, histories to 8192: 16.3 us;
-// with 1024 threads 17.4).  Longer ones are read by fewer workgroups with 1024,
+// Room for up to this many tokens, or one row, takes 512 threads (4096 words) a
+// workgroup, whose waits are shorter (128 rows of 50304 words, histories to 8192,
+// everything on: 16.7 us, with 1024 threads 18.3; one row of 50257 words with room
+// for 131k and 1152 of them held 4.35 against 5.25, all of them held 16.1 against
+// 17.2).  Longer histories of several rows are read by fewer workgroups with 1024,
 // and those of a row follow each other on one XCD, so that its history comes into
 // one L2 (16 rows of 100003 words, histories of 60k to 131k: 19.0 us; on all XCDs
-// 22.1, with 512 threads 25.0).
+// 22.1, with 512 threads 26.3).  The host does not know the lengths: two to 32 rows
+// with such room take up to 1 us longer than with 512 threads while they hold little
+// of it (8 rows of 1152 5.4 against 4.6, 2 rows of 20000 7.3 against 6.4) and 5 to 6
+// less where it is full (8 rows of 131k 17.6 against 23.6).
 constexpr int64_t kLongHistory = 16384;
 }  // namespace
 
@@ -206,7 +211,7 @@ extern "C" int scope_logit_penalties(const scope_penalty_params* p, const void* 
   SCOPE_REQUIRE(p->type == SCOPE_BF16 || p->type == SCOPE_FP16 || p->type == SCOPE_FP32, "%s: unknown type %d", fn, p->type);
   SCOPE_REQUIRE(logits && out && lens && (tokens || p->T == 0), "%s: null pointer", fn);
   const PenaltyArgs a{logits, tokens, lens, first, n_prompt, repetition, presence, frequency, temperature, bias, mask, out};
-  const bool lng = p->T > kLongHistory;
+  const bool lng = p->T > kLongHistory && p->B > 1;
   const int threads = lng ? 1024 : 512, rows = lng ? ceil_div(p->B, kXcds) * kXcds : p->B;
   const int64_t groups = static_cast<int64_t>(rows) * ceil_div(p->V, threads * kPenWords);
   // (a grid holds less than 2^32 work-items)
