@@ -695,6 +695,9 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
  *                      NaN, where the row's weight is below 2^-15 in fp16, 2^-100
  *                      in bf16, of the largest among the 32 positions around it)
  *   lse [B][Hq]        natural logarithm of the sum; -inf there
+ *   work               scope_paged_attn_workspace_bytes; with a mass it grows with
+ *                      the table's width, whatever the lengths: 4·B·Hq·MP·bs/32
+ *                      bytes beside the pieces' rows, twice that for bs = 16
  *   mass [B][Hkv][MP]  or NULL: each block's probabilities, summed over its
  *                      positions and the group's query heads, are added (lists
  *                      without repeats; two calls on one mass at a time race) */
@@ -706,7 +709,8 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
                             float* lse, void* stream);
 
 /* Takes the pages of least accumulated weight out of the table.  Of sequence
- * b's n = ceil(lens[b] / bs) blocks those with a table entry >= 0 are held;
+ * b's n = ceil(lens[b] / bs) blocks those with a table entry >= 0 are held (one
+ * past the pool too, which is no page to the others: the pool is not given here);
  * the first n_global blocks and the last `window` (at least 1) stay.  Where
  * more than budget[b] are held, the surplus goes: the blocks of least
  * Σ_h mass[b][h][i] (summed in fp64, compared in fp32; NaN above everything;

@@ -76,7 +76,7 @@ __device__ __forceinline__ float max_of(float v) {
 // r-th row (a search, two loads), so the chain of loads is paid once for all of
 // them, then every row moves 16 bytes a lane.  65539 rows of 8 heads of 128: into
 // e4m3 77 us, 5.2 TB/s, as a large copy (one row a wavefront 86, eight 88; 82
-// with loads and stores through the caches); 16-bit pages 106 us, 5.1 TB/s
+// with loads and stores through the caches); 16-bit pages 105 us, 5.1 TB/s
 // (there past the caches 108).
 struct AppendArgs {
   int64_t N, k_sn, k_sh, v_sn, v_sh;
@@ -364,7 +364,9 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // fp32 factor, spills at D = 128 (79.7).
 // Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
 // 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
-// GB) 5.6 TB/s with the launch behind it.  V passes the caches (131k
+// GB) 5.5 TB/s with the launch behind it.  Groups of more than 16 query heads read K
+// and V once for every 16 (8 sequences of 60k on one key head: 16 heads 59 us, 32 87,
+// 64 145).  V passes the caches (131k
 // positions with the launch behind it 96 us, through them 105); K does not (the same
 // 96 past them, but 1100 positions 10.0 -> 10.7 us).  More in flight (two tiles at
 // once, the next one's loads ahead) changed nothing.
@@ -818,9 +820,10 @@ __device__ __forceinline__ uint32_t weight_key(float f) {
 // digits found so far are counted by their next one in LDS, and the digit is
 // where the running count passes n.  Blocks with a smaller key go, of those with
 // the same key the first ones.  Bound by latency: one sequence of 1027 blocks and
-// 8 heads 7.0 us (10.8 with the key found two bits at a time by ballots), 64 of
-// 8192 blocks 15.1 us for 17 MB (a workgroup a sequence; 37.6 with the ballots
-// and 16 loads a thread under way instead of 32).
+// 8 heads 6.3 us (10.8 with the key found two bits at a time by ballots), 64 of
+// 8192 blocks 14.5 us for 15 MB (a workgroup a sequence; 37.6 with the ballots
+// and 16 loads a thread under way instead of 32), one of 16384 20.4, of 16385 38.7
+// and of 65536 72 us (64 blocks a thread).
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 
 constexpr int kDigit = 11, kBins = 1 << kDigit;

@@ -1243,8 +1243,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     cu = _ints(who, "cu", cu, c.B + 1, dev)
     N, one = shape[0], c.Hkv == 1
     _launch(dev, "scope_paged_append", C.byref(c), N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1],
-             v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1], _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(),
-             v_pages.data_ptr())
+            v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1], _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale),
+            _ptr(v_scale), k_pages.data_ptr(), v_pages.data_ptr())
 
 
 def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -1267,7 +1267,8 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     the 32 positions around it).
     ``mass`` [B, Hkv, MP] fp32 contiguous gets each block's probabilities,
     summed over its positions and the group's query heads, added in place
-    (lists without repeats then; not two calls on one mass at a time).
+    (lists without repeats then; not two calls on one mass at a time).  Its
+    workspace grows with the table's width: 4 · B · Hq · MP · bs / 32 bytes.
     Nothing of it waits for the GPU or reads a length on the host, so a call
     can be captured and replayed while the lengths and the table change.  It has
     no backward: a gradient that reaches its results raises."""
@@ -1302,9 +1303,8 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     need = _paged_work_bytes(query, B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _launch(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0,
-             qs[1] if Hq > 1 else 0, k_pages.data_ptr(),
-             v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _ptr(first),
-             _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr())
+            qs[1] if Hq > 1 else 0, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(),
+            lens.data_ptr(), _ptr(first), _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr())
     return out, lse
 
 
@@ -1314,7 +1314,8 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     table -> (table [B, MP], freed [B, MP], n_freed [B]), all int32.
 
     Of sequence b's ceil(lens[b] / bs) blocks those with a table entry >= 0
-    are held.  Where more than budget[b] (a tensor [B] or one number) are, the
+    are held (one past the pool too, which the pool's other users take for no
+    page: the pool is not given here).  Where more than budget[b] (a tensor [B] or one number) are, the
     surplus goes: the blocks of least Σ_h mass[b, h, i] (mass [B, Hkv, MP]
     fp32; summed in 64 bits, compared in 32; NaN above everything, the lower
     index on ties), except the first ``n_global`` blocks and the last
@@ -1343,7 +1344,7 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
     if window < 1 or n_global < 0:
         raise RuntimeError(f"{who}: window={window} must be at least 1 (the page being written stays), n_global={n_global} at least 0")
     _launch(dev, "scope_paged_evict", B, ms[1], MP, int(bs), window, n_global, table.data_ptr(), mass.data_ptr(),
-             lens.data_ptr(), budget.data_ptr(), out.data_ptr(), freed.data_ptr(), n_freed.data_ptr())
+            lens.data_ptr(), budget.data_ptr(), out.data_ptr(), freed.data_ptr(), n_freed.data_ptr())
     return out, freed, n_freed
 
 
@@ -1414,8 +1415,8 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
                              tokens.stride(0) if td == 2 else 0, bias.stride(0) if bias is not None and bias.dim() == 2 else 0,
                              mask.stride(0) if mask is not None and mask.dim() == 2 else 0, *num)
     _launch(dev, "scope_logit_penalties", C.byref(prm), logits.data_ptr(), tokens.data_ptr(), lens.data_ptr(),
-             _ptr(first), _ptr(n_prompt), _ptr(arr[0]), _ptr(arr[1]), _ptr(arr[2]), _ptr(arr[3]), _ptr(bias), _ptr(mask),
-             out.data_ptr())
+            _ptr(first), _ptr(n_prompt), _ptr(arr[0]), _ptr(arr[1]), _ptr(arr[2]), _ptr(arr[3]), _ptr(bias), _ptr(mask),
+            out.data_ptr())
     return out
 
 

@@ -11,9 +11,10 @@ attention layer.
 
 The reference has no decode path and no cache.  Pages are taken from the pool
 when a sequence grows into them, on the host, whose copy of the lengths needs no
-reading back; ``evict`` reads the table back to know what it freed.  ``append``
-and ``attend`` never wait for the GPU, except where ``append`` takes pages: the
-new table entries are copied from pageable host memory.  A cache is used on one
+reading back; ``evict`` reads the table back to know what it freed.  ``attend``
+never waits for the GPU.  ``append`` waits where it takes pages and wherever it is
+given ``rows``: the new table entries and the counts are copied from pageable host
+memory; a step (no ``rows``) within the pages taken does not.  A cache is used on one
 stream at a time: a page goes from one sequence to another in stream order.
 ``attend`` may be captured into a graph; the calls that also change the host's
 copy, which a replay would not, raise there.
