@@ -500,7 +500,8 @@ class ScopeDecoder(nn.Module):
                 if isinstance(penalties.get(name), int):
                     penalties[name] = ops._ints("generate", name, penalties[name], 1, self.device)
             # what it refuses it refuses here, before a step has moved the position
-            ops.logit_penalties(torch.zeros(V, device=self.device), self.tokens, self._t_dev, **penalties)
+            z = torch.zeros(V, device=self.device)
+            ops.logit_penalties(z, self.tokens, self._t_dev, out=z, **penalties)
         for s in range(n_steps):
             logits = self.step(tok)[:V]
             if penalties is not None:

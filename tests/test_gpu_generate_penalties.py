@@ -16,7 +16,8 @@ def test_refused_penalties_leave_the_decoder_where_it_was():
     m = ScopeDecoder(cfg, max_len=512, seed=1)
     first = int(m.prefill(prompt)[:1000].argmax())
     for bad, error in ((dict(repetition=0.0), ValueError), (dict(temperature=1e-50), ValueError), (dict(bias=torch.zeros(999, device=DEV)), RuntimeError),
-                       (dict(mask=torch.zeros(32, dtype=torch.int64, device=DEV)), RuntimeError), (dict(wrong=1), TypeError)):
+                       (dict(mask=torch.zeros(32, dtype=torch.int64, device=DEV)), RuntimeError), (dict(wrong=1), TypeError),
+                       (dict(out=torch.zeros(1000, device=DEV)), TypeError)):
         with pytest.raises(error):
             m.generate(3, first, penalties=bad)
         assert m.t == 256 and int(m._t_dev) == 256
