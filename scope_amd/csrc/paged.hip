@@ -357,28 +357,28 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
 // would count in the sum and not in the output: behind one key that takes nearly all
 // of the weight, 131k others 17.4 nats lower came out as 0).  There the
 // probabilities are taken relative to each tile's own largest, which becomes 2^14 to
-// 2^15, and sums and outputs follow by powers of two: a key is off by no more than 2^-39
-// of its tile's largest (half of fp16's smallest step), all of them by 2^-34 of the
-// sum.  That costs up to 1% (48 windows of 4096 at D = 64 53.8 us either way, 32
+// 2^15, and sums and outputs follow by powers of two: a key is off by no more than
+// 2^-39 of its tile's largest (half of fp16's smallest step), all of them by 2^-34 of
+// the sum.  That costs up to 1% (48 windows of 4096 at D = 64 53.8 us either way, 32
 // sequences to 16k at D = 128 58.8 -> 59.1); a tile's product of its own, joined by an
 // fp32 factor, spills at D = 128 (79.7).
 // Bound by memory: 131k positions of 8 heads of 128 in bf16 (537 MB) in 87 us,
 // 6.2 TB/s, where reading alone takes 80; 24 sequences of 9k to 65k in e4m3 (1.5
 // GB) 5.5 TB/s with the launch behind it.  Groups of more than 16 query heads read K
 // and V once for every 16 (8 sequences of 60k on one key head: 16 heads 59 us, 32 87,
-// 64 145).  V passes the caches (131k
-// positions with the launch behind it 96 us, through them 105); K does not (the same
-// 96 past them, but 1100 positions 10.0 -> 10.7 us).  More in flight (two tiles at
-// once, the next one's loads ahead) changed nothing.
+// 64 145).  V passes the caches (131k positions with the launch behind it 96 us,
+// through them 105); K does not (the same 96 past them, but 1100 positions 10.0 ->
+// 10.7 us).  More in flight (two tiles at once, the next one's loads ahead) changed
+// nothing.
 constexpr int attn_waves(int D, bool fp8) {  // wavefronts a SIMD that the registers are cut to
   // (D = 256 needs 256 registers and a few more in 16 bits: one wavefront 107 us, two
   // that spill 113; in e4m3 two 58, one 75)
   return D == 64 ? 4 : D == 128 ? 3 : fp8 ? 2 : 1;
 }
 
-// fp16: log2 of a tile's largest probability (2^15 at most), and how far below the largest so far
-// a tile is taken as it is (deeper, its keys are off by up to 2^-99 of the sum; the
-// sums stay below 2^(15 + 60 + 31), the outputs 2^16 times that)
+// fp16: log2 of a tile's largest probability (less than 15), and how far below the
+// largest so far a tile is taken as it is (deeper, its keys are off by up to 2^-99 of
+// the sum; the sums stay below 2^(15 + 60 + 31), the outputs 2^16 times that)
 constexpr float kTopBits = 14.f, kMostBelow = 60.f;
 
 // 16-bit values whose sum is a probability in the product with V

@@ -1315,13 +1315,14 @@ def paged_evict(table: torch.Tensor, mass: torch.Tensor, lens: torch.Tensor, bud
 
     Of sequence b's ceil(lens[b] / bs) blocks those with a table entry >= 0
     are held (one past the pool too, which the pool's other users take for no
-    page: the pool is not given here).  Where more than budget[b] (a tensor [B] or one number) are, the
-    surplus goes: the blocks of least Σ_h mass[b, h, i] (mass [B, Hkv, MP]
-    fp32; summed in 64 bits, compared in 32; NaN above everything, the lower
-    index on ties), except the first ``n_global`` blocks and the last
-    ``window`` ones; all the others where they do not suffice.  The returned
-    table has -1 in their place (a new tensor, or ``out``, which may be the
-    table itself); freed holds their pages in the blocks' order, then -1."""
+    page: the pool is not given here).  Where more than budget[b] (a tensor [B]
+    or one number) are, the surplus goes: the blocks of least Σ_h mass[b, h, i]
+    (mass [B, Hkv, MP] fp32; summed in 64 bits, compared in 32; NaN above
+    everything, the lower index on ties), except the first ``n_global`` blocks
+    and the last ``window`` ones; all the others where they do not suffice.
+    The returned table has -1 in their place (a new tensor, or ``out``, which
+    may be the table itself); freed holds their pages in the blocks' order,
+    then -1."""
     who = "paged_evict"
     dev = _device(who, table, mass, lens, budget if isinstance(budget, torch.Tensor) else None, out)
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.numel() > _INT_MAX:
