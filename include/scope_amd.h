@@ -708,6 +708,47 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
                             const int32_t* kv_num, const int32_t* kv_idx, float* mass, void* work, uint16_t* out,
                             float* lse, void* stream);
 
+/* The same cache in 4 bits: a row's features in groups of 32 as e2m1 codes (0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte, the even feature in the low
+ * nibble, and one e8m0 byte a group that stands for 2^(byte - 127), 255 for NaN
+ * (the MXFP4 format).  The pages are [P][Hkv][bs][D/2] bytes: the strides of
+ * scope_paged_cache count bytes then, its fp8 is not read, and `type` is that of q,
+ * k, v and out.
+ *   k_scale, v_scale  [P][Hkv][bs][D/32] bytes, page and head strides below, a
+ *                     page's head contiguous and 16-byte aligned */
+typedef struct {
+  int64_t k_sp, k_sh, v_sp, v_sh;
+} scope_paged_scales;
+
+/* scope_paged_append into such pages; both the codes and the scales are written.
+ * With 2^x the power of two at or below a group's largest |value| a, its scale is
+ * 2^(x - 2), or 2^(x - 1) where a >= 1.75 · 2^x, kept to 2^-125 .. 2^125 (bf16 rows)
+ * or 2^-125 .. 2^13 (fp16: six times it is finite); the codes are the nearest ones
+ * of value / scale, the even one of two, at most 6.  A group that holds an infinity
+ * or a NaN gets the scale 255 and codes 0. */
+int scope_paged_append_fp4(const scope_paged_cache* c, const scope_paged_scales* s, int64_t N, const uint16_t* k, int64_t k_sn,
+                           int64_t k_sh, const uint16_t* v, int64_t v_sn, int64_t v_sh, const int32_t* cu, const int32_t* table,
+                           const int32_t* lens, void* k_scale, void* v_scale, void* k_pages, void* v_pages, void* stream);
+
+/* scope_paged_decode_attn over such pages (its workspace alike).  A NaN scale of a
+ * seen row of K makes its queries' outputs NaN, one of V the features of its group. */
+int scope_paged_decode_attn_fp4(const scope_paged_cache* c, const scope_paged_scales* s, int Hq, int maxkv, float scale,
+                                const uint16_t* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
+                                const void* k_scale, const void* v_scale, const int32_t* table, const int32_t* lens,
+                                const int32_t* first, const int32_t* kv_num, const int32_t* kv_idx, float* mass, void* work,
+                                uint16_t* out, float* lse, void* stream);
+
+/* N rows out of the pages into k, v [N][Hkv][D] of `type`, contiguous: row i is that
+ * of the sequence b with cu[b] <= i < cu[b + 1] (cu [B + 1], not decreasing; NULL:
+ * sequence i) at position first[b] + i - cu[b] (first NULL: 0; NULL cu: first[b]).
+ * Rows of no sequence, outside [0, lens[b]) or of a block without a page are zeros.
+ * s NULL: pages of `type`, moved as they are, or e4m3 (c->fp8; byte · scale[h] in
+ * fp32, rounded to `type`; k_scale, v_scale [Hkv] fp32 or NULL); else 4-bit pages
+ * (exact in bf16; rounded to fp16, infinite where that does not hold the value). */
+int scope_paged_read(const scope_paged_cache* c, const scope_paged_scales* s, int64_t N, const int32_t* cu, const int32_t* table,
+                     const int32_t* lens, const int32_t* first, const void* k_scale, const void* v_scale, const void* k_pages,
+                     const void* v_pages, uint16_t* k, uint16_t* v, void* stream);
+
 /* Takes the pages of least accumulated weight out of the table.  Of sequence
  * b's n = ceil(lens[b] / bs) blocks those with a table entry >= 0 are held (one
  * past the pool too, which is no page to the others: the pool is not given here);

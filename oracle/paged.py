@@ -12,8 +12,82 @@ E4M3_MAX = 448.0
 
 def values(pages: torch.Tensor, scale: torch.Tensor | None) -> torch.Tensor:
     """The numbers that pages [P, Hkv, bs, D] stand for, fp64."""
-    x = pages.float().double()
+    x = pages if pages.dtype == torch.float64 else pages.float().double()
     return x if scale is None else x * scale.double()[:, None, None]
+
+
+# ---- 4 bits: groups of 32 features as e2m1 codes with one e8m0 scale ----------------
+E2M1 = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+GROUP = 32
+SCALE_MIN, SCALE_MAX = -125, {torch.bfloat16: 125, torch.float16: 13}  # powers of two that are written
+
+
+def quantise_group(x) -> tuple[list[int], int]:
+    """(codes, scale byte) of one group's 16-bit values, by the definition: Python's
+    exact floats, each code the nearest grid value, the even code of two."""
+    top = SCALE_MAX[x.dtype]
+    v = [float(f) for f in x.double()]
+    if not all(math.isfinite(f) for f in v):
+        return [0] * len(v), 255
+    a = max(abs(f) for f in v)
+    e = SCALE_MIN
+    if a > 0:
+        low = math.frexp(a)[1] - 1
+        e = low - 1 if a >= 1.75 * 2.0 ** low else low - 2
+    e = min(max(e, SCALE_MIN), top)
+    codes = []
+    for f in v:
+        y = abs(f) / 2.0 ** e
+        best = min(range(8), key=lambda c: (abs(E2M1[c] - y), c % 2))
+        codes.append(best + (8 if math.copysign(1.0, f) < 0 else 0))
+    return codes, e + 127
+
+
+def quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(bytes [..., D / 2], scale bytes [..., D / 32]) of 16-bit rows [..., D]: the even
+    feature in the low nibble.  The definition of quantise_group, over tensors in fp64."""
+    y = x.double().reshape(*x.shape[:-1], -1, GROUP)
+    bad = ~torch.isfinite(y).all(-1)
+    y = torch.where(bad[..., None], 0.0, y)
+    a = y.abs().amax(-1)
+    m, e = torch.frexp(a)
+    e = torch.where(a > 0, e - 3 + (m >= 0.875).int(), SCALE_MIN).clamp(SCALE_MIN, SCALE_MAX[x.dtype])
+    z = torch.ldexp(y, -e[..., None])
+    grid = torch.tensor(E2M1, dtype=torch.float64)
+    edges = (grid[1:] + grid[:-1]) / 2
+    code = torch.bucketize(z.abs().contiguous(), edges)  # (on an edge the lower code)
+    on = (code < 7) & (z.abs() == edges[code.clamp(max=6)])
+    code = code + (on & (code % 2 == 1)).long() + 8 * torch.signbit(z).long()
+    code = torch.where(bad[..., None], 0, code).reshape(*x.shape[:-1], -1, 2)
+    return (code[..., 0] + 16 * code[..., 1]).to(torch.uint8), torch.where(bad, 255, e + 127).to(torch.uint8)
+
+
+def e2m1_values(pages: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The numbers that 4-bit pages [..., D / 2] with scales [..., D / 32] stand for, fp64."""
+    b, s = pages.view(torch.uint8).long(), scale.view(torch.uint8).double()
+    code = torch.stack((b % 16, b // 16), -1).flatten(-2)
+    x = torch.tensor(E2M1 + [-f for f in E2M1], dtype=torch.float64)[code]
+    return x * torch.where(s == 255, math.nan, 2.0 ** (s - 127)).repeat_interleave(GROUP, -1)
+
+
+def append_e2m1(x, pages, scale, table, lens, cu=None):
+    """(pages, scales) after the rows x were quantised into them."""
+    q, s = quantise(x)
+    return tuple(append(r, t.view(torch.uint8), table, lens, cu).view(t.dtype) for r, t in ((q, pages), (s, scale)))
+
+
+def read(vals: torch.Tensor, table, lens, rows, cu=None, first=None) -> torch.Tensor:
+    """Rows [rows, Hkv, D] out of pages of values [P, Hkv, bs, D], one at a time."""
+    P, Hkv, bs, D = vals.shape
+    B, MP = table.shape
+    out = torch.zeros((rows, Hkv, D), dtype=vals.dtype)
+    for b in range(B):
+        r0, r1 = (b, b + 1) if cu is None else (int(cu[b]), int(cu[b + 1]))
+        for i in range(max(r0, 0), min(r1, rows)):
+            pos = (0 if first is None else int(first[b])) + i - r0
+            if 0 <= pos < min(int(lens[b]), MP * bs) and 0 <= int(table[b, pos // bs]) < P:
+                out[i] = vals[int(table[b, pos // bs]), :, pos % bs]
+    return out
 
 
 def append(x, pages, table, lens, cu=None, scale=None) -> torch.Tensor:

@@ -99,6 +99,10 @@ class PagedCache(C.Structure):
                 ("v_sp", c_int64), ("v_sh", c_int64), ("v_sr", c_int64)]
 
 
+class PagedScales(C.Structure):
+    _fields_ = [("k_sp", c_int64), ("k_sh", c_int64), ("v_sp", c_int64), ("v_sh", c_int64)]
+
+
 class PenaltyParams(C.Structure):
     _fields_ = [("B", c_int), ("type", c_int), ("tokens64", c_int), ("lens64", c_int), ("V", c_int64), ("T", c_int64),
                 ("z_sb", c_int64), ("o_sb", c_int64), ("tok_sb", c_int64), ("bias_sb", c_int64), ("mask_sb", c_int64),
@@ -165,6 +169,11 @@ _PROTOS = {
     "scope_paged_append": (c_int, [C.POINTER(PagedCache), c_int64, P, c_int64, c_int64, P, c_int64, c_int64] + [P] * 8),
     "scope_paged_attn_workspace_bytes": (c_int64, [C.POINTER(PagedCache), c_int, c_int, c_int]),
     "scope_paged_decode_attn": (c_int, [C.POINTER(PagedCache), c_int, c_int, c_float, P, c_int64, c_int64] + [P] * 14),
+    "scope_paged_append_fp4": (c_int, [C.POINTER(PagedCache), C.POINTER(PagedScales), c_int64, P, c_int64, c_int64, P, c_int64,
+                                       c_int64] + [P] * 8),
+    "scope_paged_decode_attn_fp4": (c_int, [C.POINTER(PagedCache), C.POINTER(PagedScales), c_int, c_int, c_float, P, c_int64,
+                                            c_int64] + [P] * 14),
+    "scope_paged_read": (c_int, [C.POINTER(PagedCache), C.POINTER(PagedScales), c_int64] + [P] * 11),
     "scope_paged_evict": (c_int, [c_int] * 6 + [P] * 8),
     "scope_logit_penalties": (c_int, [C.POINTER(PenaltyParams)] + [P] * 13),
     "scope_attn_bwd": (c_int, [C.POINTER(AttnParams)] + [P] * 30),

@@ -9,65 +9,10 @@
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
 
-#include "attn_common.h"
-#include "paged_plan.h"
+#include "paged_attn.h"
 
 namespace scope {
-
-namespace {
-__device__ __forceinline__ float half_to_f32(uint16_t h) { return static_cast<float>(__builtin_bit_cast(_Float16, h)); }
-__device__ __forceinline__ uint16_t f32_to_half(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
-
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-
-// op over a wavefront in six steps on neighbouring lanes' registers (row shifts by
-// 1, 2, 4, 8, then the rows' last lanes to the rows behind them): lane l gets the
-// result over lanes 0 .. l.  A step costs a few cycles, one through LDS some sixty.
-template <int CTRL, int ROWS, class Op>
-__device__ __forceinline__ uint32_t lane_step(uint32_t v, uint32_t none, Op op) {
-  return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(v), CTRL, ROWS, 0xf, false)));
-}
-template <class Op>
-__device__ __forceinline__ uint32_t lane_prefix(uint32_t v, uint32_t none, Op op) {
-  v = lane_step<0x111, 0xf>(v, none, op);
-  v = lane_step<0x112, 0xf>(v, none, op);
-  v = lane_step<0x114, 0xf>(v, none, op);
-  v = lane_step<0x118, 0xf>(v, none, op);
-  v = lane_step<0x142, 0xa>(v, none, op);
-  return lane_step<0x143, 0xc>(v, none, op);
-}
-__device__ __forceinline__ uint32_t add_u32(uint32_t a, uint32_t b) { return a + b; }
-__device__ __forceinline__ uint32_t add_f32(uint32_t a, uint32_t b) {
-  return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-}
-__device__ __forceinline__ uint32_t max_f32(uint32_t a, uint32_t b) {
-  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-}
-// op over the four lanes l % 16 + 16 k, or over two of them (k = 0, 1 and 2, 3): rows
-// of 16 lanes and halves of 32 exchanged between two copies
-template <class Op>
-__device__ __forceinline__ float over_rows2(float v, Op op) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(op(r[0], r[1]));
-}
-template <class Op>
-__device__ __forceinline__ float over_rows(float v, Op op) {
-  const uint32_t x = __float_as_uint(over_rows2(v, op));
-  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return __uint_as_float(op(r[0], r[1]));
-}
-// the sums over lanes 0 .. l of a count, and over all lanes
-__device__ __forceinline__ int prefix_of(int v) { return static_cast<int>(lane_prefix(static_cast<uint32_t>(v), 0u, add_u32)); }
-__device__ __forceinline__ float sum_of(float v) {
-  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0u, add_f32), 63));
-}
-__device__ __forceinline__ float max_of(float v) {
-  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0xff800000u, max_f32), 63));
-}
-}  // namespace
 
 // ---- append ------------------------------------------------------------------
 // Row i of the N new ones belongs to the sequence b with cu[b] <= i < cu[b + 1]
@@ -133,15 +78,6 @@ __device__ __forceinline__ uint2 e4m3x8(const uint4& u, float s, float r) {
   return make_uint2(o[0], o[1]);
 }
 
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint4 load_past(const uint4* p) {
-  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p)));
-}
-__device__ __forceinline__ void store_past(uint8_t* p, uint2 x) {
-  __builtin_nontemporal_store(__builtin_bit_cast(u32x2_t, x), reinterpret_cast<u32x2_t*>(p));
-}
-
 template <int TYPE, bool FP8>
 __global__ __launch_bounds__(256) void paged_append_kernel(scope_paged_cache c, AppendArgs a) {
   const int lane = threadIdx.x & 63;
@@ -183,84 +119,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(scope_paged_cache c, 
 }
 
 // ---- attention of one new token -------------------------------------------------
-struct PagedAttnArgs {
-  int Hq, maxkv;
-  float scale;
-  int64_t q_sb, q_sh;
-  const uint16_t* q;
-  const void* k_pages;
-  const void* v_pages;
-  const float* k_scale;
-  const float* v_scale;
-  const int32_t* table;
-  const int32_t* lens;
-  const int32_t* first;
-  const int32_t* kv_num;
-  const int32_t* kv_idx;
-  float* mass;
-  uint16_t* out;
-  float* lse;
-};
-
-// Workgroups of kAttnWaves wavefronts; piece i of the batch (paged_plan.h) is
-// blockIdx.x, (key head, group of 16 query heads) blockIdx.y.
-constexpr int kAttnThreads = 64 * kAttnWaves;
-
-struct AttnSplit {
-  int pieces, slots;   // pieces aimed at and slots of a (key head, group); with lists: pieces of every list
-  int64_t tiles_cap;   // tiles of a full table row (list)
-  float* po;           // [slots][Hq][D] partial P·V, unnormalised
-  float* pml;          // [slots][Hq][2] their maxima (log2 units) and sums
-  int2* plan;          // [B] (pieces, first slot) of each sequence
-  float* lse2;         // [B][Hq] log2 of the whole sums of rows in one piece, for the mass
-  float* tile_lse;     // [B][Hq][tiles_cap][halves] log2 of each tile's (half tile's) sum, for the mass
-};
-
-// piece i of n of sequence b: its tiles, and the sequence's first slot
-struct Piece {
-  int b, t0, t1, i, n, slot;
-};
-
-// The piece of this workgroup, found by every wavefront for itself: the batch's
-// tiles are summed, then the sequences' numbers of pieces.  false: there is none.
-__device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const PagedAttnArgs& a, const AttnSplit& s, int x,
-                                           int turn, Piece& p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
-  const auto tiles_of = [&](int b, int* lo) {
-    *lo = 0;
-    return b < c.B ? seq_tiles(a.lens[b], a.first ? a.first[b] : 0, cap, lo) : 0;
-  };
-  int lo0;
-  const int tiles0 = tiles_of(lane, &lo0);
-  // (64 sequences of less than 2^26 tiles: their sum fits 32 bits)
-  int64_t total = static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles0), 63));
-  for (int b0 = 64; b0 < c.B; b0 += 64) {
-    int lo;
-    total += static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles_of(b0 + lane, &lo)), 63));
-  }
-  const int64_t piece = piece_tiles(total, s.pieces, kPieceTiles, turn);
-  int before = 0;
-  for (int b0 = 0; b0 < c.B; b0 += 64) {
-    int lo = lo0;
-    const int tiles = b0 ? tiles_of(b0 + lane, &lo) : tiles0;
-    const int n = b0 + lane < c.B ? seq_pieces(tiles, piece) : 0;
-    const int upto = prefix_of(n);
-    const uint64_t hit = __ballot(x < before + upto);
-    if (hit) {
-      const int at = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-      p.b = b0 + at;
-      p.n = __builtin_amdgcn_readlane(n, at);
-      p.slot = before + __builtin_amdgcn_readlane(upto, at) - p.n;
-      p.i = x - p.slot;
-      piece_range(__builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(tiles, at), p.n, p.i, &p.t0, &p.t1);
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
-  }
-  return false;
-}
-
 template <int TYPE>
 __device__ __forceinline__ f32x4_t mfma_16(const uint4& a, const uint4& b, const f32x4_t& acc) {
   if constexpr (TYPE == SCOPE_BF16) {
@@ -270,39 +128,6 @@ __device__ __forceinline__ f32x4_t mfma_16(const uint4& a, const uint4& b, const
   }
 }
 
-// two 16-bit values, rounded to nearest even
-template <int TYPE>
-__device__ __forceinline__ uint32_t round2(float lo, float hi) {
-  if constexpr (TYPE == SCOPE_BF16) {
-    return cvt_pk_bf16(lo, hi);
-  } else {
-    f16x2_t v;
-    v[0] = static_cast<_Float16>(lo);
-    v[1] = static_cast<_Float16>(hi);
-    return __builtin_bit_cast(uint32_t, v);
-  }
-}
-
-// the largest 16-bit values below two positive numbers (0 below 0)
-template <int TYPE>
-__device__ __forceinline__ uint32_t below2(float lo, float hi) {
-  const uint32_t a = __builtin_elementwise_sub_sat(__float_as_uint(lo), 1u), b = __builtin_elementwise_sub_sat(__float_as_uint(hi), 1u);
-  if constexpr (TYPE == SCOPE_BF16)
-    return pack_hi16(a, b);
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(a), __uint_as_float(b)));
-}
-
-// the halves of a word of two 16-bit values
-template <int TYPE>
-__device__ __forceinline__ float low_half(uint32_t w) {
-  return TYPE == SCOPE_BF16 ? __uint_as_float(w << 16) : half_to_f32(static_cast<uint16_t>(w));
-}
-template <int TYPE>
-__device__ __forceinline__ float high_half(uint32_t w) {
-  return TYPE == SCOPE_BF16 ? __uint_as_float(w & 0xffff0000u) : half_to_f32(static_cast<uint16_t>(w >> 16));
-}
-
 // two e4m3 bytes as 16-bit values (exact)
 template <int TYPE, bool HI>
 __device__ __forceinline__ uint32_t widen2(uint32_t w) {
@@ -310,26 +135,6 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
   else
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
-}
-
-template <int N>
-struct Words {
-  uint32_t w[N];
-};
-
-// N words that are read once: they are not kept in the caches in front of others
-template <int N>
-__device__ __forceinline__ Words<N> load_once(const char* p) {
-  Words<N> x;
-  if constexpr (N == 1) {
-    x.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
-  } else {
-    typedef uint32_t words_t __attribute__((ext_vector_type(N), aligned(4)));
-    const words_t v = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(p));
-#pragma unroll
-    for (int i = 0; i < N; ++i) x.w[i] = v[i];
-  }
-  return x;
 }
 
 // The attention of one new token.  For a tile of 32 keys and 16 query heads of
@@ -610,58 +415,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     }
   }
 
-  // the wavefronts' shares: maxima and sums, then the outputs of the group's queries
-  l = over_rows(l, add_f32);
-  float* sm = lds;                       // [waves][16]
-  float* sl = lds + kAttnWaves * 16;     // [waves][16]
-  float* so = lds + kAttnWaves * 32;     // [waves][nq][D]
-  if (g4 == 0) {
-    sm[wave * 16 + c16] = m == -INFINITY ? m : ref;
-    sl[wave * 16 + c16] = l;
-  }
-  if (c16 < nq) {
-    float* o = so + (wave * nq + c16) * D + g4 * 4 * VE;
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < VE; j += 4)
-          *reinterpret_cast<float4*>(o + h * 128 + r * VE + j) = make_float4(
-              acc[h * VE + j][r], acc[h * VE + j + 1][r], acc[h * VE + j + 2][r], acc[h * VE + j + 3][r]);
-  }
-  __syncthreads();
-  const float vs = a.v_scale ? a.v_scale[hk] : 1.f;
-  for (int i = threadIdx.x; i < nq * D; i += kAttnThreads) {
-    const int q = i / D, d = i % D, h = h0 + q;
-    float M = sm[q];
-#pragma unroll
-    for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, sm[w * 16 + q]);
-    float L = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w) {
-      // (a sum of 0 is a share without keys; a NaN stays one, whatever its maximum)
-      const float f = sl[w * 16 + q] == 0.f ? 0.f : __builtin_amdgcn_exp2f(sm[w * 16 + q] - M);
-      L += f * sl[w * 16 + q];
-      o += f * so[(w * nq + q) * D + d];
-    }
-    if (p.n == 1) {
-      const float y = L == 0.f ? 0.f : o / L * vs;
-      a.out[(static_cast<int64_t>(b) * a.Hq + h) * D + d] = TYPE == SCOPE_FP16 ? f32_to_half(y) : f32_to_bf16(y);
-      if (d == 0) {
-        const float e = L == 0.f ? -INFINITY : M + __builtin_amdgcn_logf(L);
-        a.lse[static_cast<int64_t>(b) * a.Hq + h] = e * kLn2;
-        if (s.lse2) s.lse2[static_cast<int64_t>(b) * a.Hq + h] = e;
-      }
-    } else {
-      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.Hq + h;
-      s.po[at * D + d] = o;
-      if (d == 0) {
-        s.pml[2 * at] = M;
-        s.pml[2 * at + 1] = L;
-      }
-    }
-  }
+  end_piece<TYPE, D, VE, NH>(a, s, p, hk, h0, nq, m, ref, l, acc, lds);
 }
 
 // (maximum, sum relative to it) of a row from its n pieces' (maximum, sum) pairs,
@@ -980,9 +734,6 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(EvictArgs a)
   if (tid == 0) a.n_freed[b] = all;
 }
 
-namespace {
-bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
-
 int check_cache(const scope_paged_cache* c, const void* k_pages, const void* v_pages, const char* fn) {
   SCOPE_REQUIRE(c, "%s: null cache", fn);
   SCOPE_REQUIRE(c->D == 64 || c->D == 128 || c->D == 256, "%s: head dim must be 64, 128 or 256, got %d", fn, c->D);
@@ -1002,6 +753,7 @@ int check_cache(const scope_paged_cache* c, const void* k_pages, const void* v_p
   return SCOPE_OK;
 }
 
+namespace {
 // The pieces of a call and its workspace (laid out in `work` where s is given);
 // returns its bytes.
 int64_t plan_split(const scope_paged_cache& c, int Hq, int maxkv, bool with_mass, AttnSplit* out, void* work) {
@@ -1029,6 +781,32 @@ int64_t plan_split(const scope_paged_cache& c, int Hq, int maxkv, bool with_mass
   return at;
 }
 }  // namespace
+
+int check_attn(const scope_paged_cache& c, const PagedAttnArgs& a, void* work, AttnSplit* s, const char* fn) {
+  SCOPE_REQUIRE(a.Hq >= 1 && a.Hq <= 65535 && a.Hq % c.Hkv == 0, "%s: Hq=%d must be a multiple of Hkv=%d, at most 65535", fn,
+                a.Hq, c.Hkv);
+  SCOPE_REQUIRE((a.kv_num != nullptr) == (a.kv_idx != nullptr) &&
+                    (a.kv_idx ? a.maxkv >= 1 && static_cast<int64_t>(a.maxkv) * c.bs <= INT32_MAX : a.maxkv == 0),
+                "%s: kv_num and kv_idx come together, with 1 .. 2^31 / bs entries (maxkv=%d; 0 without lists)", fn, a.maxkv);
+  SCOPE_REQUIRE(a.q && a.table && a.lens && a.out && a.lse, "%s: null pointer", fn);
+  SCOPE_REQUIRE(plan_split(c, a.Hq, a.maxkv, a.mass != nullptr, s, work) == 0 || work, "%s: null pointer (the workspace)", fn);
+  SCOPE_REQUIRE(aligned16(a.q) && aligned16(work) && a.q_sb % 8 == 0 && a.q_sh % 8 == 0,
+                "%s: the rows of q and the workspace must be 16-byte aligned", fn);
+  return SCOPE_OK;
+}
+
+int launch_paged_finish(const scope_paged_cache& c, const PagedAttnArgs& a, const AttnSplit& s, hipStream_t st) {
+  if (!s.po && !a.mass) return SCOPE_OK;  // every sequence is one piece
+  const int G = a.Hq / c.Hkv, blocks = a.kv_idx ? a.maxkv : c.MP;
+  const dim3 fg((s.po ? G : 0) + (a.mass ? ceil_div(blocks, 256) : 0), c.Hkv, c.B);
+  if (c.D == 64)
+    hipLaunchKernelGGL(paged_finish_kernel<64>, fg, dim3(256), 0, st, c, a, s);
+  else if (c.D == 128)
+    hipLaunchKernelGGL(paged_finish_kernel<128>, fg, dim3(256), 0, st, c, a, s);
+  else
+    hipLaunchKernelGGL(paged_finish_kernel<256>, fg, dim3(256), 0, st, c, a, s);
+  return check_launch("paged_finish_kernel");
+}
 
 }  // namespace scope
 
@@ -1073,18 +851,10 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
                             float* lse, void* stream) {
   const char* fn = "scope_paged_decode_attn";
   if (int rc = check_cache(c, k_pages, v_pages, fn)) return rc;
-  SCOPE_REQUIRE(Hq >= 1 && Hq <= 65535 && Hq % c->Hkv == 0, "%s: Hq=%d must be a multiple of Hkv=%d, at most 65535", fn, Hq,
-                c->Hkv);
-  SCOPE_REQUIRE((kv_num != nullptr) == (kv_idx != nullptr) &&
-                    (kv_idx ? maxkv >= 1 && static_cast<int64_t>(maxkv) * c->bs <= INT32_MAX : maxkv == 0),
-                "%s: kv_num and kv_idx come together, with 1 .. 2^31 / bs entries (maxkv=%d; 0 without lists)", fn, maxkv);
-  SCOPE_REQUIRE(q && table && lens && out && lse, "%s: null pointer", fn);
-  AttnSplit s;
-  SCOPE_REQUIRE(plan_split(*c, Hq, maxkv, mass != nullptr, &s, work) == 0 || work, "%s: null pointer (the workspace)", fn);
-  SCOPE_REQUIRE(aligned16(q) && aligned16(work) && q_sb % 8 == 0 && q_sh % 8 == 0,
-                "%s: the rows of q and the workspace must be 16-byte aligned", fn);
   const PagedAttnArgs a{Hq,    maxkv, scale, q_sb,   q_sh,   q,    k_pages, v_pages, k_scale,
                         v_scale, table, lens,  first, kv_num, kv_idx, mass, out,     lse};
+  AttnSplit s;
+  if (int rc = check_attn(*c, a, work, &s, fn)) return rc;
   const int G = Hq / c->Hkv, ng = (G + 15) / 16;
   const dim3 grid(s.slots, c->Hkv * ng);
   const size_t lds = sizeof(float) * kAttnWaves * (32 + static_cast<size_t>(std::min(G, 16)) * c->D);
@@ -1107,16 +877,7 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
     c->fp8 ? launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, true>{})
            : launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, false>{});
   if (int rc = check_launch("paged_attn_kernel")) return rc;
-  if (!s.po && !mass) return SCOPE_OK;  // every sequence is one piece
-  const int blocks = kv_idx ? maxkv : c->MP;
-  const dim3 fg((s.po ? G : 0) + (mass ? ceil_div(blocks, 256) : 0), c->Hkv, c->B);
-  if (c->D == 64)
-    hipLaunchKernelGGL(paged_finish_kernel<64>, fg, dim3(256), 0, st, *c, a, s);
-  else if (c->D == 128)
-    hipLaunchKernelGGL(paged_finish_kernel<128>, fg, dim3(256), 0, st, *c, a, s);
-  else
-    hipLaunchKernelGGL(paged_finish_kernel<256>, fg, dim3(256), 0, st, *c, a, s);
-  return check_launch("paged_finish_kernel");
+  return launch_paged_finish(*c, a, s, st);
 }
 
 int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, const int32_t* table, const float* mass,

@@ -1,0 +1,614 @@
+// The paged cache in 4 bits: rows quantised as they are written, the attention of
+// one new token over such pages, and rows read back out of pages of any type.
+//
+// A row's D features go in groups of 32 to e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+// their negatives), two a byte with the even feature in the low nibble, and one e8m0
+// byte a group that stands for 2^(byte - 127), 255 for NaN: the MXFP4 format of the
+// Open Compute Project, which gfx950 converts in one instruction for two values.
+// Pages are [P][Hkv][bs][D/2] bytes (any page, head and row strides), scales
+// [P][Hkv][bs][D/32] (any page and head strides).
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged_attn.h"
+
+namespace scope {
+
+namespace {
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
+// the lane's value and those of the other lanes of its quad, op over all four
+template <class Op>
+__device__ __forceinline__ uint32_t over_quad(uint32_t v, Op op) {
+  v = op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xb1, 0xf, 0xf, true)));
+  return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4e, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+
+// the scale of an e8m0 byte, as the conversions take it: they read bits 23 .. 30 alone
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+}  // namespace
+
+// ---- rows in and out -----------------------------------------------------------
+// N rows of Hkv·D / 8 chunks of eight features, `rows` of them to a wavefront, chunks
+// dealt to its lanes in turn: lane r < rows finds the place of row i0 + r.
+struct MoveArgs {
+  int64_t N;
+  int rows, chunks, skip_rows, skip_chunks;  // 64 = skip_rows · chunks + skip_chunks
+  const int32_t* cu;
+  const int32_t* table;
+};
+
+// page (-1: none) and slot of row i, `from` [B] (NULL: 0) the position of a sequence's
+// first one, `to` [B] (NULL: the table's end) the end of its positions
+__device__ __forceinline__ int2 row_place(const scope_paged_cache& c, const MoveArgs& m, const int32_t* from, const int32_t* to,
+                                          int64_t i) {
+  int b;
+  const int64_t pos = row_position(m.cu, from, c.B, i, &b), cap = static_cast<int64_t>(c.MP) * c.bs;
+  if (pos < 0 || pos >= (to ? seq_end(to[b], cap) : cap)) return make_int2(-1, 0);
+  const int64_t page = block_page(m.table + static_cast<int64_t>(b) * c.MP, c.MP, pos / c.bs, c.P);
+  return make_int2(static_cast<int>(page), static_cast<int>(pos % c.bs));
+}
+
+// f(row of the wavefront, chunk, page, slot) for every chunk of this wavefront's n rows
+// that has a lane; places: those that row_place gave the first n lanes.
+template <class F>
+__device__ __forceinline__ void each_chunk(const MoveArgs& m, int n, int2 places, F f) {
+  const int lane = threadIdx.x & 63;
+  int r = lane / m.chunks, e = lane % m.chunks;
+  for (int at = 0; at < n * m.chunks; at += 64) {  // (all lanes go on to the end: others take their places from them)
+    const int page = __shfl(places.x, min(r, 63)), slot = __shfl(places.y, min(r, 63));
+    if (r < n) f(r, e, page, slot);
+    r += m.skip_rows;
+    e += m.skip_chunks;
+    if (e >= m.chunks) {
+      e -= m.chunks;
+      ++r;
+    }
+  }
+}
+
+struct Append4Args {
+  int64_t k_sn, k_sh, v_sn, v_sh;
+  const uint16_t* k;
+  const uint16_t* v;
+  const int32_t* lens;
+  uint8_t* k_pages;
+  uint8_t* v_pages;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+};
+
+// Eight values of a group of 32 that a quad of lanes holds as e2m1 codes; *byte: its
+// scale.  With 2^x the power of two below the largest |value| a the scale is 2^(x - 2),
+// or 2^(x - 1) where a >= 1.75 · 2^x: a is at most 7 of it, which becomes 6, so that no
+// value is off by more than half a step of the grid (codes are rounded to nearest
+// even).  Adding a quarter to a's significand carries into its exponent just there.
+// The scale stays where all codes of it are finite in the rows' type and no code is
+// subnormal in fp32; larger values become 6 of it, smaller ones 0.  A group with an
+// infinity or a NaN gets the scale NaN and codes 0.
+template <int TYPE>
+__device__ __forceinline__ uint32_t e2m1x8(const uint4& u, uint32_t* byte) {
+  constexpr uint32_t kAbs = 0x7fff7fffu, kInf = TYPE == SCOPE_FP16 ? 0x7c00u : 0x7f80u, kTop = TYPE == SCOPE_FP16 ? 140 : 252;
+  uint32_t m = max_u16x2(max_u16x2(u.x & kAbs, u.y & kAbs), max_u16x2(u.z & kAbs, u.w & kAbs));
+  m = over_quad(m, max_u16x2);
+  m = max(m & 0xffffu, m >> 16);
+  if (m >= kInf) {
+    *byte = 255;
+    return 0;
+  }
+  const float a = TYPE == SCOPE_FP16 ? half_to_f32(static_cast<uint16_t>(m)) : bf16_to_f32(static_cast<uint16_t>(m));
+  const uint32_t e = (__float_as_uint(a) + 0x200000u) >> 23;
+  *byte = min(max(e, 4u) - 2u, kTop);
+  const float s = scale_of(*byte);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t o = 0;
+  if constexpr (TYPE == SCOPE_FP16) {
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2_t, w[0]), s, 0);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2_t, w[1]), s, 1);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2_t, w[2]), s, 2);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, __builtin_bit_cast(f16x2_t, w[3]), s, 3);
+  } else {
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2_t, w[0]), s, 0);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2_t, w[1]), s, 1);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2_t, w[2]), s, 2);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o, __builtin_bit_cast(bf16x2_t, w[3]), s, 3);
+  }
+  return o;
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void paged_append4_kernel(scope_paged_cache c, scope_paged_scales z, MoveArgs m, Append4Args a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * m.rows;
+  int2 place = make_int2(-1, 0);
+  if (lane < m.rows && i0 + lane < m.N) place = row_place(c, m, a.lens, nullptr, i0 + lane);
+  const int dshift = __builtin_ctz(c.D) - 3;
+  const int n = static_cast<int>(min(static_cast<int64_t>(m.rows), m.N - i0));
+  each_chunk(m, n, place, [&](int r, int e, int page, int slot) {
+    if (page < 0) return;  // (a quad of lanes has one row: its chunks are a multiple of eight)
+    const int h = e >> dshift, d = (e & ((1 << dshift) - 1)) * 8;
+    const uint4 xk = load_past(reinterpret_cast<const uint4*>(a.k + (i0 + r) * a.k_sn + h * a.k_sh + d));
+    const uint4 xv = load_past(reinterpret_cast<const uint4*>(a.v + (i0 + r) * a.v_sn + h * a.v_sh + d));
+    uint32_t bk, bv;
+    const uint32_t ck = e2m1x8<TYPE>(xk, &bk), cv = e2m1x8<TYPE>(xv, &bv);
+    *reinterpret_cast<uint32_t*>(a.k_pages + page * c.k_sp + h * c.k_sh + slot * c.k_sr + d / 2) = ck;
+    *reinterpret_cast<uint32_t*>(a.v_pages + page * c.v_sp + h * c.v_sh + slot * c.v_sr + d / 2) = cv;
+    if ((lane & 3) == 0) {
+      const int at = slot * (c.D / 32) + d / 32;
+      a.k_scale[page * z.k_sp + h * z.k_sh + at] = static_cast<uint8_t>(bk);
+      a.v_scale[page * z.v_sp + h * z.v_sh + at] = static_cast<uint8_t>(bv);
+    }
+  });
+}
+
+struct ReadArgs {
+  const int32_t* lens;
+  const int32_t* first;
+  const void* k_pages;
+  const void* v_pages;
+  const void* k_scale;
+  const void* v_scale;
+  uint16_t* k;
+  uint16_t* v;
+};
+
+enum { kPages16 = 0, kPages8 = 1, kPages4 = 2 };
+
+// eight features of a row of pages, from `at` elements (bytes of 4-bit pages) on
+template <int KIND, int TYPE>
+__device__ __forceinline__ uint4 read8(const void* pages, int64_t at, float scale) {
+  if constexpr (KIND == kPages16) {
+    return *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pages) + at);
+  } else {
+    uint32_t o[4];
+    if constexpr (KIND == kPages8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pages) + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const auto x = i % 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(i / 2 ? w.y : w.x, true) : __builtin_amdgcn_cvt_pk_f32_fp8(i / 2 ? w.y : w.x, false);
+        o[i] = round2<TYPE>(x[0] * scale, x[1] * scale);
+      }
+    } else {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(pages) + at);
+      const auto put = [&](int i, auto x) { o[i] = round2<TYPE>(x[0], x[1]); };
+      if constexpr (TYPE == SCOPE_BF16) {  // (exact)
+        o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+        o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+        o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+        o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+      } else {
+        put(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0));
+        put(1, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1));
+        put(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2));
+        put(3, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3));
+      }
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+template <int KIND, int TYPE>
+__global__ __launch_bounds__(256) void paged_read_kernel(scope_paged_cache c, scope_paged_scales z, MoveArgs m, ReadArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * m.rows;
+  int2 place = make_int2(-1, 0);
+  if (lane < m.rows && i0 + lane < m.N) place = row_place(c, m, a.first, a.lens, i0 + lane);
+  const int dshift = __builtin_ctz(c.D) - 3;
+  const int n = static_cast<int>(min(static_cast<int64_t>(m.rows), m.N - i0));
+  each_chunk(m, n, place, [&](int r, int e, int page, int slot) {
+    const int h = e >> dshift, d = (e & ((1 << dshift) - 1)) * 8;
+    uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
+    if (page >= 0) {
+      float sk = 1.f, sv = 1.f;
+      if constexpr (KIND == kPages8) {
+        if (a.k_scale) sk = static_cast<const float*>(a.k_scale)[h];
+        if (a.v_scale) sv = static_cast<const float*>(a.v_scale)[h];
+      }
+      if constexpr (KIND == kPages4) {
+        const int at = slot * (c.D / 32) + d / 32;
+        sk = scale_of(static_cast<const uint8_t*>(a.k_scale)[page * z.k_sp + h * z.k_sh + at]);
+        sv = scale_of(static_cast<const uint8_t*>(a.v_scale)[page * z.v_sp + h * z.v_sh + at]);
+      }
+      const int dd = KIND == kPages4 ? d / 2 : d;
+      xk = read8<KIND, TYPE>(a.k_pages, page * c.k_sp + h * c.k_sh + slot * c.k_sr + dd, sk);
+      xv = read8<KIND, TYPE>(a.v_pages, page * c.v_sp + h * c.v_sh + slot * c.v_sr + dd, sv);
+    }
+    const int64_t to = (i0 + r) * c.Hkv * c.D + e * 8;
+    *reinterpret_cast<uint4*>(a.k + to) = xk;
+    *reinterpret_cast<uint4*>(a.v + to) = xv;
+  });
+}
+
+// ---- attention of one new token -------------------------------------------------
+// As over 16-bit pages (paged.hip: the tiles, the masks, the split), with K and V
+// widened to bf16, which holds every code and scale exactly; a q in fp16 is the sum of
+// two bf16 values, exactly.
+template <int TYPE, int D>
+__global__ __launch_bounds__(kAttnThreads, D == 256 ? 2 : 3) void paged_attn4_kernel(scope_paged_cache c, scope_paged_scales z,
+                                                                                      PagedAttnArgs a, AttnSplit s) {
+  constexpr int NJ = D / 32;                     // products over D
+  constexpr int VE = D / 16 < 8 ? D / 16 : 8;    // features of a lane in a row of V
+  constexpr int NH = D / (16 * VE);              // rows of V in halves
+  constexpr int KW = D == 64 ? 2 : 4;            // words of a lane in a row of K (twice for D = 256)
+  constexpr int NK = D / (32 * KW);              // (loads of them)
+  constexpr int NQ = TYPE == SCOPE_FP16 ? 2 : 1; // parts of q
+  constexpr int SB = D / 32;                     // bytes of a row's scales
+  constexpr int NP = 3;                          // bf16 values whose sum is a probability
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g4 = lane >> 4, c16 = lane & 15;
+  const int G = a.Hq / c.Hkv, ng = (G + 15) / 16;
+  const int hk = blockIdx.y / ng, cg = blockIdx.y % ng, nq = min(16, G - 16 * cg);
+  const int h0 = hk * G + 16 * cg;  // first query head
+  const bool lists = a.kv_idx != nullptr;
+  Piece p;
+  int n_list = 0;
+  if (lists) {
+    // pieces of one length for every list, so that the list is read without waiting for its number
+    p.b = blockIdx.x / s.pieces;
+    p.i = blockIdx.x % s.pieces;
+    p.n = s.pieces;
+    p.slot = p.b * s.pieces;
+    n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
+    piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
+  } else if (!find_piece(c, a, s, blockIdx.x, piece_turn(D), p)) {
+    return;
+  }
+  const int b = p.b;
+  if (s.plan && blockIdx.y == 0 && p.i == 0 && threadIdx.x == 0) s.plan[b] = make_int2(p.n, p.slot);
+  const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
+  const int end = static_cast<int>(seq_end(a.lens[b], cap)), low = a.first ? max(a.first[b], 0) : 0;
+  const int32_t* row = a.table + static_cast<int64_t>(b) * c.MP;
+  const int32_t* list = lists ? a.kv_idx + (static_cast<int64_t>(b) * c.Hkv + hk) * a.maxkv : nullptr;
+  const int shift = __builtin_ctz(c.bs);
+  const bool small = c.bs == 16;  // a tile is two pages
+
+  // Q^T: column c is query head h0 + c
+  uint4 qf[NQ][NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int d = D == 64 ? g4 * 16 + j * 8 : (j / 4) * 128 + g4 * 32 + (j % 4) * 8;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (c16 < nq) u = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (h0 + c16) * a.q_sh + d);
+    if constexpr (TYPE == SCOPE_BF16) {
+      qf[0][j] = u;
+    } else {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = low_half<SCOPE_FP16>(w[i]), y = high_half<SCOPE_FP16>(w[i]);
+        hi[i] = round2<SCOPE_BF16>(x, y);
+        lo[i] = round2<SCOPE_BF16>(x - low_half<SCOPE_BF16>(hi[i]), y - high_half<SCOPE_BF16>(hi[i]));
+      }
+      qf[0][j] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      qf[1][j] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+  }
+  const float to_log2 = a.scale * kLog2e;
+
+  f32x4_t acc[NH * VE];
+#pragma unroll
+  for (int i = 0; i < NH * VE; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // the maximum so far, what the probabilities are taken relative to, their sum
+  float m = -INFINITY, ref = 0.f, l = 0.f;
+
+  const char* kbase = static_cast<const char*>(a.k_pages) + hk * c.k_sh;
+  const char* vbase = static_cast<const char*>(a.v_pages) + hk * c.v_sh;
+  const uint8_t* ksbase = reinterpret_cast<const uint8_t*>(a.k_scale) + hk * z.k_sh;
+  const uint8_t* vsbase = reinterpret_cast<const uint8_t*>(a.v_scale) + hk * z.v_sh;
+  const int krow = (c16 >> 2) * 8 + (c16 & 3), vrow = g4 * 8;
+  const int krow_in = small ? krow & 15 : krow, vrow_in = small ? vrow & 15 : vrow;
+  const int64_t koff = krow_in * c.k_sr + g4 * (KW * 4);
+  const int64_t voff = vrow_in * c.v_sr + c16 * (VE / 2);
+  const int ksoff = krow_in * SB + (D == 64 ? g4 >> 1 : g4), vsoff = vrow_in * SB;
+  // where the byte of this lane's features is among a row's (a word's): rotated by this, it is at bit 23
+  const int vturn = (8 * (D == 64 ? c16 >> 3 : c16 >> 2) + 9) & 31;
+
+  // pages and blocks of this wavefront's next 64 tiles, one a lane (two where a tile is two pages)
+  int pg0 = -1, pg1 = -1, lb0 = 0, lb1 = 0;
+  const auto resolve = [&](int t) {
+    const auto one = [&](int64_t e, int& lb) -> int {  // entry e of the list, or block e
+      const int64_t blk = !lists ? e : e < a.maxkv ? list[e] : -1;
+      const int64_t page = block_page(row, c.MP, blk, c.P);
+      lb = page < 0 ? 0 : static_cast<int>(blk);
+      return lists && e >= n_list ? -1 : static_cast<int>(page);
+    };
+    pg0 = pg1 = -1;
+    lb0 = lb1 = 0;
+    if (t < p.t1) {
+      const int64_t e = (static_cast<int64_t>(t) * kTileKeys) >> shift;
+      pg0 = one(e, lb0);
+      if (small) pg1 = one(e + 1, lb1);
+    }
+  };
+
+  resolve(p.t0 + wave + lane * kAttnWaves);
+  if (lists) p.t1 = min(p.t1, static_cast<int>((static_cast<int64_t>(n_list) * c.bs + kTileKeys - 1) / kTileKeys));
+  int u = 0;
+  for (int t = p.t0 + wave; t < p.t1; t += kAttnWaves, ++u) {
+    if (u == 64) {
+      resolve(t + lane * kAttnWaves);
+      u = 0;
+    }
+    const int page0 = __builtin_amdgcn_readlane(pg0, u), page1 = small ? __builtin_amdgcn_readlane(pg1, u) : page0;
+    const auto put_sum = [&](float x) {  // log2 of the tile's sum (of this lane's half of it)
+      if (c16 < nq && (g4 & (small ? 1 : 3)) == 0)
+        s.tile_lse[(((static_cast<int64_t>(b) * a.Hq + h0 + c16) * s.tiles_cap + t) << small) + (small ? g4 >> 1 : 0)] = x;
+    };
+    if (page0 < 0 && page1 < 0) {  // nothing to see
+      if (s.tile_lse) put_sum(-INFINITY);
+      continue;
+    }
+    const int r0 = small ? 0 : (t * kTileKeys) & (c.bs - 1);  // the tile's first row in its page
+    // this lane's rows of K (product operand) and of V (and of the scores)
+    const int kp = small && krow >= 16 ? page1 : page0, vp = small && vrow >= 16 ? page1 : page0;
+    const int64_t kpage = max(kp, 0), vpage = max(vp, 0);
+    const char* kr = kbase + kpage * c.k_sp + r0 * c.k_sr + koff;
+    const char* vr = vbase + vpage * c.v_sp + r0 * c.v_sr + voff;
+    const uint8_t* ksr = ksbase + kpage * z.k_sp + r0 * SB + ksoff;
+    const uint8_t* vsr = vsbase + vpage * z.v_sp + r0 * SB + vsoff;
+    Words<KW> kf[2][NK];
+    uint32_t ks[2][NK];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        kf[i][j] = *reinterpret_cast<const Words<KW>*>(__builtin_assume_aligned(kr + 4 * i * c.k_sr + j * 64, 4 * KW));
+        ks[i][j] = ksr[4 * i * SB + 4 * j];
+      }
+    uint32_t vf[NH][8], vs[2 * SB];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        if constexpr (VE == 4)
+          vf[h][i] = *reinterpret_cast<const uint16_t*>(vr + i * c.v_sr);
+        else
+          vf[h][i] = *reinterpret_cast<const uint32_t*>(vr + i * c.v_sr + h * 64);
+      }
+#pragma unroll
+    for (int i = 0; i < SB / 2; ++i) {
+      const uint4 w = *reinterpret_cast<const uint4*>(vsr + 16 * i);
+      vs[4 * i] = w.x;
+      vs[4 * i + 1] = w.y;
+      vs[4 * i + 2] = w.z;
+      vs[4 * i + 3] = w.w;
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all loads are under way before the first is waited for
+
+    // scores
+    f32x4_t sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint32_t w = kf[i][j / KW].w[j % KW];
+        const float f = scale_of(ks[i][j / KW]);
+        const uint4 kk = make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)),
+                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)),
+                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)),
+                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3)));
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) sc[i] = mfma16(kk, qf[k][j], sc[i]);
+      }
+    }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * to_log2;
+    // the lane's first key; keys outside [low, end) and of no page are not seen
+    const int lbl = small && vrow >= 16 ? __builtin_amdgcn_readlane(lb1, u) : __builtin_amdgcn_readlane(lb0, u);
+    const int64_t pos = static_cast<int64_t>(lbl) * c.bs + r0 + vrow_in;
+    const int from = vp < 0 ? 8 : static_cast<int>(min(max(low - pos, static_cast<int64_t>(0)), static_cast<int64_t>(8)));
+    const int to = static_cast<int>(min(max(end - pos, static_cast<int64_t>(0)), static_cast<int64_t>(8)));
+    const bool cut = __any(from > 0 || to < 8);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool see = !cut || (i >= from && i < to);
+      x[i] = see ? x[i] : -INFINITY;
+      top = fmaxf(top, x[i]);
+    }
+    if (__any(top > m + 8.f)) {
+      top = over_rows(top, max_f32);
+      const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < NH * VE; ++i) acc[i] *= f;
+      m = mn;
+      ref = m == -INFINITY ? 0.f : m;
+    }
+    float lt = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+      lt += x[i];
+    }
+    l += lt;
+    if (s.tile_lse) {
+      lt = small ? over_rows2(lt, add_f32) : over_rows(lt, add_f32);
+      put_sum(ref + __builtin_amdgcn_logf(lt));
+    }
+    // the probabilities as a sum of bf16 values each
+    uint4 pf[NP];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = round2<SCOPE_BF16>(x[2 * i], x[2 * i + 1]);
+        x[2 * i] -= low_half<SCOPE_BF16>(w[i]);
+        x[2 * i + 1] -= high_half<SCOPE_BF16>(w[i]);
+      }
+      pf[k] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      uint32_t v[8][VE / 2];  // the eight rows as bf16 pairs of neighbouring features
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t w = vf[h][i], sw = D == 64 ? vs[i / 2] >> (16 * (i % 2)) : D == 128 ? vs[i] : vs[2 * i + h];
+        // (a row that is not seen may hold anything, and 0 times NaN is NaN)
+        const bool see = !cut || (i >= from && i < to);
+        w = see ? w : 0u;
+        sw = see ? sw : 0u;
+        const float f = __uint_as_float(__builtin_amdgcn_alignbit(sw, sw, vturn));
+        v[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0));
+        v[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1));
+        if constexpr (VE == 8) {
+          v[i][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2));
+          v[i][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+        uint32_t op[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          op[w] = j % 2 ? pack_hi16(v[2 * w][j / 2], v[2 * w + 1][j / 2]) : pack_lo16(v[2 * w][j / 2], v[2 * w + 1][j / 2]);
+        const uint4 vt = make_uint4(op[0], op[1], op[2], op[3]);
+#pragma unroll
+        for (int k = 0; k < NP; ++k) acc[h * VE + j] = mfma16(vt, pf[k], acc[h * VE + j]);
+      }
+    }
+  }
+  PagedAttnArgs plain = a;
+  plain.v_scale = nullptr;  // (the outputs have no factor of their own)
+  end_piece<TYPE, D, VE, NH>(plain, s, p, hk, h0, nq, m, ref, l, acc, lds);
+}
+
+namespace {
+int check_scales(const scope_paged_cache* c, const scope_paged_scales* z, const void* k_scale, const void* v_scale, const char* fn) {
+  SCOPE_REQUIRE(z && k_scale && v_scale, "%s: null scales", fn);
+  SCOPE_REQUIRE(z->k_sp % 16 == 0 && z->k_sh % 16 == 0 && z->v_sp % 16 == 0 && z->v_sh % 16 == 0 && aligned16(k_scale) &&
+                    aligned16(v_scale),
+                "%s: the scales of a page's head must be 16-byte aligned", fn);
+  return SCOPE_OK;
+}
+
+// pages of bytes as check_cache knows them
+scope_paged_cache in_bytes(const scope_paged_cache& c) {
+  scope_paged_cache x = c;
+  x.fp8 = 1;
+  return x;
+}
+
+MoveArgs move_args(const scope_paged_cache& c, int64_t N, const int32_t* cu, const int32_t* table) {
+  const int chunks = c.Hkv * (c.D / 8);
+  return MoveArgs{N, moved_rows(N, chunks), chunks, 64 / chunks, 64 % chunks, cu, table};
+}
+}  // namespace
+
+}  // namespace scope
+
+using namespace scope;
+
+extern "C" {
+
+int scope_paged_append_fp4(const scope_paged_cache* c, const scope_paged_scales* z, int64_t N, const uint16_t* k, int64_t k_sn,
+                           int64_t k_sh, const uint16_t* v, int64_t v_sn, int64_t v_sh, const int32_t* cu, const int32_t* table,
+                           const int32_t* lens, void* k_scale, void* v_scale, void* k_pages, void* v_pages, void* stream) {
+  const char* fn = "scope_paged_append_fp4";
+  SCOPE_REQUIRE(c, "%s: null cache", fn);
+  const scope_paged_cache bytes = in_bytes(*c);
+  if (int rc = check_cache(&bytes, k_pages, v_pages, fn)) return rc;
+  if (int rc = check_scales(c, z, k_scale, v_scale, fn)) return rc;
+  SCOPE_REQUIRE(N >= 0 && N <= INT32_MAX, "%s: %lld rows (0 .. 2^31 - 1)", fn, (long long)N);
+  SCOPE_REQUIRE(cu || N <= c->B, "%s: %lld rows for %d sequences need cu", fn, (long long)N, c->B);
+  if (N == 0) return SCOPE_OK;
+  SCOPE_REQUIRE(k && v && table && lens, "%s: null pointer", fn);
+  SCOPE_REQUIRE(aligned16(k) && aligned16(v) && k_sn % 8 == 0 && k_sh % 8 == 0 && v_sn % 8 == 0 && v_sh % 8 == 0,
+                "%s: the rows of k and v must be 16-byte aligned", fn);
+  const MoveArgs m = move_args(*c, N, cu, table);
+  const Append4Args a{k_sn, k_sh, v_sn, v_sh, k, v, lens, static_cast<uint8_t*>(k_pages), static_cast<uint8_t*>(v_pages),
+                      static_cast<uint8_t*>(k_scale), static_cast<uint8_t*>(v_scale)};
+  const dim3 grid(ceil_div(N, 4 * m.rows)), block(256);
+  if (c->type == SCOPE_BF16)
+    hipLaunchKernelGGL(paged_append4_kernel<SCOPE_BF16>, grid, block, 0, as_stream(stream), bytes, *z, m, a);
+  else
+    hipLaunchKernelGGL(paged_append4_kernel<SCOPE_FP16>, grid, block, 0, as_stream(stream), bytes, *z, m, a);
+  return check_launch("paged_append4_kernel");
+}
+
+int scope_paged_read(const scope_paged_cache* c, const scope_paged_scales* z, int64_t N, const int32_t* cu, const int32_t* table,
+                     const int32_t* lens, const int32_t* first, const void* k_scale, const void* v_scale, const void* k_pages,
+                     const void* v_pages, uint16_t* k, uint16_t* v, void* stream) {
+  const char* fn = "scope_paged_read";
+  SCOPE_REQUIRE(c, "%s: null cache", fn);
+  const scope_paged_cache as = z ? in_bytes(*c) : *c;
+  if (int rc = check_cache(&as, k_pages, v_pages, fn)) return rc;
+  if (z)
+    if (int rc = check_scales(c, z, k_scale, v_scale, fn)) return rc;
+  SCOPE_REQUIRE(N >= 0 && N <= INT32_MAX, "%s: %lld rows (0 .. 2^31 - 1)", fn, (long long)N);
+  SCOPE_REQUIRE(cu || N <= c->B, "%s: %lld rows for %d sequences need cu", fn, (long long)N, c->B);
+  if (N == 0) return SCOPE_OK;
+  SCOPE_REQUIRE(table && lens && k && v, "%s: null pointer", fn);
+  SCOPE_REQUIRE(aligned16(k) && aligned16(v), "%s: k and v must be 16-byte aligned", fn);
+  const MoveArgs m = move_args(*c, N, cu, table);
+  const ReadArgs a{lens, first, k_pages, v_pages, k_scale, v_scale, k, v};
+  const scope_paged_scales none{};
+  const dim3 grid(ceil_div(N, 4 * m.rows)), block(256);
+  hipStream_t st = as_stream(stream);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, as, z ? *z : none, m, a); };
+  if (z)
+    c->type == SCOPE_BF16 ? launch(paged_read_kernel<kPages4, SCOPE_BF16>) : launch(paged_read_kernel<kPages4, SCOPE_FP16>);
+  else if (c->fp8)
+    c->type == SCOPE_BF16 ? launch(paged_read_kernel<kPages8, SCOPE_BF16>) : launch(paged_read_kernel<kPages8, SCOPE_FP16>);
+  else  // (16-bit values are moved as they are)
+    launch(paged_read_kernel<kPages16, SCOPE_BF16>);
+  return check_launch("paged_read_kernel");
+}
+
+int scope_paged_decode_attn_fp4(const scope_paged_cache* c, const scope_paged_scales* z, int Hq, int maxkv, float scale,
+                                const uint16_t* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
+                                const void* k_scale, const void* v_scale, const int32_t* table, const int32_t* lens,
+                                const int32_t* first, const int32_t* kv_num, const int32_t* kv_idx, float* mass, void* work,
+                                uint16_t* out, float* lse, void* stream) {
+  const char* fn = "scope_paged_decode_attn_fp4";
+  SCOPE_REQUIRE(c, "%s: null cache", fn);
+  const scope_paged_cache bytes = in_bytes(*c);
+  if (int rc = check_cache(&bytes, k_pages, v_pages, fn)) return rc;
+  if (int rc = check_scales(c, z, k_scale, v_scale, fn)) return rc;
+  PagedAttnArgs a{Hq,
+                  maxkv,
+                  scale,
+                  q_sb,
+                  q_sh,
+                  q,
+                  k_pages,
+                  v_pages,
+                  reinterpret_cast<const float*>(k_scale),
+                  reinterpret_cast<const float*>(v_scale),
+                  table,
+                  lens,
+                  first,
+                  kv_num,
+                  kv_idx,
+                  mass,
+                  out,
+                  lse};
+  AttnSplit s;
+  if (int rc = check_attn(bytes, a, work, &s, fn)) return rc;
+  const int G = Hq / c->Hkv, ng = (G + 15) / 16;
+  const dim3 grid(s.slots, c->Hkv * ng);
+  const size_t lds = sizeof(float) * kAttnWaves * (32 + static_cast<size_t>(std::min(G, 16)) * c->D);
+  hipStream_t st = as_stream(stream);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kAttnThreads), lds, st, bytes, *z, a, s); };
+  if (c->type == SCOPE_BF16)
+    c->D == 64    ? launch(paged_attn4_kernel<SCOPE_BF16, 64>)
+    : c->D == 128 ? launch(paged_attn4_kernel<SCOPE_BF16, 128>)
+                  : launch(paged_attn4_kernel<SCOPE_BF16, 256>);
+  else
+    c->D == 64    ? launch(paged_attn4_kernel<SCOPE_FP16, 64>)
+    : c->D == 128 ? launch(paged_attn4_kernel<SCOPE_FP16, 128>)
+                  : launch(paged_attn4_kernel<SCOPE_FP16, 256>);
+  if (int rc = check_launch("paged_attn4_kernel")) return rc;
+  a.v_scale = nullptr;
+  return launch_paged_finish(bytes, a, s, st);
+}
+
+}  // extern "C"

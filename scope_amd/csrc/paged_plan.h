@@ -118,13 +118,21 @@ SCOPE_HD int append_rows(int64_t N) {
   return rows;
 }
 
+// rows of a wavefront that moves N of them in `chunks` of eight features each: as
+// many as fill its lanes, and those of append_rows
+SCOPE_HD int moved_rows(int64_t N, int chunks) {
+  int rows = append_rows(N);
+  while (rows < 64 && rows * chunks < 64) rows *= 2;
+  return rows;
+}
+
 // where row i of the new ones goes: its sequence in *b and its position, -1 for
 // a row of no sequence.  cu [B + 1] or null (row i to sequence i); whatever cu
-// holds, *b stays in [0, B).
+// holds, *b stays in [0, B).  lens [B] or null (0): the position of a sequence's first.
 SCOPE_HD int64_t row_position(const int32_t* cu, const int32_t* lens, int B, int64_t i, int* b) {
   if (!cu) {
     *b = static_cast<int>(i);
-    return static_cast<int64_t>(lens[i]);
+    return lens ? static_cast<int64_t>(lens[i]) : 0;
   }
   int lo = 0, hi = B;  // the last b in [0, B) with cu[b] <= i, if cu does not decrease
   while (lo + 1 < hi) {
@@ -136,7 +144,7 @@ SCOPE_HD int64_t row_position(const int32_t* cu, const int32_t* lens, int B, int
   }
   *b = lo;
   if (i < cu[lo] || i >= cu[lo + 1]) return -1;
-  return static_cast<int64_t>(lens[lo]) + (i - cu[lo]);
+  return (lens ? static_cast<int64_t>(lens[lo]) : 0) + (i - cu[lo]);
 }
 
 }  // namespace scope

@@ -1108,7 +1108,7 @@ def decoder_step(prm, table: torch.Tensor, work: torch.Tensor, tok: torch.Tensor
 
 # ---- the paged cache of a decode loop over several sequences --------------------
 _PAGED_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_FP8 = torch.float8_e4m3fn
+_FP8, _FP4, _E8M0 = torch.float8_e4m3fn, torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
 _F32_MIN, _F32_MAX = 2.0 ** -126, (2 - 2.0 ** -23) * 2.0 ** 127
 _INT_MAX = 2 ** 31 - 1  # (a C int takes the low 32 bits of what is larger)
 
@@ -1192,16 +1192,23 @@ def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: 
     shape, pt = k_pages.shape, k_pages.dtype
     if len(shape) != 4 or shape != v_pages.shape or pt != v_pages.dtype:
         raise RuntimeError(f"{who}: k_pages and v_pages must be [P, Hkv, bs, D] of one shape and type")
-    fp8 = pt == _FP8
-    if (dtype != torch.bfloat16 and dtype != torch.float16) or not (fp8 or pt == dtype):
-        raise RuntimeError(f"{who}: bfloat16 or float16 rows with pages of their type or float8_e4m3fn "
+    fp8, fp4 = pt == _FP8, pt == _FP4
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or not (fp8 or fp4 or pt == dtype):
+        raise RuntimeError(f"{who}: bfloat16 or float16 rows with pages of their type, float8_e4m3fn or float4_e2m1fn_x2 "
                            f"(got {dtype} and {pt})")
     if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.numel() > _INT_MAX:
         raise RuntimeError(f"{who}: table must be a contiguous int32 [B, MP] of less than 2^31 entries")
     P, Hkv, bs, D = shape
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t is not None and (not fp8 or t.dtype != torch.float32 or t.numel() != Hkv or not t.is_contiguous()):
-            raise RuntimeError(f"{who}: {name} must be a contiguous float32 [{Hkv}], with float8_e4m3fn pages")
+    if fp4:
+        D *= 2
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is None or t.dtype != _E8M0 or t.shape != (P, Hkv, bs, D // 32) or t.stride()[2:] != (D // 32, 1):
+                raise RuntimeError(f"{who}: {name} must be float8_e8m0fnu [{P}, {Hkv}, {bs}, {D // 32}], contiguous in a page's head, "
+                                   "with float4_e2m1fn_x2 pages")
+    else:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is not None and (not fp8 or t.dtype != torch.float32 or t.numel() != Hkv or not t.is_contiguous()):
+                raise RuntimeError(f"{who}: {name} must be a contiguous float32 [{Hkv}], with float8_e4m3fn pages")
     kp, kh, kr, kd = k_pages.stride()
     vp, vh, vr, vd = v_pages.stride()
     if kd != 1 or vd != 1:
@@ -1214,6 +1221,16 @@ def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: 
     return _lib.PagedCache(B, Hkv, D, bs, MP, _PAGED_TYPES[dtype], fp8, P, kp, kh, kr, vp, vh, vr)
 
 
+def _paged_scales(c: "_lib.PagedCache", k_scale: torch.Tensor, v_scale: torch.Tensor) -> "_lib.PagedScales":
+    """The strides of a 4-bit cache's scales."""
+    (kp, kh, _, _), (vp, vh, _, _) = k_scale.stride(), v_scale.stride()
+    if c.P == 1:
+        kp = vp = 0
+    if c.Hkv == 1:
+        kh = vh = 0
+    return _lib.PagedScales(kp, kh, vp, vh)
+
+
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                  lens: torch.Tensor, *, cu: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None) -> None:
@@ -1222,7 +1239,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     k, v [N, Hkv, D] bf16 or fp16 (any row and head strides, rows 16-byte
     aligned); k_pages, v_pages [P, Hkv, bs, D] of the same type, or
     float8_e4m3fn holding x / scale[h] cut to ±448 (k_scale, v_scale [Hkv]
-    fp32); table [B, MP] int32 page ids; lens [B] the positions each sequence
+    fp32), or float4_e2m1fn_x2 [P, Hkv, bs, D / 2] with k_scale, v_scale [P,
+    Hkv, bs, D / 32] float8_e8m0fnu, which are written too: a power of two for
+    each 32 features, at least a seventh of the largest (a group with an
+    infinity or a NaN becomes NaN); table [B, MP] int32 page ids; lens [B] the positions each sequence
     holds before the call (it is not changed).  Row i goes to sequence b with
     cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing; without it N <= B
     and row i to sequence i), position lens[b] + i - cu[b].  Rows of no
@@ -1235,16 +1255,58 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)
     if len(shape) != 3 or shape != v.shape or v.dtype != dtype or shape[1] != c.Hkv or shape[2] != c.D or ks[2] != 1 or vs[2] != 1:
         raise RuntimeError(f"{who}: k and v must be [N, {c.Hkv}, {c.D}] of one type with a contiguous last dimension")
-    if not (c.k_sp and c.k_sh and c.k_sr and c.v_sp and c.v_sh and c.v_sr):
-        for t in (k_pages, v_pages):
-            if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-                raise RuntimeError(f"{who}: the pages are an expanded tensor: their rows share memory")
+    fp4 = k_pages.dtype == _FP4
+    for t in (k_pages, v_pages) + ((k_scale, v_scale) if fp4 else ()):
+        if 0 in t.stride() and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            raise RuntimeError(f"{who}: the pages are an expanded tensor: their rows share memory")
     lens = _ints(who, "lens", lens, c.B, dev)
     cu = _ints(who, "cu", cu, c.B + 1, dev)
     N, one = shape[0], c.Hkv == 1
-    _launch(dev, "scope_paged_append", C.byref(c), N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1],
-            v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1], _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale),
-            _ptr(v_scale), k_pages.data_ptr(), v_pages.data_ptr())
+    args = (N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1], v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1],
+            _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(), v_pages.data_ptr())
+    if fp4:
+        _launch(dev, "scope_paged_append_fp4", C.byref(c), C.byref(_paged_scales(c, k_scale, v_scale)), *args)
+    else:
+        _launch(dev, "scope_paged_append", C.byref(c), *args)
+
+
+def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, rows: int,
+               cu: torch.Tensor | None = None, first: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+               v_scale: torch.Tensor | None = None, dtype: torch.dtype | None = None):
+    """Rows of a paged cache one after the other -> k, v [rows, Hkv, D] of
+    ``dtype``: what a dense attention of a prompt's next tokens takes, or
+    another pool.
+
+    The cache as ``paged_append`` fills it, pages of any type.  Row i is that of
+    sequence b with cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing;
+    without it rows <= B and row i is of sequence i), position first[b] + i -
+    cu[b] (first [B], without it 0; without cu first[b]).  Rows of no sequence,
+    outside [0, lens[b]), past the table, or of a block whose entry is outside
+    [0, P) are zeros.  ``dtype``: bfloat16 or float16; 16-bit pages are read in
+    their own type (the default then), others in bfloat16 by default.  4-bit
+    values are exact in bfloat16; e4m3 ones are the fp32 product with their
+    scale, rounded.  Nothing of it waits for the GPU.  It has no backward: a
+    gradient that reaches its results raises."""
+    who = "paged_read"
+    if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad):
+        return _NoGradient.apply(who, functools.partial(paged_read, k_pages, v_pages, table, lens, rows=rows, cu=cu, first=first,
+                                                        k_scale=k_scale, v_scale=v_scale, dtype=dtype), k_pages, v_pages)
+    dev = _device(who, k_pages, v_pages, table, lens, cu, first, k_scale, v_scale)
+    pt = k_pages.dtype
+    if dtype is None:
+        dtype = torch.bfloat16 if pt == _FP8 or pt == _FP4 else pt
+    c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)
+    rows = int(rows)
+    if not 0 <= rows <= (_INT_MAX if cu is not None else c.B):
+        raise RuntimeError(f"{who}: rows={rows} must be 0 .. 2^31 - 1, without cu at most the sequences' number ({c.B})")
+    lens = _ints(who, "lens", lens, c.B, dev)
+    cu = _ints(who, "cu", cu, c.B + 1, dev)
+    first = _ints(who, "first", first, c.B, dev)
+    k, v = (torch.empty((rows, c.Hkv, c.D), dtype=dtype, device=dev) for _ in range(2))
+    scales = C.byref(_paged_scales(c, k_scale, v_scale)) if pt == _FP4 else None
+    _launch(dev, "scope_paged_read", C.byref(c), scales, rows, _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(first), _ptr(k_scale),
+            _ptr(v_scale), k_pages.data_ptr(), v_pages.data_ptr(), k.data_ptr(), v.data_ptr())
+    return k, v
 
 
 def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -1302,9 +1364,13 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
     need = _paged_work_bytes(query, B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _launch(dev, "scope_paged_decode_attn", C.byref(c), Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0,
-            qs[1] if Hq > 1 else 0, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(),
-            lens.data_ptr(), _ptr(first), _ptr(kv_num), _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr())
+    args = (Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0, qs[1] if Hq > 1 else 0, k_pages.data_ptr(),
+            v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _ptr(first), _ptr(kv_num),
+            _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr())
+    if k_pages.dtype == _FP4:
+        _launch(dev, "scope_paged_decode_attn_fp4", C.byref(c), C.byref(_paged_scales(c, k_scale, v_scale)), *args)
+    else:
+        _launch(dev, "scope_paged_decode_attn", C.byref(c), *args)
     return out, lse
 
 
