@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     p.slot = p.b * s.pieces;
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
-  } else if (!find_piece(c, a, s, blockIdx.x, piece_turn(D), p)) {
+  } else if (!find_piece(c, a, blockIdx.x, piece_turn(D), [&](int64_t) { return s.pieces; }, p)) {
     return;
   }
   const int b = p.b;
@@ -415,7 +415,26 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     }
   }
 
-  end_piece<TYPE, D, VE, NH>(a, s, p, hk, h0, nq, m, ref, l, acc, lds);
+  // the wavefronts' shares: maxima and sums, then the outputs of the group's queries
+  l = over_rows(l, add_f32);
+  const Shares z = shares_of(lds);
+  if (g4 == 0) {
+    z.sm[wave * 16 + c16] = m == -INFINITY ? m : ref;
+    z.sl[wave * 16 + c16] = l;
+  }
+  if (c16 < nq) {
+    float* o = z.so + (wave * nq + c16) * D + g4 * 4 * VE;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VE; j += 4)
+          *reinterpret_cast<float4*>(o + h * 128 + r * VE + j) = make_float4(
+              acc[h * VE + j][r], acc[h * VE + j + 1][r], acc[h * VE + j + 2][r], acc[h * VE + j + 3][r]);
+  }
+  __syncthreads();
+  join_shares<TYPE, D>(a, s, p, h0, nq, a.v_scale ? a.v_scale[hk] : 1.f, z);
 }
 
 // (maximum, sum relative to it) of a row from its n pieces' (maximum, sum) pairs,

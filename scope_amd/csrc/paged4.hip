@@ -227,56 +227,102 @@ __global__ __launch_bounds__(256) void paged_read_kernel(scope_paged_cache c, sc
 // As over 16-bit pages (paged.hip: the tiles, the masks, the split), with K and V
 // widened to bf16, which holds every code and scale exactly; a q in fp16 is the sum of
 // two bf16 values, exactly.
-template <int TYPE, int D>
-__global__ __launch_bounds__(kAttnThreads, D == 256 ? 2 : 3) void paged_attn4_kernel(scope_paged_cache c, scope_paged_scales z,
+typedef const __attribute__((address_space(1))) char* bytes_t;  // in device memory
+template <class T>
+__device__ __forceinline__ T read_as(bytes_t p) {
+  return *(const __attribute__((address_space(1))) T*)p;  // (an address-space cast needs a C-style cast)
+}
+
+template <class T>
+__device__ __forceinline__ T read_once(bytes_t p) {
+  return __builtin_nontemporal_load((const __attribute__((address_space(1))) T*)p);
+}
+template <int D>
+struct Tile4 {  // a lane's share of 32 keys and their scales
+  static constexpr int VE = D / 16 < 8 ? D / 16 : 8;  // features in a row of V
+  static constexpr int NH = D / (16 * VE);            // (in halves)
+  static constexpr int KW = D == 64 ? 2 : 4;          // words in a row of K
+  static constexpr int NK = D / (32 * KW);            // (parts of it)
+  static constexpr int SB = D / 32;                   // bytes of a row's scales
+  typedef uint32_t Row __attribute__((ext_vector_type(KW)));
+  Row k[2][NK];
+  uint32_t ks[2][NK];
+  uint32_t v[NH][8];
+  uint32_t vs[2 * SB];
+};
+
+constexpr int attn4_waves(int D, int type, bool wide, bool small) {  // wavefronts a SIMD that the registers are cut to
+  return D == 256 ? (wide ? 1 : 2) : D == 64 ? (wide ? 3 : 4) : wide ? 2 : small || type == SCOPE_FP16 ? 3 : 4;
+}
+
+template <int TYPE, int D, bool WIDE, bool SMALL>
+__global__ __launch_bounds__(kAttnThreads, attn4_waves(D, TYPE, WIDE, SMALL)) void paged_attn4_kernel(scope_paged_cache c, scope_paged_scales z,
                                                                                       PagedAttnArgs a, AttnSplit s) {
-  constexpr int NJ = D / 32;                     // products over D
-  constexpr int VE = D / 16 < 8 ? D / 16 : 8;    // features of a lane in a row of V
-  constexpr int NH = D / (16 * VE);              // rows of V in halves
-  constexpr int KW = D == 64 ? 2 : 4;            // words of a lane in a row of K (twice for D = 256)
-  constexpr int NK = D / (32 * KW);              // (loads of them)
-  constexpr int NQ = TYPE == SCOPE_FP16 ? 2 : 1; // parts of q
-  constexpr int SB = D / 32;                     // bytes of a row's scales
-  constexpr int NP = 3;                          // bf16 values whose sum is a probability
+  using Tile = Tile4<D>;
+  constexpr int VE = Tile::VE, NH = Tile::NH, KW = Tile::KW, NK = Tile::NK, SB = Tile::SB;
+  constexpr int NP2 = VE / 2;                     // pairs of features of a lane in a row of V
+  constexpr int NJ = D / 32;                      // products over D
+  constexpr int NQ = TYPE == SCOPE_FP16 ? 2 : 1;  // bf16 values whose sum is one of q
+  constexpr int NP = 3;                           // bf16 values whose sum is a probability
+  constexpr int NC = WIDE ? 2 : 1;                // outputs of even and of odd features: in columns of their own, or beside each other
+  constexpr bool kPast = !SMALL && D >= 128;      // K passes the caches
   extern __shared__ float lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g4 = lane >> 4, c16 = lane & 15;
+  // (what is the same for a wavefront is told to the compiler: scalar registers, branches and addresses)
+  const auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int lane = threadIdx.x & 63, wave = same(threadIdx.x >> 6), g4 = lane >> 4, c16 = lane & 15;
   const int G = a.Hq / c.Hkv, ng = (G + 15) / 16;
-  const int hk = blockIdx.y / ng, cg = blockIdx.y % ng, nq = min(16, G - 16 * cg);
-  const int h0 = hk * G + 16 * cg;  // first query head
+  // the columns of one piece start together, and pieces that there are not last
+  const int cols = gridDim.y;
+  const int64_t id = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+  const int slot = same(static_cast<int>(id / cols)), column = same(static_cast<int>(id % cols));
+  const int hk = column / ng, cg = column % ng, nq = min(16, G - 16 * cg);
+  const int h0 = hk * G + 16 * cg;                // first query head
+  const int col = WIDE ? c16 : c16 & 7;           // this lane's
   const bool lists = a.kv_idx != nullptr;
   Piece p;
   int n_list = 0;
   if (lists) {
     // pieces of one length for every list, so that the list is read without waiting for its number
-    p.b = blockIdx.x / s.pieces;
-    p.i = blockIdx.x % s.pieces;
+    p.b = slot / s.pieces;
+    p.i = slot % s.pieces;
     p.n = s.pieces;
     p.slot = p.b * s.pieces;
+    p.len = a.lens[p.b];
+    p.first = a.first ? a.first[p.b] : 0;
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
-  } else if (!find_piece(c, a, s, blockIdx.x, piece_turn(D), p)) {
+  } else if (!find_piece(c, a, slot, piece_turn(D),
+                         [&](int64_t total) { return min(s.pieces, (pieces_wanted4(total * cols) + cols - 1) / cols); }, p)) {
     return;
   }
+  p.b = same(p.b);
+  p.i = same(p.i);
+  p.n = same(p.n);
+  p.slot = same(p.slot);
+  p.t0 = same(p.t0);
+  p.t1 = same(p.t1);
   const int b = p.b;
-  if (s.plan && blockIdx.y == 0 && p.i == 0 && threadIdx.x == 0) s.plan[b] = make_int2(p.n, p.slot);
+  if (s.plan && column == 0 && p.i == 0 && threadIdx.x == 0) s.plan[b] = make_int2(p.n, p.slot);
   const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
-  const int end = static_cast<int>(seq_end(a.lens[b], cap)), low = a.first ? max(a.first[b], 0) : 0;
+  const int end = same(static_cast<int>(seq_end(p.len, cap))), low = same(max(p.first, 0));
   const int32_t* row = a.table + static_cast<int64_t>(b) * c.MP;
   const int32_t* list = lists ? a.kv_idx + (static_cast<int64_t>(b) * c.Hkv + hk) * a.maxkv : nullptr;
   const int shift = __builtin_ctz(c.bs);
-  const bool small = c.bs == 16;  // a tile is two pages
 
-  // Q^T: column c is query head h0 + c
+  // Q^T: column c is query head h0 + col.  Scores are taken times the scale's size, q
+  // with its sign (0 where it is 0), so that the largest product is the largest score.
+  const float c_log2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, keep = a.scale == 0.f ? 0u : ~0u;
   uint4 qf[NQ][NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int d = D == 64 ? g4 * 16 + j * 8 : (j / 4) * 128 + g4 * 32 + (j % 4) * 8;
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (c16 < nq) u = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (h0 + c16) * a.q_sh + d);
+    if (col < nq) u = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (h0 + col) * a.q_sh + d);
+    const uint32_t w[4] = {(u.x ^ flip) & keep, (u.y ^ flip) & keep, (u.z ^ flip) & keep, (u.w ^ flip) & keep};
     if constexpr (TYPE == SCOPE_BF16) {
-      qf[0][j] = u;
+      qf[0][j] = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -288,29 +334,34 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 2 : 3) void paged_attn4_ke
       qf[1][j] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
-  const float to_log2 = a.scale * kLog2e;
 
-  f32x4_t acc[NH * VE];
+  f32x4_t acc[NC][NH * NP2];
 #pragma unroll
-  for (int i = 0; i < NH * VE; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < NC; ++n)
+#pragma unroll
+    for (int i = 0; i < NH * NP2; ++i) acc[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   // the maximum so far, what the probabilities are taken relative to, their sum
   float m = -INFINITY, ref = 0.f, l = 0.f;
 
-  const char* kbase = static_cast<const char*>(a.k_pages) + hk * c.k_sh;
-  const char* vbase = static_cast<const char*>(a.v_pages) + hk * c.v_sh;
-  const uint8_t* ksbase = reinterpret_cast<const uint8_t*>(a.k_scale) + hk * z.k_sh;
-  const uint8_t* vsbase = reinterpret_cast<const uint8_t*>(a.v_scale) + hk * z.v_sh;
+  const bytes_t kbase = (bytes_t)a.k_pages + hk * c.k_sh;
+  const bytes_t vbase = (bytes_t)a.v_pages + hk * c.v_sh;
+  const bytes_t ksbase = (bytes_t)a.k_scale + hk * z.k_sh;
+  const bytes_t vsbase = (bytes_t)a.v_scale + hk * z.v_sh;
+  // operand A of the scores: row m is key 8 (m / 4) + 4 i + m % 4 of the tile in product i
   const int krow = (c16 >> 2) * 8 + (c16 & 3), vrow = g4 * 8;
-  const int krow_in = small ? krow & 15 : krow, vrow_in = small ? vrow & 15 : vrow;
-  const int64_t koff = krow_in * c.k_sr + g4 * (KW * 4);
-  const int64_t voff = vrow_in * c.v_sr + c16 * (VE / 2);
-  const int ksoff = krow_in * SB + (D == 64 ? g4 >> 1 : g4), vsoff = vrow_in * SB;
+  const int krow_in = SMALL ? krow & 15 : krow, vrow_in = SMALL ? vrow & 15 : vrow;
+  // (row strides are less than 2^26 bytes)
+  const uint32_t koff = krow_in * static_cast<uint32_t>(c.k_sr) + g4 * (KW * 4);
+  const uint32_t voff = vrow_in * static_cast<uint32_t>(c.v_sr) + c16 * (VE / 2);
+  const uint32_t ksoff = krow_in * SB + (D == 64 ? g4 >> 1 : g4), vsoff = vrow_in * SB;
   // where the byte of this lane's features is among a row's (a word's): rotated by this, it is at bit 23
   const int vturn = (8 * (D == 64 ? c16 >> 3 : c16 >> 2) + 9) & 31;
+  // a probability's upper half in the half of a word that this lane's column takes (bytes of 0 beside it)
+  const uint32_t half = c16 < 8 ? 0x0c0c0706u : 0x07060c0cu;
 
   // pages and blocks of this wavefront's next 64 tiles, one a lane (two where a tile is two pages)
   int pg0 = -1, pg1 = -1, lb0 = 0, lb1 = 0;
-  const auto resolve = [&](int t) {
+  const auto resolve = [&](int t) __attribute__((always_inline)) {
     const auto one = [&](int64_t e, int& lb) -> int {  // entry e of the list, or block e
       const int64_t blk = !lists ? e : e < a.maxkv ? list[e] : -1;
       const int64_t page = block_page(row, c.MP, blk, c.P);
@@ -322,163 +373,273 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 2 : 3) void paged_attn4_ke
     if (t < p.t1) {
       const int64_t e = (static_cast<int64_t>(t) * kTileKeys) >> shift;
       pg0 = one(e, lb0);
-      if (small) pg1 = one(e + 1, lb1);
+      if constexpr (SMALL) pg1 = one(e + 1, lb1);
+    }
+  };
+  struct Where {  // a tile's pages (-1: none), their first positions in it, its first row in its page
+    int page0, page1, pos0, pos1, r0;
+  };
+  int u = 0;
+  const auto where = [&](int t) __attribute__((always_inline)) {  // of tile t, entry u of the 64
+    Where w;
+    w.page0 = __builtin_amdgcn_readlane(pg0, u);
+    w.page1 = SMALL ? __builtin_amdgcn_readlane(pg1, u) : w.page0;
+    w.r0 = SMALL ? 0 : (t * kTileKeys) & (c.bs - 1);
+    w.pos0 = (__builtin_amdgcn_readlane(lb0, u) << shift) + w.r0;
+    w.pos1 = SMALL ? __builtin_amdgcn_readlane(lb1, u) << shift : w.pos0 + 16;
+    return w;
+  };
+
+  const auto put_sum = [&](int t, float x) {  // log2 of tile t's sum (of this lane's half of it)
+    if (c16 < nq && (g4 & (SMALL ? 1 : 3)) == 0)
+      s.tile_lse[((static_cast<int64_t>(b) * a.Hq + h0 + c16) * s.tiles_cap + t) * (SMALL ? 2 : 1) + (SMALL ? g4 >> 1 : 0)] = x;
+  };
+  int t = p.t0 + wave;
+  const auto seek = [&]() __attribute__((always_inline)) {  // from tile t on to one that has a page
+    while (t < p.t1) {
+      if (u == 64) {
+        resolve(t + lane * kAttnWaves);
+        u = 0;
+      }
+      if (__builtin_amdgcn_readlane(pg0, u) >= 0 || (SMALL && __builtin_amdgcn_readlane(pg1, u) >= 0)) return;
+      if (s.tile_lse) put_sum(t, -INFINITY);
+      t += kAttnWaves;
+      ++u;
     }
   };
 
-  resolve(p.t0 + wave + lane * kAttnWaves);
-  if (lists) p.t1 = min(p.t1, static_cast<int>((static_cast<int64_t>(n_list) * c.bs + kTileKeys - 1) / kTileKeys));
-  int u = 0;
-  for (int t = p.t0 + wave; t < p.t1; t += kAttnWaves, ++u) {
-    if (u == 64) {
-      resolve(t + lane * kAttnWaves);
-      u = 0;
-    }
-    const int page0 = __builtin_amdgcn_readlane(pg0, u), page1 = small ? __builtin_amdgcn_readlane(pg1, u) : page0;
-    const auto put_sum = [&](float x) {  // log2 of the tile's sum (of this lane's half of it)
-      if (c16 < nq && (g4 & (small ? 1 : 3)) == 0)
-        s.tile_lse[(((static_cast<int64_t>(b) * a.Hq + h0 + c16) * s.tiles_cap + t) << small) + (small ? g4 >> 1 : 0)] = x;
+  const auto load = [&](const Where& w, Tile& x) __attribute__((always_inline)) {
+    // (a scalar address and a lane's offset as the loads take them, which the compiler would
+    // otherwise add up in registers that earlier loads are still on their way to)
+    const auto row = [](bytes_t p) __attribute__((always_inline)) {
+      if constexpr (!SMALL) asm("" : "+s"(p));
+      return p;
     };
-    if (page0 < 0 && page1 < 0) {  // nothing to see
-      if (s.tile_lse) put_sum(-INFINITY);
-      continue;
-    }
-    const int r0 = small ? 0 : (t * kTileKeys) & (c.bs - 1);  // the tile's first row in its page
-    // this lane's rows of K (product operand) and of V (and of the scores)
-    const int kp = small && krow >= 16 ? page1 : page0, vp = small && vrow >= 16 ? page1 : page0;
-    const int64_t kpage = max(kp, 0), vpage = max(vp, 0);
-    const char* kr = kbase + kpage * c.k_sp + r0 * c.k_sr + koff;
-    const char* vr = vbase + vpage * c.v_sp + r0 * c.v_sr + voff;
-    const uint8_t* ksr = ksbase + kpage * z.k_sp + r0 * SB + ksoff;
-    const uint8_t* vsr = vsbase + vpage * z.v_sp + r0 * SB + vsoff;
-    Words<KW> kf[2][NK];
-    uint32_t ks[2][NK];
+    const auto off = [](uint32_t x) __attribute__((always_inline)) {
+      if constexpr (!SMALL) asm volatile("" : "+v"(x));
+      return x;
+    };
+    const uint32_t ko = off(koff), kso = off(ksoff), vo = off(voff), vso = off(vsoff);
+    const auto get = [&](bytes_t kr, bytes_t vr, bytes_t ksr, bytes_t vsr) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        const bytes_t r = row(kr + 4 * i * c.k_sr);
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        kf[i][j] = *reinterpret_cast<const Words<KW>*>(__builtin_assume_aligned(kr + 4 * i * c.k_sr + j * 64, 4 * KW));
-        ks[i][j] = ksr[4 * i * SB + 4 * j];
+        for (int j = 0; j < NK; ++j) x.k[i][j] = kPast ? read_once<typename Tile::Row>(r + ko + j * 64) : read_as<typename Tile::Row>(r + ko + j * 64);
       }
-    uint32_t vf[NH][8], vs[2 * SB];
+      ksr = row(ksr);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        if constexpr (VE == 4)
-          vf[h][i] = *reinterpret_cast<const uint16_t*>(vr + i * c.v_sr);
-        else
-          vf[h][i] = *reinterpret_cast<const uint32_t*>(vr + i * c.v_sr + h * 64);
+        for (int j = 0; j < NK; ++j) x.ks[i][j] = read_as<uint8_t>(ksr + kso + 4 * i * SB + 4 * j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bytes_t r = row(vr + i * c.v_sr);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          if constexpr (VE == 4)
+            x.v[h][i] = read_as<uint16_t>(r + vo);
+          else
+            x.v[h][i] = read_as<uint32_t>(r + vo + h * 64);
+        }
       }
+      vsr = row(vsr);
 #pragma unroll
-    for (int i = 0; i < SB / 2; ++i) {
-      const uint4 w = *reinterpret_cast<const uint4*>(vsr + 16 * i);
-      vs[4 * i] = w.x;
-      vs[4 * i + 1] = w.y;
-      vs[4 * i + 2] = w.z;
-      vs[4 * i + 3] = w.w;
+      for (int i = 0; i < SB / 2; ++i) {
+        const u32x4_t q = read_as<u32x4_t>(vsr + vso + 16 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.vs[4 * i + j] = q[j];
+      }
+    };
+    if constexpr (!SMALL) {
+      const int64_t page = max(w.page0, 0);
+      get(kbase + page * c.k_sp + w.r0 * c.k_sr, vbase + page * c.v_sp + w.r0 * c.v_sr, ksbase + page * z.k_sp + w.r0 * SB,
+          vsbase + page * z.v_sp + w.r0 * SB);
+    } else {
+      const int64_t kp = max(krow >= 16 ? w.page1 : w.page0, 0), vp = max(vrow >= 16 ? w.page1 : w.page0, 0);
+      get(kbase + kp * c.k_sp, vbase + vp * c.v_sp, ksbase + kp * z.k_sp, vsbase + vp * z.v_sp);
     }
-    __builtin_amdgcn_sched_barrier(0);  // all loads are under way before the first is waited for
+  };
 
+  const auto compute = [&](int t, const Where& w, Tile& y) __attribute__((always_inline)) {
+    // keys outside [low, end) and of no page are not seen: most tiles have none
+    const bool whole = w.page0 >= 0 && w.page1 >= 0 && w.pos0 >= low && w.pos0 + 16 <= end && w.pos1 >= low && w.pos1 + 16 <= end;
+    int from = 0, to = 8;  // of the lane's eight keys
+    if (!whole) {
+      const bool back = vrow >= 16;
+      const int page = back ? w.page1 : w.page0, pos = (back ? w.pos1 : w.pos0) + (vrow & 15);
+      from = page < 0 ? 8 : low - pos;  // (positions and lengths are at least 0: no overflow)
+      to = end - pos;
+      // a row of V that is not seen may hold anything, and 0 times NaN is NaN
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool see = i >= from && i < to;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) y.v[h][i] = see ? y.v[h][i] : 0u;
+        if constexpr (D == 64) {
+          y.vs[i / 2] &= see ? ~0u : i % 2 ? 0xffffu : 0xffff0000u;
+        } else {
+#pragma unroll
+          for (int h = 0; h < NH; ++h) y.vs[NH * i + h] = see ? y.vs[NH * i + h] : 0u;
+        }
+      }
+    }
     // scores
     f32x4_t sc[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 2; ++i) sc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint32_t w = kf[i][j / KW].w[j % KW];
-        const float f = scale_of(ks[i][j / KW]);
-        const uint4 kk = make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)),
-                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)),
-                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)),
-                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3)));
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t x = y.k[i][j / KW][j % KW];
+        const float f = scale_of(y.ks[i][j / KW]);
+        const uint4 kk = make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 0)),
+                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 1)),
+                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 2)),
+                                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(x, f, 3)));
 #pragma unroll
         for (int k = 0; k < NQ; ++k) sc[i] = mfma16(kk, qf[k][j], sc[i]);
       }
-    }
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * to_log2;
-    // the lane's first key; keys outside [low, end) and of no page are not seen
-    const int lbl = small && vrow >= 16 ? __builtin_amdgcn_readlane(lb1, u) : __builtin_amdgcn_readlane(lb0, u);
-    const int64_t pos = static_cast<int64_t>(lbl) * c.bs + r0 + vrow_in;
-    const int from = vp < 0 ? 8 : static_cast<int>(min(max(low - pos, static_cast<int64_t>(0)), static_cast<int64_t>(8)));
-    const int to = static_cast<int>(min(max(end - pos, static_cast<int64_t>(0)), static_cast<int64_t>(8)));
-    const bool cut = __any(from > 0 || to < 8);
-    float top = -INFINITY;
+    for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3];
+    if (!whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool see = !cut || (i >= from && i < to);
-      x[i] = see ? x[i] : -INFINITY;
-      top = fmaxf(top, x[i]);
+      for (int i = 0; i < 8; ++i) x[i] = i >= from && i < to ? x[i] : -INFINITY;
     }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * c_log2;
     if (__any(top > m + 8.f)) {
       top = over_rows(top, max_f32);
       const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= f;
 #pragma unroll
-      for (int i = 0; i < NH * VE; ++i) acc[i] *= f;
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int i = 0; i < NH * NP2; ++i) acc[n][i] *= f;
       m = mn;
       ref = m == -INFINITY ? 0.f : m;
     }
     float lt = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+      x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c_log2, -ref));
       lt += x[i];
     }
     l += lt;
     if (s.tile_lse) {
-      lt = small ? over_rows2(lt, add_f32) : over_rows(lt, add_f32);
-      put_sum(ref + __builtin_amdgcn_logf(lt));
+      lt = SMALL ? over_rows2(lt, add_f32) : over_rows(lt, add_f32);
+      put_sum(t, ref + __builtin_amdgcn_logf(lt));
     }
-    // the probabilities as a sum of bf16 values each
-    uint4 pf[NP];
+    // four rows of V at a time: the probabilities as a sum of bf16 values each (the upper
+    // half of what is left of them), and their products with the rows' features, in pairs
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      uint32_t w[4];
+    for (int r = 0; r < 8; r += 4) {
+      uint32_t pw[NC][NP][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = round2<SCOPE_BF16>(x[2 * i], x[2 * i + 1]);
-        x[2 * i] -= low_half<SCOPE_BF16>(w[i]);
-        x[2 * i + 1] -= high_half<SCOPE_BF16>(w[i]);
-      }
-      pf[k] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+      for (int k = 0; k < NP; ++k)
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      uint32_t v[8][VE / 2];  // the eight rows as bf16 pairs of neighbouring features
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t bits = __float_as_uint(x[r + i]), hi = bits & 0xffff0000u;
+          if constexpr (WIDE) {
+            pw[0][k][i] = bits >> 16;
+            pw[1][k][i] = hi;
+          } else {
+            pw[0][k][i] = __builtin_amdgcn_perm(bits, 0u, half);
+          }
+          x[r + i] -= __uint_as_float(hi);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t w = vf[h][i], sw = D == 64 ? vs[i / 2] >> (16 * (i % 2)) : D == 128 ? vs[i] : vs[2 * i + h];
-        // (a row that is not seen may hold anything, and 0 times NaN is NaN)
-        const bool see = !cut || (i >= from && i < to);
-        w = see ? w : 0u;
-        sw = see ? sw : 0u;
-        const float f = __uint_as_float(__builtin_amdgcn_alignbit(sw, sw, vturn));
-        v[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0));
-        v[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1));
-        if constexpr (VE == 8) {
-          v[i][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2));
-          v[i][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3));
+      for (int h = 0; h < NH; ++h) {
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t sw = D == 64 ? y.vs[(r + i) / 2] >> (16 * (i % 2)) : y.vs[NH * (r + i) + h];
+          f[i] = __uint_as_float(__builtin_amdgcn_alignbit(sw, sw, vturn));
+        }
+        const auto pair = [&](auto at) __attribute__((always_inline)) {  // pair `at` of the features
+          constexpr int e = decltype(at)::value;
+          uint32_t o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            o[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(y.v[h][r + i], f[i], e));
+          const uint4 vt = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+          for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int k = 0; k < NP; ++k)
+              acc[n][h * NP2 + e] = mfma16(vt, make_uint4(pw[n][k][0], pw[n][k][1], pw[n][k][2], pw[n][k][3]), acc[n][h * NP2 + e]);
+        };
+        pair(std::integral_constant<int, 0>{});
+        pair(std::integral_constant<int, 1>{});
+        if constexpr (NP2 == 4) {
+          pair(std::integral_constant<int, 2>{});
+          pair(std::integral_constant<int, 3>{});
         }
       }
-#pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        uint32_t op[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          op[w] = j % 2 ? pack_hi16(v[2 * w][j / 2], v[2 * w + 1][j / 2]) : pack_lo16(v[2 * w][j / 2], v[2 * w + 1][j / 2]);
-        const uint4 vt = make_uint4(op[0], op[1], op[2], op[3]);
-#pragma unroll
-        for (int k = 0; k < NP; ++k) acc[h * VE + j] = mfma16(vt, pf[k], acc[h * VE + j]);
-      }
     }
+  };
+
+  resolve(p.t0 + wave + lane * kAttnWaves);
+  if (lists) p.t1 = min(p.t1, same(static_cast<int>((static_cast<int64_t>(n_list) * c.bs + kTileKeys - 1) / kTileKeys)));
+  // Two tiles in turn: one's loads are under way while the other is worked on.  (Behind the
+  // last one it is loaded once more: loads on one side of a branch would be waited for at
+  // its end with all that are under way.)
+  seek();
+  if (t < p.t1) {
+    Tile x, y;
+    Where wx = where(t), wy;
+    int tx = t, ty;
+    bool last = true;  // x is still to be worked on behind the loop
+    load(wx, x);
+    t += kAttnWaves;
+    ++u;
+    seek();
+    while (t < p.t1) {
+      wy = where(t);
+      ty = t;
+      load(wy, y);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(tx, wx, x);
+      t += kAttnWaves;
+      ++u;
+      seek();
+      wx = wy;
+      if (t < p.t1) wx = where(t);
+      tx = t;
+      load(wx, x);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(ty, wy, y);
+      if (tx >= p.t1) {
+        last = false;
+        break;
+      }
+      t += kAttnWaves;
+      ++u;
+      seek();
+    }
+    if (last) compute(tx, wx, x);
   }
-  PagedAttnArgs plain = a;
-  plain.v_scale = nullptr;  // (the outputs have no factor of their own)
-  end_piece<TYPE, D, VE, NH>(plain, s, p, hk, h0, nq, m, ref, l, acc, lds);
+
+  l = over_rows(l, add_f32);
+  const Shares sh = shares_of(lds);
+  if (g4 == 0) {
+    sh.sm[wave * 16 + c16] = m == -INFINITY ? m : ref;
+    sh.sl[wave * 16 + c16] = l;
+  }
+  if (col < nq) {
+    float* o = sh.so + (wave * nq + col) * D + g4 * 4 * VE + (WIDE ? 0 : c16 >> 3);
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < NP2; ++j) o[h * 128 + r * VE + 2 * j + n] = acc[n][h * NP2 + j][r];
+  }
+  __syncthreads();
+  join_shares<TYPE, D>(a, s, p, h0, nq, 1.f, sh);
 }
 
 namespace {
@@ -487,6 +648,8 @@ int check_scales(const scope_paged_cache* c, const scope_paged_scales* z, const 
   SCOPE_REQUIRE(z->k_sp % 16 == 0 && z->k_sh % 16 == 0 && z->v_sp % 16 == 0 && z->v_sh % 16 == 0 && aligned16(k_scale) &&
                     aligned16(v_scale),
                 "%s: the scales of a page's head must be 16-byte aligned", fn);
+  constexpr int64_t kMost = 1 << 26;  // (the attention's lanes count 32 rows in 32 bits)
+  SCOPE_REQUIRE(c->k_sr >= 0 && c->k_sr < kMost && c->v_sr >= 0 && c->v_sr < kMost, "%s: the pages' rows must be less than 2^26 bytes apart", fn);
   return SCOPE_OK;
 }
 
@@ -598,14 +761,20 @@ int scope_paged_decode_attn_fp4(const scope_paged_cache* c, const scope_paged_sc
   const size_t lds = sizeof(float) * kAttnWaves * (32 + static_cast<size_t>(std::min(G, 16)) * c->D);
   hipStream_t st = as_stream(stream);
   const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kAttnThreads), lds, st, bytes, *z, a, s); };
-  if (c->type == SCOPE_BF16)
-    c->D == 64    ? launch(paged_attn4_kernel<SCOPE_BF16, 64>)
-    : c->D == 128 ? launch(paged_attn4_kernel<SCOPE_BF16, 128>)
-                  : launch(paged_attn4_kernel<SCOPE_BF16, 256>);
-  else
-    c->D == 64    ? launch(paged_attn4_kernel<SCOPE_FP16, 64>)
-    : c->D == 128 ? launch(paged_attn4_kernel<SCOPE_FP16, 128>)
-                  : launch(paged_attn4_kernel<SCOPE_FP16, 256>);
+  const auto of_sizes = [&](auto type, auto wide, auto small) {
+    constexpr int T = decltype(type)::value;
+    constexpr bool W = decltype(wide)::value, S = decltype(small)::value;
+    if (c->D == 64)
+      launch(paged_attn4_kernel<T, 64, W, S>);
+    else if (c->D == 128)
+      launch(paged_attn4_kernel<T, 128, W, S>);
+    else
+      launch(paged_attn4_kernel<T, 256, W, S>);
+  };
+  using std::false_type, std::true_type;
+  const auto of_width = [&](auto type, auto small) { G > 8 ? of_sizes(type, true_type{}, small) : of_sizes(type, false_type{}, small); };
+  const auto of_type = [&](auto type) { c->bs == 16 ? of_width(type, true_type{}) : of_width(type, false_type{}); };
+  c->type == SCOPE_BF16 ? of_type(std::integral_constant<int, SCOPE_BF16>{}) : of_type(std::integral_constant<int, SCOPE_FP16>{});
   if (int rc = check_launch("paged_attn4_kernel")) return rc;
   a.v_scale = nullptr;
   return launch_paged_finish(bytes, a, s, st);

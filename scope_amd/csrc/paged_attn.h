@@ -104,34 +104,40 @@ struct AttnSplit {
   float* tile_lse;     // [B][Hq][tiles_cap][halves] log2 of each tile's (half tile's) sum, for the mass
 };
 
-// piece i of n of sequence b: its tiles, and the sequence's first slot
+// piece i of n of sequence b: its tiles, and the sequence's first slot; the sequence's
+// length and first position, as they were given
 struct Piece {
-  int b, t0, t1, i, n, slot;
+  int b, t0, t1, i, n, slot, len, first;
 };
 
 // The piece of this workgroup, found by every wavefront for itself: the batch's
 // tiles are summed, then the sequences' numbers of pieces.  false: there is none.
-__device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const PagedAttnArgs& a, const AttnSplit& s, int x,
-                                           int turn, Piece& p) {
+// wanted(tiles of the batch): how many pieces they are cut into, about.
+template <class Wanted>
+__device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const PagedAttnArgs& a, int x, int turn, Wanted wanted,
+                                           Piece& p) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = static_cast<int64_t>(c.MP) * c.bs;
-  const auto tiles_of = [&](int b, int* lo) {
-    *lo = 0;
-    return b < c.B ? seq_tiles(a.lens[b], a.first ? a.first[b] : 0, cap, lo) : 0;
+  const auto tiles_of = [&](int b, int* lo, int* len, int* first) {
+    *lo = *len = *first = 0;
+    if (b >= c.B) return 0;
+    *len = a.lens[b];
+    if (a.first) *first = a.first[b];
+    return seq_tiles(*len, *first, cap, lo);
   };
-  int lo0;
-  const int tiles0 = tiles_of(lane, &lo0);
+  int lo0, len0, first0;
+  const int tiles0 = tiles_of(lane, &lo0, &len0, &first0);
   // (64 sequences of less than 2^26 tiles: their sum fits 32 bits)
   int64_t total = static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles0), 63));
   for (int b0 = 64; b0 < c.B; b0 += 64) {
-    int lo;
-    total += static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles_of(b0 + lane, &lo)), 63));
+    int lo, len, first;
+    total += static_cast<uint32_t>(__builtin_amdgcn_readlane(prefix_of(tiles_of(b0 + lane, &lo, &len, &first)), 63));
   }
-  const int64_t piece = piece_tiles(total, s.pieces, kPieceTiles, turn);
+  const int64_t piece = piece_tiles(total, wanted(total), kPieceTiles, turn);
   int before = 0;
   for (int b0 = 0; b0 < c.B; b0 += 64) {
-    int lo = lo0;
-    const int tiles = b0 ? tiles_of(b0 + lane, &lo) : tiles0;
+    int lo = lo0, len = len0, first = first0;
+    const int tiles = b0 ? tiles_of(b0 + lane, &lo, &len, &first) : tiles0;
     const int n = b0 + lane < c.B ? seq_pieces(tiles, piece) : 0;
     const int upto = prefix_of(n);
     const uint64_t hit = __ballot(x < before + upto);
@@ -141,6 +147,8 @@ __device__ __forceinline__ bool find_piece(const scope_paged_cache& c, const Pag
       p.n = __builtin_amdgcn_readlane(n, at);
       p.slot = before + __builtin_amdgcn_readlane(upto, at) - p.n;
       p.i = x - p.slot;
+      p.len = __builtin_amdgcn_readlane(len, at);
+      p.first = __builtin_amdgcn_readlane(first, at);
       piece_range(__builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(tiles, at), p.n, p.i, &p.t0, &p.t1);
       return true;
     }
@@ -202,48 +210,30 @@ __device__ __forceinline__ Words<N> load_once(const char* p) {
   return x;
 }
 
-// The end of a piece: the wavefronts' maxima m (what the sums are relative to: ref),
-// sums l and outputs acc (lane l: query l % 16, feature 128 h + VE (4 (l / 16) + r) + j
-// in acc[h·VE + j][r]) are joined over LDS and written, to the result where the piece is
-// a sequence's only one.
-template <int TYPE, int D, int VE, int NH>
-__device__ __forceinline__ void end_piece(const PagedAttnArgs& a, const AttnSplit& s, const Piece& p, int hk, int h0, int nq,
-                                          float m, float ref, float l, const f32x4_t (&acc)[NH * VE], float* lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g4 = lane >> 4, c16 = lane & 15, b = p.b;
-  // the wavefronts' shares: maxima and sums, then the outputs of the group's queries
-  l = over_rows(l, add_f32);
-  float* sm = lds;                       // [waves][16]
-  float* sl = lds + kAttnWaves * 16;     // [waves][16]
-  float* so = lds + kAttnWaves * 32;     // [waves][nq][D]
-  if (g4 == 0) {
-    sm[wave * 16 + c16] = m == -INFINITY ? m : ref;
-    sl[wave * 16 + c16] = l;
-  }
-  if (c16 < nq) {
-    float* o = so + (wave * nq + c16) * D + g4 * 4 * VE;
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < VE; j += 4)
-          *reinterpret_cast<float4*>(o + h * 128 + r * VE + j) = make_float4(
-              acc[h * VE + j][r], acc[h * VE + j + 1][r], acc[h * VE + j + 2][r], acc[h * VE + j + 3][r]);
-  }
-  __syncthreads();
-  const float vs = a.v_scale ? a.v_scale[hk] : 1.f;
+// The end of a piece: the wavefronts' maxima and sums (relative to those) in sm, sl
+// [waves][16] and their outputs in so [waves][nq][D], in LDS, are joined and written, to
+// the result where the piece is a sequence's only one.  vs: a factor on the outputs.
+struct Shares {
+  float *sm, *sl, *so;
+};
+__device__ __forceinline__ Shares shares_of(float* lds) { return {lds, lds + kAttnWaves * 16, lds + kAttnWaves * 32}; }
+
+template <int TYPE, int D>
+__device__ __forceinline__ void join_shares(const PagedAttnArgs& a, const AttnSplit& s, const Piece& p, int h0, int nq, float vs,
+                                            const Shares& z) {
+  const int b = p.b;
   for (int i = threadIdx.x; i < nq * D; i += kAttnThreads) {
     const int q = i / D, d = i % D, h = h0 + q;
-    float M = sm[q];
+    float M = z.sm[q];
 #pragma unroll
-    for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, sm[w * 16 + q]);
+    for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, z.sm[w * 16 + q]);
     float L = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < kAttnWaves; ++w) {
       // (a sum of 0 is a share without keys; a NaN stays one, whatever its maximum)
-      const float f = sl[w * 16 + q] == 0.f ? 0.f : __builtin_amdgcn_exp2f(sm[w * 16 + q] - M);
-      L += f * sl[w * 16 + q];
-      o += f * so[(w * nq + q) * D + d];
+      const float f = z.sl[w * 16 + q] == 0.f ? 0.f : __builtin_amdgcn_exp2f(z.sm[w * 16 + q] - M);
+      L += f * z.sl[w * 16 + q];
+      o += f * z.so[(w * nq + q) * D + d];
     }
     if (p.n == 1) {
       const float y = L == 0.f ? 0.f : o / L * vs;
@@ -254,7 +244,7 @@ __device__ __forceinline__ void end_piece(const PagedAttnArgs& a, const AttnSpli
         if (s.lse2) s.lse2[static_cast<int64_t>(b) * a.Hq + h] = e;
       }
     } else {
-      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.Hq + h;
+      const int64_t at = static_cast<int64_t>(p.slot + p.i) * a.Hq + h;
       s.po[at * D + d] = o;
       if (d == 0) {
         s.pml[2 * at] = M;

@@ -40,6 +40,9 @@ constexpr int kMostPieces = 1536;
 SCOPE_HD int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
 SCOPE_HD int piece_turn(int D) { return D == 256 ? kAttnWaves : 1; }
 
+// Workgroups aimed at over 4-bit pages, by the batch's tiles over all key heads.
+SCOPE_HD int pieces_wanted4(int64_t tiles) { return tiles < 25000 ? 512 : tiles < 100000 ? 1024 : kMostPieces; }
+
 // positions that a sequence of `len` holds in a table row of `cap`
 SCOPE_HD int64_t seq_end(int64_t len, int64_t cap) { return len < 0 ? 0 : len < cap ? len : cap; }
 
