@@ -218,8 +218,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(scope_paged_cache c, sc
       xv = read8<KIND, TYPE>(a.v_pages, page * c.v_sp + h * c.v_sh + slot * c.v_sr + dd, sv);
     }
     const int64_t to = (i0 + r) * c.Hkv * c.D + e * 8;
-    *reinterpret_cast<uint4*>(a.k + to) = xk;
-    *reinterpret_cast<uint4*>(a.v + to) = xv;
+    store_past(a.k + to, xk);
+    store_past(a.v + to, xv);
   });
 }
 
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kAttnThreads, attn4_waves(D, TYPE, WIDE, SMALL)) vo
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
   } else if (!find_piece(c, a, slot, piece_turn(D),
-                         [&](int64_t total) { return min(s.pieces, (pieces_wanted4(total * cols) + cols - 1) / cols); }, p)) {
+                         [&](int64_t total) { return min(s.pieces, pieces_wanted4(total, cols, c.B, 256 * attn4_waves(D, TYPE, WIDE, SMALL))); }, p)) {
     return;
   }
   p.b = same(p.b);

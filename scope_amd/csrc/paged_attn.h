@@ -69,6 +69,9 @@ __device__ __forceinline__ uint4 load_past(const uint4* p) {
 __device__ __forceinline__ void store_past(uint8_t* p, uint2 x) {
   __builtin_nontemporal_store(__builtin_bit_cast(u32x2_t, x), reinterpret_cast<u32x2_t*>(p));
 }
+__device__ __forceinline__ void store_past(uint16_t* p, uint4 x) {
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, x), reinterpret_cast<u32x4_t*>(p));
+}
 
 // ---- attention of one new token -------------------------------------------------
 struct PagedAttnArgs {

@@ -40,8 +40,16 @@ constexpr int kMostPieces = 1536;
 SCOPE_HD int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
 SCOPE_HD int piece_turn(int D) { return D == 256 ? kAttnWaves : 1; }
 
-// Workgroups aimed at over 4-bit pages, by the batch's tiles over all key heads.
-SCOPE_HD int pieces_wanted4(int64_t tiles) { return tiles < 25000 ? 512 : tiles < 100000 ? 1024 : kMostPieces; }
+// Pieces aimed at over 4-bit pages, for a batch of `total` tiles in each of `cols`
+// columns (key head and group of 16 query heads), where the device holds `resident`
+// workgroups at once: they are to start together (a sequence adds one piece at most to
+// those aimed at), and to have some ten tiles each before they are more than 512.
+SCOPE_HD int pieces_wanted4(int64_t total, int cols, int B, int resident) {
+  const int all = resident / cols, less = B > 1 ? all - B : all, one = less > all / 2 ? less : all / 2;
+  const int64_t few = 512 / cols, by_tiles = total / 10, some = few > by_tiles ? few : by_tiles;
+  const int64_t n = some < one ? some : one, most = total / 120, m = n > most ? n : most;
+  return m > 1 ? static_cast<int>(m < kMostPieces ? m : kMostPieces) : 1;
+}
 
 // positions that a sequence of `len` holds in a table row of `cap`
 SCOPE_HD int64_t seq_end(int64_t len, int64_t cap) { return len < 0 ? 0 : len < cap ? len : cap; }

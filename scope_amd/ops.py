@@ -1201,11 +1201,11 @@ def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: 
     P, Hkv, bs, D = shape
     if fp4:
         D *= 2
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if t is None or t.dtype != _E8M0 or t.shape != (P, Hkv, bs, D // 32) or t.stride()[2:] != (D // 32, 1):
-                raise RuntimeError(f"{who}: {name} must be float8_e8m0fnu [{P}, {Hkv}, {bs}, {D // 32}], contiguous in a page's head, "
-                                   "with float4_e2m1fn_x2 pages")
-    else:
+        want = (P, Hkv, bs, D // 32)
+        for t in (k_scale, v_scale):
+            if t is None or t.dtype != _E8M0 or t.shape != want:
+                raise RuntimeError(f"{who}: k_scale and v_scale must be float8_e8m0fnu {list(want)} with float4_e2m1fn_x2 pages")
+    elif k_scale is not None or v_scale is not None:
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
             if t is not None and (not fp8 or t.dtype != torch.float32 or t.numel() != Hkv or not t.is_contiguous()):
                 raise RuntimeError(f"{who}: {name} must be a contiguous float32 [{Hkv}], with float8_e4m3fn pages")
@@ -1221,9 +1221,11 @@ def _paged_cache(who: str, k_pages: torch.Tensor, v_pages: torch.Tensor, table: 
     return _lib.PagedCache(B, Hkv, D, bs, MP, _PAGED_TYPES[dtype], fp8, P, kp, kh, kr, vp, vh, vr)
 
 
-def _paged_scales(c: "_lib.PagedCache", k_scale: torch.Tensor, v_scale: torch.Tensor) -> "_lib.PagedScales":
+def _paged_scales(who: str, c: "_lib.PagedCache", k_scale: torch.Tensor, v_scale: torch.Tensor) -> "_lib.PagedScales":
     """The strides of a 4-bit cache's scales."""
-    (kp, kh, _, _), (vp, vh, _, _) = k_scale.stride(), v_scale.stride()
+    (kp, kh, kr, kd), (vp, vh, vr, vd) = k_scale.stride(), v_scale.stride()
+    if kd != 1 or vd != 1 or not kr == vr == c.D // 32:
+        raise RuntimeError(f"{who}: k_scale and v_scale (float8_e8m0fnu) must be contiguous in a page's head")
     if c.P == 1:
         kp = vp = 0
     if c.Hkv == 1:
@@ -1265,7 +1267,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     args = (N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1], v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1],
             _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(), v_pages.data_ptr())
     if fp4:
-        _launch(dev, "scope_paged_append_fp4", C.byref(c), C.byref(_paged_scales(c, k_scale, v_scale)), *args)
+        _launch(dev, "scope_paged_append_fp4", C.byref(c), C.byref(_paged_scales(who, c, k_scale, v_scale)), *args)
     else:
         _launch(dev, "scope_paged_append", C.byref(c), *args)
 
@@ -1302,8 +1304,9 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     lens = _ints(who, "lens", lens, c.B, dev)
     cu = _ints(who, "cu", cu, c.B + 1, dev)
     first = _ints(who, "first", first, c.B, dev)
-    k, v = (torch.empty((rows, c.Hkv, c.D), dtype=dtype, device=dev) for _ in range(2))
-    scales = C.byref(_paged_scales(c, k_scale, v_scale)) if pt == _FP4 else None
+    k = torch.empty((rows, c.Hkv, c.D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    scales = C.byref(_paged_scales(who, c, k_scale, v_scale)) if pt == _FP4 else None
     _launch(dev, "scope_paged_read", C.byref(c), scales, rows, _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(first), _ptr(k_scale),
             _ptr(v_scale), k_pages.data_ptr(), v_pages.data_ptr(), k.data_ptr(), v.data_ptr())
     return k, v
@@ -1368,7 +1371,7 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
             v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), _ptr(first), _ptr(kv_num),
             _ptr(kv_idx), _ptr(mass), _ptr(work), out.data_ptr(), lse.data_ptr())
     if k_pages.dtype == _FP4:
-        _launch(dev, "scope_paged_decode_attn_fp4", C.byref(c), C.byref(_paged_scales(c, k_scale, v_scale)), *args)
+        _launch(dev, "scope_paged_decode_attn_fp4", C.byref(c), C.byref(_paged_scales(who, c, k_scale, v_scale)), *args)
     else:
         _launch(dev, "scope_paged_decode_attn", C.byref(c), *args)
     return out, lse
