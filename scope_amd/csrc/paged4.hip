@@ -252,7 +252,7 @@ struct Tile4 {  // a lane's share of 32 keys and their scales
 };
 
 constexpr int attn4_waves(int D, int type, bool wide, bool small) {  // wavefronts a SIMD that the registers are cut to
-  return D == 256 ? (wide ? 1 : 2) : D == 64 ? (wide ? 3 : 4) : wide ? 2 : small || type == SCOPE_FP16 ? 3 : 4;
+  return D == 256 ? 2 : D == 64 ? (wide ? 3 : 4) : wide ? 2 : small || type == SCOPE_FP16 ? 3 : 4;
 }
 
 template <int TYPE, int D, bool WIDE, bool SMALL>
@@ -266,6 +266,7 @@ __global__ __launch_bounds__(kAttnThreads, attn4_waves(D, TYPE, WIDE, SMALL)) vo
   constexpr int NP = 3;                           // bf16 values whose sum is a probability
   constexpr int NC = WIDE ? 2 : 1;                // outputs of even and of odd features: in columns of their own, or beside each other
   constexpr bool kPast = !SMALL && D >= 128;      // K passes the caches
+  constexpr bool kAhead = !(WIDE && D == 256);  // the next tile's loads are under way (else registers spill)
   extern __shared__ float lds[];
   // (what is the same for a wavefront is told to the compiler: scalar registers, branches and addresses)
   const auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
@@ -586,7 +587,18 @@ __global__ __launch_bounds__(kAttnThreads, attn4_waves(D, TYPE, WIDE, SMALL)) vo
   // last one it is loaded once more: loads on one side of a branch would be waited for at
   // its end with all that are under way.)
   seek();
-  if (t < p.t1) {
+  if constexpr (!kAhead) {
+    while (t < p.t1) {
+      Tile x;
+      const Where w = where(t);
+      load(w, x);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(t, w, x);
+      t += kAttnWaves;
+      ++u;
+      seek();
+    }
+  } else if (t < p.t1) {
     Tile x, y;
     Where wx = where(t), wy;
     int tx = t, ty;

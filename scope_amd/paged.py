@@ -6,6 +6,7 @@ attention layer.
     cache.append(k, v, rows=[1000, 17, 0, 0, 0, 0, 0, 0])    # prompts, ragged
     cache.append(k, v)                                       # one row a sequence
     out, lse = cache.attend(q, scale=0.12)                   # weights accumulate
+    k, v = cache.read()                                      # every row that is held, for a dense attention
     cache.evict(512, window=4, n_global=1)                   # back to 512 pages a sequence
     cache.release(3)                                         # a sequence ends
 
@@ -17,7 +18,7 @@ given ``rows``: the new table entries and the counts are copied from pageable ho
 memory; a step (no ``rows``) within the pages taken does not.  A cache is used on one
 stream at a time: a page goes from one sequence to another in stream order.
 ``attend`` may be captured into a graph; the calls that also change the host's
-copy, which a replay would not, raise there.
+copy, or go by it (``read``), which a replay would not, raise there.
 """
 from __future__ import annotations
 
@@ -31,12 +32,15 @@ class PagedKVCache:
 
     ``pages`` the pool holds, for ``sequences`` sequences of up to ``max_len``
     positions each.  ``dtype``: bfloat16 or float16, or float8_e4m3fn with
-    ``k_scale`` / ``v_scale`` [kv_heads] fp32 (value = stored · scale; None: 1).
+    ``k_scale`` / ``v_scale`` [kv_heads] fp32 (value = stored · scale; None: 1),
+    or float4_e2m1fn_x2, whose scales (a power of two for 32 features) are formed
+    as rows are written: 68 bytes for a row of 128 features.
 
-    k_pages, v_pages [pages, kv_heads, page_size, head_dim], table [sequences,
-    max pages] int32 (-1: no page), lens [sequences] int32 and mass
-    [sequences, kv_heads, max pages] fp32 live on the device and may be handed
-    to ``ops.paged_*`` directly; they keep their addresses."""
+    k_pages, v_pages [pages, kv_heads, page_size, head_dim] (4 bits: head_dim / 2,
+    with k_scale, v_scale [pages, kv_heads, page_size, head_dim / 32]
+    float8_e8m0fnu), table [sequences, max pages] int32 (-1: no page), lens
+    [sequences] int32 and mass [sequences, kv_heads, max pages] fp32 live on the
+    device and may be handed to ``ops.paged_*`` directly; they keep their addresses."""
 
     def __init__(self, *, pages: int, sequences: int, max_len: int, kv_heads: int, head_dim: int, page_size: int = 128,
                  dtype: torch.dtype = torch.bfloat16, k_scale: torch.Tensor | None = None,
@@ -45,8 +49,18 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: pages={pages}, sequences={sequences} and max_len={max_len} must be at least 1")
         self.page_size, self.max_len = page_size, max_len
         width = -(-max_len // page_size)
-        self.k_pages, self.v_pages = (torch.zeros((pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
-                                      for _ in range(2))
+        if dtype == torch.float4_e2m1fn_x2:
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("PagedKVCache: 4-bit pages form their scales themselves")
+            if head_dim % 32:
+                raise ValueError(f"PagedKVCache: 4-bit pages need a head dim that is a multiple of 32, got {head_dim}")
+            k_scale, v_scale = (torch.zeros((pages, kv_heads, page_size, head_dim // 32), dtype=torch.uint8,
+                                            device=device).view(torch.float8_e8m0fnu) for _ in range(2))
+            self.k_pages, self.v_pages = (torch.zeros((pages, kv_heads, page_size, head_dim // 2), dtype=torch.uint8,
+                                                      device=device).view(dtype) for _ in range(2))
+        else:
+            self.k_pages, self.v_pages = (torch.zeros((pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+                                          for _ in range(2))
         self.k_scale, self.v_scale = k_scale, v_scale
         self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(sequences, dtype=torch.int32, device=device)
@@ -119,6 +133,24 @@ class PagedKVCache:
         return ops.paged_decode_attn(q, self.k_pages, self.v_pages, self.table, self.lens, scale=scale, first=first,
                                      kv_num=kv_num, kv_idx=kv_idx, mass=self.mass if accumulate else None,
                                      k_scale=self.k_scale, v_scale=self.v_scale)
+
+    def read(self, rows=None, first=None, *, dtype: torch.dtype | None = None):
+        """The rows of the ``rows[b]`` positions from first[b] on of each sequence b, one
+        sequence after the other -> k, v [sum(rows), kv_heads, head_dim] of ``dtype``
+        (``ops.paged_read``; 16-bit pages in their own).  ``first`` of None is 0,
+        ``rows`` of None what each sequence holds from there on; positions whose page
+        was evicted are zeros.  The numbers are the host's: nothing waits for the GPU
+        but their copy from pageable memory."""
+        self._on_host("read")
+        B = len(self._len)
+        first = [0] * B if first is None else [int(n) for n in first]
+        rows = [max(0, n - f) for n, f in zip(self._len, first)] if rows is None else [int(n) for n in rows]
+        if len(first) != B or len(rows) != B or any(f < 0 or n < 0 or (n and f + n > held) for f, n, held in zip(first, rows, self._len)):
+            raise ValueError(f"PagedKVCache: rows {rows} from {first} on are not held ({self._len})")
+        at = torch.tensor([first + [0], rows + [0]], dtype=torch.int32).to(self.lens.device)
+        cu = torch.cat((at.new_zeros(1), at[1, :B].cumsum(0, dtype=torch.int32)))
+        return ops.paged_read(self.k_pages, self.v_pages, self.table, self.lens, rows=sum(rows), cu=cu, first=at[0, :B],
+                              k_scale=self.k_scale, v_scale=self.v_scale, dtype=dtype)
 
     def evict(self, budget, *, window: int = 1, n_global: int = 0) -> int:
         """Brings every sequence back to ``budget`` pages (a number or int [sequences])

@@ -378,6 +378,18 @@ def test_attn_is_that_over_the_values(ops):
     assert (lse - wl).abs().max() <= 2.0 ** -15
 
 
+@pytest.mark.parametrize("D,G", [(64, 3), (128, 12), (256, 16)])
+def test_attn_of_an_evicted_cache(ops, D, G):
+    """Most blocks without a page, long runs of them among those that have one: more than a wavefront looks up at once."""
+    bs = 16
+    c = cache4([9000, 20, 5000], Hq=G, Hkv=1, D=D, bs=bs, seed=18)
+    table = c["table"].clone()
+    g = torch.Generator().manual_seed(1)
+    table[torch.rand(table.shape, generator=g) < 0.6] = -1
+    table[0, 20:520] = -1
+    check4(ops, c, DEV, scale=0.12, table=table, mass=torch.zeros((3, 1, table.shape[1])))
+
+
 def test_attn_shared_pages(ops):
     c = cache4([300, 300], Hq=2, Hkv=1, D=64, bs=32, seed=17)
     table = c["table"].clone()
