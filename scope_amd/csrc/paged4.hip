@@ -71,6 +71,10 @@ __device__ __forceinline__ void each_chunk(const MoveArgs& m, int n, int2 places
   }
 }
 
+// Rows written: a quad of lanes has a group of 32 features, so that its largest value
+// takes two steps in registers, and every lane moves 16 bytes in and 4 out.  Bound by
+// memory: 65539 rows of 8 heads of 128 (340 MB) 66 us, 5.1 TB/s, as a large copy (four
+// rows a wavefront instead of two, or none passing the caches, 5 to 20 us more).
 struct Append4Args {
   int64_t k_sn, k_sh, v_sn, v_sh;
   const uint16_t* k;
@@ -145,6 +149,9 @@ __global__ __launch_bounds__(256) void paged_append4_kernel(scope_paged_cache c,
   });
 }
 
+// Rows read: 16 bytes out a lane, past the caches (131072 rows of 4 bits 149 -> 140 us, 4.9
+// TB/s; 12k of e4m3 38.5 -> 26.6; one row a wavefront 142, K and V by workgroups of their
+// own 158).
 struct ReadArgs {
   const int32_t* lens;
   const int32_t* first;
@@ -224,19 +231,17 @@ __global__ __launch_bounds__(256) void paged_read_kernel(scope_paged_cache c, sc
 }
 
 // ---- attention of one new token -------------------------------------------------
-// As over 16-bit pages (paged.hip: the tiles, the masks, the split), with K and V
-// widened to bf16, which holds every code and scale exactly; a q in fp16 is the sum of
-// two bf16 values, exactly.
 typedef const __attribute__((address_space(1))) char* bytes_t;  // in device memory
 template <class T>
 __device__ __forceinline__ T read_as(bytes_t p) {
   return *(const __attribute__((address_space(1))) T*)p;  // (an address-space cast needs a C-style cast)
 }
-
+// past the caches
 template <class T>
 __device__ __forceinline__ T read_once(bytes_t p) {
   return __builtin_nontemporal_load((const __attribute__((address_space(1))) T*)p);
 }
+
 template <int D>
 struct Tile4 {  // a lane's share of 32 keys and their scales
   static constexpr int VE = D / 16 < 8 ? D / 16 : 8;  // features in a row of V
@@ -251,22 +256,55 @@ struct Tile4 {  // a lane's share of 32 keys and their scales
   uint32_t vs[2 * SB];
 };
 
-constexpr int attn4_waves(int D, int type, bool wide, bool small) {  // wavefronts a SIMD that the registers are cut to
-  return D == 256 ? 2 : D == 64 ? (wide ? 3 : 4) : wide ? 2 : small || type == SCOPE_FP16 ? 3 : 4;
+// The tiles, the split, the running maximum and the join are those of the attention over
+// 16-bit pages (paged.hip); what differs:
+//   S^T = K·Q^T   K's codes become bf16 with their scale, two in one instruction, which is
+//                 exact, and are operand A; a q in fp16 is the sum of two bf16 values.
+//   O^T = V^T·P^T a conversion gives a position's two neighbouring features in one word,
+//                 the operand wants two positions of one feature there.  Instead of
+//                 transposing (32 v_perm a tile), a product runs over 16 positions with
+//                 both features as its depth, operand B holding the probability in the
+//                 half of the one and 0 in that of the other: columns 0 .. 7 the even
+//                 features' outputs of the group's heads, 8 .. 15 the odd ones'.  Groups
+//                 of more than 8 heads (WIDE) take two products.  WIDE for 8 heads too: 16
+//                 sequences to 32k at D = 128 43 -> 50 us, at D = 256 74 -> 82.
+//                 A probability is the sum of three bf16 values, the upper halves of what
+//                 is left of it: all of its 24 bits, so that the product is fp32's.
+// Bound by memory while a wavefront has tiles enough: 24 sequences of 9k to 65k with 64
+// query heads (928 MB) 6.2 TB/s with the launch behind it.  Below that the start counts
+// (four dependent loads from the lengths to the first row, some 5 us) and the second launch
+// (6 us): 131k positions with weights (143 MB) 33.4 us, of which the kernel 29.5; at D = 64
+// the vector units are busy 64% of the time (48 windows of 4096, 69 MB: 26 us).
+// The next tile's loads are under way while one is worked on: a tile has a quarter of the
+// bytes of 16-bit rows and as many instructions (131k positions 46.6 -> 32.8 us).  Two
+// tiles ahead 31.4 us for 30.3 at D = 64, spilling elsewhere.  WIDE at D = 256 has no
+// registers for it: with one wavefront a SIMD 138 us (16 sequences to 32k), with two that
+// load as they go 94.
+// K passes the caches where its rows are long enough (24 sequences 176 -> 164 us, 131k
+// positions 40.4 -> 35.1, V alone 173 and 35.1, both 167 and 38.4; pages of 16 30.3 ->
+// 31.4, D = 64 32.0 -> 32.8).
+// K's codes as they are in the scaled product of 4-bit and 8-bit operands, q in e4m3
+// parts, saves 32 conversions a tile and changed nothing there; forming the parts took
+// 1.2 us (nine blocks a head 5.4 -> 6.6, 48 windows 27.2 -> 30.4).
+constexpr int attn4_waves(int D, bool wide) {  // wavefronts a SIMD that the registers are cut to
+  // (D = 64: with 3 windows 30.4 -> 31.8 us, 8 sequences to 60k 56 -> 61; WIDE at D = 128
+  // with 3 29.0 -> 30.5 and fp16 spills)
+  return D == 256 || (wide && D == 128) ? 2 : D == 64 && !wide ? 4 : 3;
 }
 
+// SMALL: pages of 16 positions, two a tile (other pages' addresses are scalars).
 template <int TYPE, int D, bool WIDE, bool SMALL>
-__global__ __launch_bounds__(kAttnThreads, attn4_waves(D, TYPE, WIDE, SMALL)) void paged_attn4_kernel(scope_paged_cache c, scope_paged_scales z,
-                                                                                      PagedAttnArgs a, AttnSplit s) {
+__global__ __launch_bounds__(kAttnThreads, attn4_waves(D, WIDE)) void paged_attn4_kernel(scope_paged_cache c, scope_paged_scales z,
+                                                                                         PagedAttnArgs a, AttnSplit s) {
   using Tile = Tile4<D>;
   constexpr int VE = Tile::VE, NH = Tile::NH, KW = Tile::KW, NK = Tile::NK, SB = Tile::SB;
   constexpr int NP2 = VE / 2;                     // pairs of features of a lane in a row of V
   constexpr int NJ = D / 32;                      // products over D
   constexpr int NQ = TYPE == SCOPE_FP16 ? 2 : 1;  // bf16 values whose sum is one of q
   constexpr int NP = 3;                           // bf16 values whose sum is a probability
-  constexpr int NC = WIDE ? 2 : 1;                // outputs of even and of odd features: in columns of their own, or beside each other
+  constexpr int NC = WIDE ? 2 : 1;                // products for even and odd features
   constexpr bool kPast = !SMALL && D >= 128;      // K passes the caches
-  constexpr bool kAhead = !(WIDE && D == 256);  // the next tile's loads are under way (else registers spill)
+  constexpr bool kAhead = !(WIDE && D == 256);    // the next tile's loads are under way
   extern __shared__ float lds[];
   // (what is the same for a wavefront is told to the compiler: scalar registers, branches and addresses)
   const auto same = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
@@ -292,9 +330,9 @@ __global__ __launch_bounds__(kAttnThreads, attn4_waves(D, TYPE, WIDE, SMALL)) vo
     p.first = a.first ? a.first[p.b] : 0;
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
-  } else if (!find_piece(c, a, slot, piece_turn(D),
-                         [&](int64_t total) { return min(s.pieces, pieces_wanted4(total, cols, c.B, 256 * attn4_waves(D, TYPE, WIDE, SMALL))); }, p)) {
-    return;
+  } else {
+    const auto wanted = [&](int64_t total) { return min(s.pieces, pieces_wanted4(total, cols, c.B, 256 * attn4_waves(D, WIDE))); };
+    if (!find_piece(c, a, slot, piece_turn(D), wanted, p)) return;
   }
   p.b = same(p.b);
   p.i = same(p.i);
@@ -426,7 +464,8 @@ __global__ __launch_bounds__(kAttnThreads, attn4_waves(D, TYPE, WIDE, SMALL)) vo
       for (int i = 0; i < 2; ++i) {
         const bytes_t r = row(kr + 4 * i * c.k_sr);
 #pragma unroll
-        for (int j = 0; j < NK; ++j) x.k[i][j] = kPast ? read_once<typename Tile::Row>(r + ko + j * 64) : read_as<typename Tile::Row>(r + ko + j * 64);
+        for (int j = 0; j < NK; ++j)
+          x.k[i][j] = kPast ? read_once<typename Tile::Row>(r + ko + j * 64) : read_as<typename Tile::Row>(r + ko + j * 64);
       }
       ksr = row(ksr);
 #pragma unroll
