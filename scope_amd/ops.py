@@ -1243,8 +1243,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     float8_e4m3fn holding x / scale[h] cut to ±448 (k_scale, v_scale [Hkv]
     fp32), or float4_e2m1fn_x2 [P, Hkv, bs, D / 2] with k_scale, v_scale [P,
     Hkv, bs, D / 32] float8_e8m0fnu, which are written too: a power of two for
-    each 32 features, at least a seventh of the largest (a group with an
-    infinity or a NaN becomes NaN); table [B, MP] int32 page ids; lens [B] the positions each sequence
+    each 32 features, so that the largest is at most 7 of it (cut to 6) and over
+    3.5 (a group with an infinity or a NaN becomes NaN); table [B, MP] int32 page ids; lens [B] the positions each sequence
     holds before the call (it is not changed).  Row i goes to sequence b with
     cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing; without it N <= B
     and row i to sequence i), position lens[b] + i - cu[b].  Rows of no
@@ -1273,7 +1273,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
 
 
 def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *, rows: int,
-               cu: torch.Tensor | None = None, first: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+               cu: torch.Tensor | None = None, first=None, k_scale: torch.Tensor | None = None,
                v_scale: torch.Tensor | None = None, dtype: torch.dtype | None = None):
     """Rows of a paged cache one after the other -> k, v [rows, Hkv, D] of
     ``dtype``: what a dense attention of a prompt's next tokens takes, or
@@ -1282,7 +1282,7 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     The cache as ``paged_append`` fills it, pages of any type.  Row i is that of
     sequence b with cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing;
     without it rows <= B and row i is of sequence i), position first[b] + i -
-    cu[b] (first [B], without it 0; without cu first[b]).  Rows of no sequence,
+    cu[b] (first [B] or one number, without it 0; without cu first[b]).  Rows of no sequence,
     outside [0, lens[b]), past the table, or of a block whose entry is outside
     [0, P) are zeros.  ``dtype``: bfloat16 or float16; 16-bit pages are read in
     their own type (the default then), others in bfloat16 by default.  4-bit
@@ -1293,7 +1293,7 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad):
         return _NoGradient.apply(who, functools.partial(paged_read, k_pages, v_pages, table, lens, rows=rows, cu=cu, first=first,
                                                         k_scale=k_scale, v_scale=v_scale, dtype=dtype), k_pages, v_pages)
-    dev = _device(who, k_pages, v_pages, table, lens, cu, first, k_scale, v_scale)
+    dev = _device(who, k_pages, v_pages, table, lens, cu, first if isinstance(first, torch.Tensor) else None, k_scale, v_scale)
     pt = k_pages.dtype
     if dtype is None:
         dtype = torch.bfloat16 if pt == _FP8 or pt == _FP4 else pt
@@ -1329,7 +1329,9 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     the table are skipped).  A row that sees nothing gives 0 and lse -inf; an
     infinite value of v in a seen row gives that infinity (or NaN, where the
     row's weight is below 2^-15 in fp16, 2^-100 in bf16, of the largest among
-    the 32 positions around it).
+    the 32 positions around it).  4-bit pages (their rows less than 2^26 bytes
+    apart) hold no infinities: a group without a number in a seen row of v makes
+    its features NaN, one of k the whole output.
     ``mass`` [B, Hkv, MP] fp32 contiguous gets each block's probabilities,
     summed over its positions and the group's query heads, added in place
     (lists without repeats then; not two calls on one mass at a time).  Its

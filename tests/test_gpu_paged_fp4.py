@@ -171,6 +171,55 @@ def test_read_of_every_byte_and_scale(ops, dtype):
         assert torch.equal(torch.isnan(x.cpu()), torch.isnan(want)) and torch.equal(x.cpu().nan_to_num(7.0), want.nan_to_num(7.0))
 
 
+def test_read_from_one_number_on(ops):
+    c = cache([40, 3, 25], Hq=2, Hkv=1, D=64, bs=16, seed=2)
+    d = on_gpu(c)
+    for first in (0, 2, 24, -5, 10 ** 12):
+        k, _ = ops.paged_read(*(d[k] for k in TENSORS[1:]), rows=3, first=first)
+        assert torch.equal(k.cpu(), OP.read(c["k_pages"], c["table"], c["lens"], 3, None, [first] * 3))
+
+
+def test_rows_past_the_largest_grid_of_two_a_wavefront(ops):
+    """2^27 + 3 rows (one row's memory, expanded) written, of which a few blocks have a page; and their ends read."""
+    N, bs, held = 2 ** 27 + 3, 256, 5
+    MP = -(-(N + held) // bs)
+    print(f"append of {N} rows", flush=True)
+    table = torch.full((1, MP), -1, dtype=torch.int32, device=DEV)
+    blocks = [0, 1, MP // 3, MP - 2, MP - 1]
+    table[0, torch.tensor(blocks, device=DEV)] = torch.arange(len(blocks), dtype=torch.int32, device=DEV)
+    row = torch.randn((1, 1, 64), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    kp, vp = (torch.zeros((len(blocks) + 1, 1, bs, 32), dtype=torch.uint8, device=DEV).view(FP4) for _ in range(2))
+    ks, vs = (torch.zeros((len(blocks) + 1, 1, bs, 2), dtype=torch.uint8, device=DEV).view(E8M0) for _ in range(2))
+    ops.paged_append(row.to(DEV).expand(N, 1, 64), -row.to(DEV).expand(N, 1, 64), kp, vp, table, torch.tensor([held], device=DEV),
+                     cu=torch.tensor([0, N], dtype=torch.int32, device=DEV), k_scale=ks, v_scale=vs)
+    pos = torch.tensor(blocks)[:, None] * bs + torch.arange(bs)
+    written = (pos >= held) & (pos < N + held)
+    for got, s, x in ((kp, ks, row), (vp, vs, -row)):
+        q, e = OP.quantise(x[0])
+        for t, want in ((raw(got), q), (raw(s), e)):
+            assert torch.equal(t[:-1, 0][written], want.expand(int(written.sum()), -1)) and not t[:-1, 0][~written].any() and not t[-1].any()
+    lens = torch.tensor([N + held], device=DEV)
+    k, v = ops.paged_read(kp, vp, table, lens, rows=bs, cu=torch.tensor([0, bs], device=DEV), first=N + held - bs + 3, k_scale=ks, v_scale=vs)
+    want = OP.e2m1_values(*OP.quantise(row[0])).to(torch.bfloat16).to(DEV)
+    assert torch.equal(k[:bs - 3, 0], want.expand(bs - 3, -1)) and torch.equal(v[:bs - 3, 0], -want.expand(bs - 3, -1)) and not k[bs - 3:].any()
+
+
+def test_read_of_more_than_2_31_values(ops):
+    """One page under every block of a long sequence: the last rows of outputs past 2^31 elements."""
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB of device memory")
+    bs, Hkv, D, rows = 256, 8, 128, 2 ** 21 + 77
+    c = on_gpu(cache4([bs], Hq=8, Hkv=Hkv, D=D, bs=bs, seed=4))
+    table = c["table"][:, :1].expand(1, -(-rows // bs)).contiguous()
+    kw = dict(k_scale=c["k_scale"], v_scale=c["v_scale"])
+    k, v = ops.paged_read(c["k_pages"], c["v_pages"], table, torch.tensor([rows], device=DEV), rows=rows,
+                          cu=torch.tensor([0, rows], device=DEV), **kw)
+    wk, wv = ops.paged_read(c["k_pages"], c["v_pages"], table[:, :1], torch.tensor([bs], device=DEV), rows=bs,
+                            cu=torch.tensor([0, bs], device=DEV), **kw)
+    for got, want in ((k, wk), (v, wv)):
+        assert torch.equal(got[-77:], want[:77]) and torch.equal(got[-77 - bs:-77], want) and torch.equal(got[:bs], want)
+
+
 def test_read_without_rows(ops):
     c = on_gpu(cache4([20], Hq=2, Hkv=1, D=64, bs=16))
     for cu in (None, torch.zeros(2, dtype=torch.int32, device=DEV)):
@@ -363,6 +412,40 @@ def test_attn_of_every_code_and_of_small_and_large_scales(ops, dtype):
     check4(ops, c, DEV, scale=0.12, mass=torch.zeros((2, 2, c["table"].shape[1])))
     c["q"][:, ::2] *= 2.0 ** -12 if dtype == "fp16" else 2.0 ** -60
     check4(ops, c, DEV, scale=0.12)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attn_of_scales_at_the_ends(ops, dtype):
+    """Scales of V over 240 powers of two (what fp16 holds), of K down to the smallest ones."""
+    g = torch.Generator().manual_seed(9)
+    c = cache4([200, 61], Hq=6, Hkv=2, D=64, bs=32, dtype=dtype, seed=4)
+    of = lambda x, n: torch.tensor(x, dtype=torch.uint8)[torch.randint(0, len(x), c[n].shape, generator=g)].view(E8M0)  # noqa: E731
+    c["v_scale"] = of([8, 60, 127, 200, 245] if dtype == "bf16" else [100, 110, 127, 135], "v_scale")
+    c["k_scale"] = of([0, 1, 2, 30, 100, 128], "k_scale")
+    check4(ops, c, DEV, scale=0.12)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv", [(3000, 2, 1), (9, 300, 150)])
+def test_attn_of_many_sequences_and_of_many_heads(ops, B, Hq, Hkv):
+    """More sequences than are looked through at once, more columns than workgroups fit: as the attention over the
+    same cache in 16 bits, each rounded once."""
+    print(f"paged attn fp4 B={B} heads {Hq}/{Hkv}", flush=True)
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 70, (B,), generator=g).tolist()
+    c = on_gpu(cache4(lens, Hq=Hq, Hkv=Hkv, D=64, bs=16, seed=B))
+    out, lse = attend(ops, c)
+    rows = sum(lens)
+    cu = torch.tensor([0] + lens, device=DEV).cumsum(0)
+    k, v = ops.paged_read(*(c[k] for k in TENSORS[1:]), rows=rows, cu=cu, k_scale=c["k_scale"], v_scale=c["v_scale"])
+    kp, vp = (torch.zeros((c["k_pages"].shape[0], Hkv, 16, 64), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ops.paged_append(k, v, kp, vp, c["table"], torch.zeros(B, dtype=torch.int32, device=DEV), cu=cu)
+    want, wl = ops.paged_decode_attn(c["q"], kp, vp, c["table"], c["lens"], scale=0.12)
+    none = torch.tensor(lens, device=DEV) == 0
+    assert bool((out[none] == 0).all()) and bool((lse[none] == -math.inf).all())
+    # each result is rounded to bf16; before that a score, |scale|·Σ|q k| below 8, is off by 2^-14 at most, a probability
+    # by 2^-13 of it and an output by that of Σp|v|, below 8 too
+    assert bool(((out.float() - want.float()).abs() <= 2 * 2.0 ** -8 * want.float().abs() + 2 * 2.0 ** -10).all())
+    assert (lse - wl)[~none].abs().max() <= 2 * 2.0 ** -13
 
 
 def test_attn_is_that_over_the_values(ops):

@@ -287,3 +287,74 @@ int main() {
         open(src, "w").write(code)
         subprocess.run(["g++", "-std=c++17", src, "-o", exe], check=True)
         assert subprocess.run([exe]).returncode == 0
+
+
+def test_the_pieces_of_a_batch_have_slots():
+    """The pieces that the attention's wavefronts find over 4-bit pages are no more than the slots that the host laid
+    out, cover every tile once, and are as many as the device holds where the batch is large."""
+    import random
+    import subprocess
+    import tempfile
+
+    code = r'''
+#include <stdio.h>
+#include <stdlib.h>
+#include "%s/scope_amd/csrc/paged_plan.h"
+using namespace scope;
+int main(int argc, char** argv) {
+  // lines of B Hkv Hq D bs MP resident, then B lengths and B first positions
+  int B, Hkv, Hq, D, bs, MP, resident, line = 0;
+  while (scanf("%%d %%d %%d %%d %%d %%d %%d", &B, &Hkv, &Hq, &D, &bs, &MP, &resident) == 7) {
+    ++line;
+    int* lens = (int*)malloc(4 * B);
+    int* first = (int*)malloc(4 * B);
+    for (int b = 0; b < B; ++b) if (scanf("%%d", lens + b) != 1) return 1;
+    for (int b = 0; b < B; ++b) if (scanf("%%d", first + b) != 1) return 1;
+    const SplitSizes s = split_sizes(B, Hkv, D, bs, MP, Hq, 0);
+    const int cols = Hkv * ((Hq / Hkv + 15) / 16);
+    const int64_t cap = (int64_t)MP * bs;
+    int64_t total = 0, pieces = 0;
+    int lo;
+    for (int b = 0; b < B; ++b) total += seq_tiles(lens[b], first[b], cap, &lo);
+    const int w = pieces_wanted4(total, cols, B, resident), n = w < s.pieces ? w : s.pieces;
+    if (n < 1) return 2;
+    const int64_t piece = piece_tiles(total, n, kPieceTiles, piece_turn(D));
+    for (int b = 0; b < B; ++b) {
+      const int tiles = seq_tiles(lens[b], first[b], cap, &lo), m = seq_pieces(tiles, piece);
+      int at = lo;
+      for (int i = 0; i < m; ++i) {
+        int t0, t1;
+        piece_range(lo, tiles, m, i, &t0, &t1);
+        if (t0 != at || t1 < t0) return 3;
+        at = t1;
+      }
+      if (at != lo + tiles) return 4;
+      if (m > 1 && !s.split) return 5;
+      if (m > s.pieces + 1 && B == 1) return 6;
+      pieces += m;
+    }
+    if (pieces > s.slots) { printf("line %%d: %%lld pieces, %%d slots\\n", line, (long long)pieces, s.slots); return 7; }
+    // (as many as start together, one more a sequence, unless they would be longer than 120 tiles)
+    if (B == 1 && total > 12LL * resident / cols && total < 100LL * resident / cols && resident >= 2 * cols && s.pieces >= resident / cols &&
+        pieces * 2 < resident / cols) return 8;
+    free(lens);
+    free(first);
+  }
+  return line == 400 ? 0 : 9;
+}''' % ROOT
+    rng = random.Random(5)
+    lines = []
+    for _ in range(400):
+        B = rng.choice([1, 1, 2, 7, 63, 64, 65, 300])
+        Hkv, G = rng.choice([1, 2, 4, 8, 64, 600]), rng.choice([1, 4, 8, 16, 17, 40])
+        bs, D = rng.choice([16, 32, 128, 256]), rng.choice([64, 128, 256])
+        MP = max(1, int(2 ** rng.uniform(0, 13)))
+        lens = [rng.choice([rng.randint(-3, MP * bs + 5), int(MP * bs * rng.random() ** 4)]) for _ in range(B)]
+        first = [rng.choice([0, -2, rng.randint(0, MP * bs)]) for _ in range(B)]
+        lines.append(f"{B} {Hkv} {Hkv * G} {D} {bs} {MP} {rng.choice([512, 768, 1024])}\n{' '.join(map(str, lens))}\n{' '.join(map(str, first))}\n")
+    with tempfile.TemporaryDirectory() as d:
+        src, exe = os.path.join(d, "a.cc"), os.path.join(d, "a")
+        open(src, "w").write(code)
+        subprocess.run(["g++", "-std=c++17", src, "-o", exe], check=True)
+        r = subprocess.run([exe], input="".join(lines), text=True, capture_output=True)
+        assert r.returncode == 0, (r.returncode, r.stdout)
