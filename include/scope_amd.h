@@ -712,8 +712,8 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
  * 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte, the even feature in the low
  * nibble, and one e8m0 byte a group that stands for 2^(byte - 127), 255 for NaN
  * (the MXFP4 format).  The pages are [P][Hkv][bs][D/2] bytes: the strides of
- * scope_paged_cache count bytes then, its fp8 is not read, and `type` is that of q,
- * k, v and out.
+ * scope_paged_cache count bytes then (a row less than 2^26 from the next), its fp8
+ * is not read, and `type` is that of q, k, v and out.
  *   k_scale, v_scale  [P][Hkv][bs][D/32] bytes, page and head strides below, a
  *                     page's head contiguous and 16-byte aligned */
 typedef struct {
@@ -725,7 +725,8 @@ typedef struct {
  * 2^(x - 2), or 2^(x - 1) where a >= 1.75 · 2^x, kept to 2^-125 .. 2^125 (bf16 rows)
  * or 2^-125 .. 2^13 (fp16: six times it is finite); the codes are the nearest ones
  * of value / scale, the even one of two, at most 6.  A group that holds an infinity
- * or a NaN gets the scale 255 and codes 0. */
+ * or a NaN gets the scale 255 and codes 0.  No two rows may share a slot: one's codes
+ * could end beside the other's scales. */
 int scope_paged_append_fp4(const scope_paged_cache* c, const scope_paged_scales* s, int64_t N, const uint16_t* k, int64_t k_sn,
                            int64_t k_sh, const uint16_t* v, int64_t v_sn, int64_t v_sh, const int32_t* cu, const int32_t* table,
                            const int32_t* lens, void* k_scale, void* v_scale, void* k_pages, void* v_pages, void* stream);

@@ -311,9 +311,8 @@ __global__ __launch_bounds__(kAttnThreads, attn4_waves(D, WIDE)) void paged_attn
   const int lane = threadIdx.x & 63, wave = same(threadIdx.x >> 6), g4 = lane >> 4, c16 = lane & 15;
   const int G = a.Hq / c.Hkv, ng = (G + 15) / 16;
   // the columns of one piece start together, and pieces that there are not last
-  const int cols = gridDim.y;
-  const int64_t id = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
-  const int slot = same(static_cast<int>(id / cols)), column = same(static_cast<int>(id % cols));
+  const uint32_t cols = gridDim.y, id = blockIdx.y * gridDim.x + blockIdx.x;  // (less than 2^17 slots and 2^13 columns)
+  const int slot = same(id / cols), column = same(id % cols);
   const int hk = column / ng, cg = column % ng, nq = min(16, G - 16 * cg);
   const int h0 = hk * G + 16 * cg;                // first query head
   const int col = WIDE ? c16 : c16 & 7;           // this lane's

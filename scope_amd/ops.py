@@ -1241,10 +1241,11 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     k, v [N, Hkv, D] bf16 or fp16 (any row and head strides, rows 16-byte
     aligned); k_pages, v_pages [P, Hkv, bs, D] of the same type, or
     float8_e4m3fn holding x / scale[h] cut to ±448 (k_scale, v_scale [Hkv]
-    fp32), or float4_e2m1fn_x2 [P, Hkv, bs, D / 2] with k_scale, v_scale [P,
-    Hkv, bs, D / 32] float8_e8m0fnu, which are written too: a power of two for
-    each 32 features, so that the largest is at most 7 of it (cut to 6) and over
-    3.5 (a group with an infinity or a NaN becomes NaN); table [B, MP] int32 page ids; lens [B] the positions each sequence
+    fp32), or float4_e2m1fn_x2 [P, Hkv, bs, D / 2] (rows less than 2^26 bytes
+    apart) with k_scale, v_scale [P, Hkv, bs, D / 32] float8_e8m0fnu, which are
+    written too: a power of two for each 32 features, of which the largest is
+    3.5 to 7 (over 6 it becomes 6; a group with an infinity or a NaN becomes
+    NaN); table [B, MP] int32 page ids; lens [B] the positions each sequence
     holds before the call (it is not changed).  Row i goes to sequence b with
     cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing; without it N <= B
     and row i to sequence i), position lens[b] + i - cu[b].  Rows of no
@@ -1282,11 +1283,12 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     The cache as ``paged_append`` fills it, pages of any type.  Row i is that of
     sequence b with cu[b] <= i < cu[b + 1] (cu [B + 1] int, not decreasing;
     without it rows <= B and row i is of sequence i), position first[b] + i -
-    cu[b] (first [B] or one number, without it 0; without cu first[b]).  Rows of no sequence,
-    outside [0, lens[b]), past the table, or of a block whose entry is outside
-    [0, P) are zeros.  ``dtype``: bfloat16 or float16; 16-bit pages are read in
-    their own type (the default then), others in bfloat16 by default.  4-bit
-    values are exact in bfloat16; e4m3 ones are the fp32 product with their
+    cu[b] (first [B] or one number, without it 0; without cu first[b]).  Rows
+    of no sequence, outside [0, lens[b]), past the table, or of a block whose
+    entry is outside [0, P) are zeros.  ``dtype``: bfloat16 or float16; 16-bit
+    pages are read in their own type (the default then), others in bfloat16 by
+    default.  4-bit values are exact in bfloat16 and infinite where float16 does
+    not hold them; e4m3 ones are the fp32 product with their
     scale, rounded.  Nothing of it waits for the GPU.  It has no backward: a
     gradient that reaches its results raises."""
     who = "paged_read"

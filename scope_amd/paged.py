@@ -147,9 +147,9 @@ class PagedKVCache:
         rows = [max(0, n - f) for n, f in zip(self._len, first)] if rows is None else [int(n) for n in rows]
         if len(first) != B or len(rows) != B or any(f < 0 or n < 0 or (n and f + n > held) for f, n, held in zip(first, rows, self._len)):
             raise ValueError(f"PagedKVCache: rows {rows} from {first} on are not held ({self._len})")
-        at = torch.tensor([first + [0], rows + [0]], dtype=torch.int32).to(self.lens.device)
-        cu = torch.cat((at.new_zeros(1), at[1, :B].cumsum(0, dtype=torch.int32)))
-        return ops.paged_read(self.k_pages, self.v_pages, self.table, self.lens, rows=sum(rows), cu=cu, first=at[0, :B],
+        at, n = torch.tensor([first, rows], dtype=torch.int32).to(self.lens.device)
+        cu = torch.cat((n.new_zeros(1), n.cumsum(0, dtype=torch.int32)))
+        return ops.paged_read(self.k_pages, self.v_pages, self.table, self.lens, rows=sum(rows), cu=cu, first=at,
                               k_scale=self.k_scale, v_scale=self.v_scale, dtype=dtype)
 
     def evict(self, budget, *, window: int = 1, n_global: int = 0) -> int:
