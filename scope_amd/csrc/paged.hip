@@ -475,7 +475,9 @@ __global__ __launch_bounds__(256) void paged_finish_kernel(scope_paged_cache c, 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int2 plan = make_int2(1, 0);
   if (s.po) plan = lists ? make_int2(s.pieces, b * s.pieces) : s.plan[b];
-  const int n = plan.x;
+  // (lengths that another stream changes under a call leave any plan: it stays among the slots)
+  plan.y = min(max(plan.y, 0), s.slots - 1);
+  const int n = min(min(max(plan.x, 1), s.slots - plan.y), kMostPieces);
   const int64_t step = 2ll * a.Hq;
   const float* ml0 = s.pml + (static_cast<int64_t>(plan.y) * a.Hq + hk * G) * 2;  // of the group's first head
   if (x < 0) {
