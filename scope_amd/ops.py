@@ -1157,6 +1157,10 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError(f"{ctx.who} is not differentiable: detach its inputs or its results")
 
 
+def _wants_grad(t: torch.Tensor | None) -> bool:
+    return t is not None and t.requires_grad
+
+
 def _sat32(x: torch.Tensor) -> torch.Tensor:
     """Integers as contiguous int32; those past 32 bits as the nearest one, on the
     same side of every length and index."""
@@ -1292,9 +1296,9 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     scale, rounded.  Nothing of it waits for the GPU.  It has no backward: a
     gradient that reaches its results raises."""
     who = "paged_read"
-    if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad):
+    if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad or _wants_grad(k_scale) or _wants_grad(v_scale)):
         return _NoGradient.apply(who, functools.partial(paged_read, k_pages, v_pages, table, lens, rows=rows, cu=cu, first=first,
-                                                        k_scale=k_scale, v_scale=v_scale, dtype=dtype), k_pages, v_pages)
+                                                        k_scale=k_scale, v_scale=v_scale, dtype=dtype), k_pages, v_pages, k_scale, v_scale)
     dev = _device(who, k_pages, v_pages, table, lens, cu, first if isinstance(first, torch.Tensor) else None, k_scale, v_scale)
     pt = k_pages.dtype
     if dtype is None:
@@ -1342,10 +1346,11 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     can be captured and replayed while the lengths and the table change.  It has
     no backward: a gradient that reaches its results raises."""
     who = "paged_decode_attn"
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or _wants_grad(k_scale)
+                                    or _wants_grad(v_scale)):
         return _NoGradient.apply(who, functools.partial(paged_decode_attn, q, k_pages, v_pages, table, lens, scale=scale, first=first,
                                                         kv_num=kv_num, kv_idx=kv_idx, mass=mass, k_scale=k_scale, v_scale=v_scale),
-                                 q, k_pages, v_pages)
+                                 q, k_pages, v_pages, k_scale, v_scale)
     dev = _device(who, q, k_pages, v_pages, table, lens, first, kv_num, kv_idx, mass, k_scale, v_scale)
     shape, qs, dtype = q.shape, q.stride(), q.dtype
     c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)

@@ -157,6 +157,26 @@ def test_a_gradient_that_reaches_the_rows_raises(on_cpu, monkeypatch):  # noqa: 
         assert not any(x.requires_grad for x in ops.paged_read(kp, c["v_pages"], c["table"], c["lens"], rows=2))
 
 
+@needs_lib
+@pytest.mark.parametrize("name", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("fp8", [True, False])
+def test_a_gradient_that_reaches_the_scales_raises(on_cpu, monkeypatch, name, fp8):  # noqa: F811
+    """The results of e4m3 and 4-bit pages are products with their scales."""
+    ops = on_cpu
+    monkeypatch.setattr(ops, "_launch", lambda *a: None)
+    of = dict(Hq=4, Hkv=2, D=64, bs=16)
+    c = cache([40, 5], fp8=True, **of) if fp8 else cache4([40, 5], **of)
+    c[name] = c[name].clone().requires_grad_()
+    kw = dict(k_scale=c["k_scale"], v_scale=c["v_scale"])
+    for who, call in (("paged_read", lambda: ops.paged_read(c["k_pages"], c["v_pages"], c["table"], c["lens"], rows=2, **kw)),
+                      ("paged_decode_attn", lambda: call_of(ops, c))):
+        for x in call():
+            with pytest.raises(RuntimeError, match=f"{who} is not differentiable"):
+                x.float().sum().backward()
+        with torch.no_grad():
+            assert not any(x.requires_grad for x in call())
+
+
 def test_no_cpu_path():
     from scope_amd import ops
 
