@@ -1450,11 +1450,13 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
     ``out`` may be the logits themselves.  There is no backward: a gradient that
     reaches the result raises (what is written to ``out`` leaves the graph)."""
     who = "logit_penalties"
-    if torch.is_grad_enabled() and out is None and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+    numbers = (repetition, presence, frequency, temperature)
+    floats = all([type(x) is float for x in numbers])
+    if torch.is_grad_enabled() and out is None and (logits.requires_grad or _wants_grad(bias) or (
+            not floats and any(_wants_grad(x) for x in numbers if isinstance(x, torch.Tensor)))):
         return _NoGradient.apply(who, functools.partial(logit_penalties, logits, tokens, lens, first=first, n_prompt=n_prompt,
                                                         repetition=repetition, presence=presence, frequency=frequency,
-                                                        temperature=temperature, bias=bias, mask=mask), logits, bias)
-    numbers = (repetition, presence, frequency, temperature)
+                                                        temperature=temperature, bias=bias, mask=mask), logits, bias, *numbers)
     dev = _device(who, logits, tokens, bias, mask, out,
                   *[x for x in (lens, first, n_prompt, *numbers) if isinstance(x, torch.Tensor)])
     zd, shape, dtype = logits.dim(), logits.shape, logits.dtype
@@ -1476,7 +1478,7 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
             or (out.data_ptr() == logits.data_ptr() and B > 1 and out.stride(0) != logits.stride(0)):
         raise RuntimeError(f"{who}: out must have the logits' shape and type, rows of its own, and their strides if it is them")
     num, arr = numbers, (None, None, None, None)
-    if not all([type(x) is float for x in numbers]):
+    if not floats:
         arr = [_f32(x) if isinstance(x, torch.Tensor) else None for x in numbers]
         num = [1.0 if isinstance(x, torch.Tensor) else float(x) for x in numbers]
         for name, x in zip(("repetition", "presence", "frequency", "temperature"), numbers):

@@ -150,3 +150,16 @@ def test_a_gradient_that_reaches_the_results_raises(on_cpu, monkeypatch):
     assert ops.logit_penalties(z.detach(), t, 3, out=z.detach()).requires_grad is False
     with pytest.raises(RuntimeError, match="kv_num and kv_idx"):
         ops.paged_decode_attn(q, *rest, scale=0.1, kv_num=torch.ones(2, 2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("name", ["repetition", "presence", "frequency", "temperature"])
+def test_a_gradient_that_reaches_a_penaltys_rows_raises(on_cpu, monkeypatch, name):
+    """Penalties of one number a row, asked for a gradient."""
+    ops = on_cpu
+    monkeypatch.setattr(ops, "_launch", lambda *a: None)
+    z, t = torch.zeros(2, 70), torch.zeros(2, 9, dtype=torch.int64)
+    x = torch.ones(2, requires_grad=True)
+    with pytest.raises(RuntimeError, match="logit_penalties is not differentiable"):
+        ops.logit_penalties(z, t, 3, **{name: x}).sum().backward()
+    assert ops.logit_penalties(z, t, 3, **{name: x}, out=z).requires_grad is False
+    assert ops.logit_penalties(z, t, 3, **{name: x.detach()}).requires_grad is False
