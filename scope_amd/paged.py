@@ -137,13 +137,14 @@ class PagedKVCache:
     def read(self, rows=None, first=None, *, dtype: torch.dtype | None = None):
         """The rows of the ``rows[b]`` positions from first[b] on of each sequence b, one
         sequence after the other -> k, v [sum(rows), kv_heads, head_dim] of ``dtype``
-        (``ops.paged_read``; 16-bit pages in their own).  ``first`` of None is 0,
-        ``rows`` of None what each sequence holds from there on; positions whose page
-        was evicted are zeros.  The numbers are the host's: nothing waits for the GPU
-        but their copy from pageable memory."""
+        (``ops.paged_read``; 16-bit pages in their own).  ``first`` may be one number
+        for all, None is 0; ``rows`` of None is what each sequence holds from there on;
+        positions whose page was evicted are zeros.  The numbers are the host's: nothing
+        waits for the GPU but their copy from pageable memory."""
         self._on_host("read")
         B = len(self._len)
-        first = [0] * B if first is None else [int(n) for n in first]
+        first = 0 if first is None else first.tolist() if isinstance(first, torch.Tensor) else first
+        first = [int(n) for n in first] if hasattr(first, "__iter__") else [int(first)] * B
         rows = [max(0, n - f) for n, f in zip(self._len, first)] if rows is None else [int(n) for n in rows]
         if len(first) != B or len(rows) != B or any(f < 0 or n < 0 or (n and f + n > held) for f, n, held in zip(first, rows, self._len)):
             raise ValueError(f"PagedKVCache: rows {rows} from {first} on are not held ({self._len})")

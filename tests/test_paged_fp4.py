@@ -177,6 +177,33 @@ def test_a_gradient_that_reaches_the_scales_raises(on_cpu, monkeypatch, name, fp
             assert not any(x.requires_grad for x in call())
 
 
+@pytest.fixture()
+def held(monkeypatch):
+    """A cache of three sequences of 40, 0 and 7 rows on the CPU, and what its reads pass on: (rows, first, cu)."""
+    from scope_amd import PagedKVCache, ops
+
+    monkeypatch.setattr(ops, "paged_append", lambda *a, **kw: None)
+    monkeypatch.setattr(ops, "paged_read", lambda *a, rows, cu, first, **kw: (rows, first.tolist(), cu.tolist()))
+    c = PagedKVCache(pages=9, sequences=3, max_len=64, kv_heads=1, head_dim=64, page_size=16, device="cpu")
+    x = torch.zeros((47, 1, 64), dtype=torch.bfloat16)
+    c.append(x, x, [40, 0, 7])
+    return c
+
+
+def test_a_cache_is_read_from_one_number_on(held):
+    assert held.read() == held.read(first=0) == (47, [0, 0, 0], [0, 40, 40, 47])
+    rows, first, cu = held.read(first=5)
+    assert (rows, cu) == (37, [0, 35, 35, 37]) and (first[0], first[2]) == (5, 5)
+    for f in ([5, 0, 5], torch.tensor([5, 0, 5])):
+        assert held.read(first=f) == (37, [5, 0, 5], [0, 35, 35, 37])
+    for f in (torch.tensor(2), 2):
+        rows, first, cu = held.read([3, 0, 5], f)
+        assert (rows, cu) == (8, [0, 3, 3, 8]) and (first[0], first[2]) == (2, 2)
+    for f in (-1, [0, -1, 0], [0, 0], []):
+        with pytest.raises(ValueError, match="are not held"):
+            held.read(first=f)
+
+
 def test_no_cpu_path():
     from scope_amd import ops
 
