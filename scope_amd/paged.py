@@ -148,7 +148,8 @@ class PagedKVCache:
         rows = [max(0, n - f) for n, f in zip(self._len, first)] if rows is None else [int(n) for n in rows]
         if len(first) != B or len(rows) != B or any(f < 0 or n < 0 or (n and f + n > held) for f, n, held in zip(first, rows, self._len)):
             raise ValueError(f"PagedKVCache: rows {rows} from {first} on are not held ({self._len})")
-        at, n = torch.tensor([first, rows], dtype=torch.int32).to(self.lens.device)
+        # (where no row is read, first may be any number)
+        at, n = torch.tensor([[f if n else 0 for f, n in zip(first, rows)], rows], dtype=torch.int32).to(self.lens.device)
         cu = torch.cat((n.new_zeros(1), n.cumsum(0, dtype=torch.int32)))
         return ops.paged_read(self.k_pages, self.v_pages, self.table, self.lens, rows=sum(rows), cu=cu, first=at,
                               k_scale=self.k_scale, v_scale=self.v_scale, dtype=dtype)

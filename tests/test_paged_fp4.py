@@ -204,6 +204,12 @@ def test_a_cache_is_read_from_one_number_on(held):
             held.read(first=f)
 
 
+def test_a_cache_read_from_behind_its_rows_gives_none(held):
+    for far in (40, 2 ** 31, 2 ** 63):
+        assert held.read(first=far) == (0, [0, 0, 0], [0, 0, 0, 0])
+        assert held.read([2, 0, 0], [38, far, far]) == (2, [38, 0, 0], [0, 2, 2, 2])
+
+
 def test_no_cpu_path():
     from scope_amd import ops
 
