@@ -76,10 +76,9 @@ class PagedKVCache:
     def length(self, sequence: int) -> int:
         return self._len[sequence]
 
-    def _on_host(self, what: str) -> None:
+    def _on_host(self, what: str, does: str = "changes lengths or pages on the host, which a replayed graph would not") -> None:
         if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"PagedKVCache: {what} changes lengths or pages on the host, which a replayed graph would not; "
-                               "capture the operators of scope_amd.ops instead")
+            raise RuntimeError(f"PagedKVCache: {what} {does}; capture the operators of scope_amd.ops instead")
 
     def reserve(self, rows) -> None:
         """Takes the pages that rows[b] more positions of each sequence b need;
@@ -141,7 +140,7 @@ class PagedKVCache:
         for all, None is 0; ``rows`` of None is what each sequence holds from there on;
         positions whose page was evicted are zeros.  The numbers are the host's: nothing
         waits for the GPU but their copy from pageable memory."""
-        self._on_host("read")
+        self._on_host("read", "goes by the lengths on the host, which a replayed graph would not see change")
         B = len(self._len)
         first = 0 if first is None else first.tolist() if isinstance(first, torch.Tensor) else first
         first = [int(n) for n in first] if hasattr(first, "__iter__") else [int(first)] * B

@@ -210,6 +210,20 @@ def test_a_cache_read_from_behind_its_rows_gives_none(held):
         assert held.read([2, 0, 0], [38, far, far]) == (2, [38, 0, 0], [0, 2, 2, 2])
 
 
+def test_what_a_captured_call_of_the_cache_says(held, monkeypatch):
+    """read changes nothing on the host, the others do."""
+    class OnGPU:
+        is_cuda = True
+
+    held.table = OnGPU()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="read goes by the lengths on the host"):
+        held.read()
+    for call, name in ((lambda: held.reserve([1, 1, 1]), "reserve"), (lambda: held.evict(1), "evict"), (lambda: held.release(0), "release")):
+        with pytest.raises(RuntimeError, match=f"{name} changes lengths or pages on the host"):
+            call()
+
+
 def test_no_cpu_path():
     from scope_amd import ops
 
