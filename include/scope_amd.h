@@ -693,7 +693,10 @@ int scope_paged_append(const scope_paged_cache* c, int64_t N, const uint16_t* k,
  *   out [B][Hq][D]     softmax(scale · q·k) · v; zeros where nothing is seen; an
  *                      infinite value of v in a seen row gives that infinity (or
  *                      NaN, where the row's weight is below 2^-15 in fp16, 2^-100
- *                      in bf16, of the largest among the 32 positions around it)
+ *                      in bf16, of the largest among the 32 positions around it).
+ *                      Sums in fp32, over bf16 values with weights of up to 2^8:
+ *                      sure to be finite while 2^8 · Σ|v| of the seen rows is
+ *                      below 2^128
  *   lse [B][Hq]        natural logarithm of the sum; -inf there
  *   work               scope_paged_attn_workspace_bytes; with a mass it grows with
  *                      the table's width, whatever the lengths: 4·B·Hq·MP·bs/32
@@ -732,7 +735,9 @@ int scope_paged_append_fp4(const scope_paged_cache* c, const scope_paged_scales*
                            const int32_t* lens, void* k_scale, void* v_scale, void* k_pages, void* v_pages, void* stream);
 
 /* scope_paged_decode_attn over such pages (its workspace alike).  A NaN scale of a
- * seen row of K makes its queries' outputs NaN, one of V the features of its group. */
+ * seen row of K makes its queries' outputs NaN, one of V the features of its group.
+ * So may the scales 253 and 254, which the append does not write, over a value of
+ * 2^128 or more. */
 int scope_paged_decode_attn_fp4(const scope_paged_cache* c, const scope_paged_scales* s, int Hq, int maxkv, float scale,
                                 const uint16_t* q, int64_t q_sb, int64_t q_sh, const void* k_pages, const void* v_pages,
                                 const void* k_scale, const void* v_scale, const int32_t* table, const int32_t* lens,
@@ -745,7 +750,8 @@ int scope_paged_decode_attn_fp4(const scope_paged_cache* c, const scope_paged_sc
  * Rows of no sequence, outside [0, lens[b]) or of a block without a page are zeros.
  * s NULL: pages of `type`, moved as they are, or e4m3 (c->fp8; byte · scale[h] in
  * fp32, rounded to `type`; k_scale, v_scale [Hkv] fp32 or NULL); else 4-bit pages
- * (exact in bf16; rounded to fp16, infinite where that does not hold the value). */
+ * (exact in bf16, infinite from 2^128 on, which scales that the append does not write
+ * reach; rounded to fp16, infinite where that does not hold the value). */
 int scope_paged_read(const scope_paged_cache* c, const scope_paged_scales* s, int64_t N, const int32_t* cu, const int32_t* table,
                      const int32_t* lens, const int32_t* first, const void* k_scale, const void* v_scale, const void* k_pages,
                      const void* v_pages, uint16_t* k, uint16_t* v, void* stream);

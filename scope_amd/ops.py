@@ -1291,9 +1291,9 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     of no sequence, outside [0, lens[b]), past the table, or of a block whose
     entry is outside [0, P) are zeros.  ``dtype``: bfloat16 or float16; 16-bit
     pages are read in their own type (the default then), others in bfloat16 by
-    default.  4-bit values are exact in bfloat16 and infinite where float16 does
-    not hold them; e4m3 ones are the fp32 product with their
-    scale, rounded.  Nothing of it waits for the GPU.  It has no backward: a
+    default.  4-bit values are exact in bfloat16 but for those of 2^128 and more
+    (under scales that no append writes), which are infinite there, as in float16
+    what it does not hold; e4m3 ones are the fp32 product with their scale, rounded.  Nothing of it waits for the GPU.  It has no backward: a
     gradient that reaches its results raises."""
     who = "paged_read"
     if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad or _wants_grad(k_scale) or _wants_grad(v_scale)):
@@ -1337,7 +1337,10 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     row's weight is below 2^-15 in fp16, 2^-100 in bf16, of the largest among
     the 32 positions around it).  4-bit pages (their rows less than 2^26 bytes
     apart) hold no infinities: a group without a number in a seen row of v makes
-    its features NaN, one of k the whole output.
+    its features NaN, one of k the whole output, and so may one under a scale of
+    2^126 or 2^127 (which no append writes) with a value of 2^128 or more.  Over
+    bfloat16 and 4-bit pages outputs are sums in fp32 with weights of up to 2^8:
+    one is sure to be finite while 2^8 · Σ|v| over the seen rows is below 2^128.
     ``mass`` [B, Hkv, MP] fp32 contiguous gets each block's probabilities,
     summed over its positions and the group's query heads, added in place
     (lists without repeats then; not two calls on one mass at a time).  Its

@@ -10,8 +10,8 @@ import pytest
 import torch
 
 from oracle import paged as OP
-from tests.paged_fp4_inputs import E8M0, FP4, cache4, check4, pages
-from tests.paged_inputs import TYPES, cache, tables
+from tests.paged_fp4_inputs import E8M0, FP4, bounds4, cache4, check4, pages
+from tests.paged_inputs import TYPES, assert_within, cache, tables
 from tests.test_paged_fp4 import groups
 
 pytestmark = pytest.mark.gpu
@@ -169,6 +169,21 @@ def test_read_of_every_byte_and_scale(ops, dtype):
     want = OP.e2m1_values(kp, ks).reshape(4096, 1, 64).to(TYPES[dtype])
     for x in (k, v):
         assert torch.equal(torch.isnan(x.cpu()), torch.isnan(want)) and torch.equal(x.cpu().nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_read_is_infinite_where_the_type_does_not_hold_the_value(ops, dtype):
+    """All codes under all scales, infinities as such: from 2^128 on in bf16 (scales 253 and 254), past 65504 in fp16."""
+    codes = torch.arange(16, dtype=torch.uint8).repeat_interleave(2).reshape(1, 1, 1, 32).expand(256, 1, 16, 32) * 17  # (both features)
+    ks = torch.arange(256, dtype=torch.uint8).reshape(256, 1, 1, 1).expand(256, 1, 16, 2).contiguous()
+    table = torch.arange(256, dtype=torch.int32, device=DEV)[None]
+    p, s = codes.contiguous().to(DEV).view(FP4), ks.to(DEV).view(E8M0)
+    got, _ = ops.paged_read(p, p, table, torch.tensor([4096], device=DEV), rows=4096, cu=torch.tensor([0, 4096], device=DEV), k_scale=s,
+                            v_scale=s, dtype=TYPES[dtype])
+    want = OP.e2m1_values(codes, ks).reshape(4096, 1, 64).to(TYPES[dtype])
+    nan, got = torch.isnan(want), got.cpu()
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], want[~nan])
+    assert bool(torch.isinf(got).any()) and bool(torch.isinf(got[:253 * 16]).any()) == (dtype == "fp16")
 
 
 def test_read_from_one_number_on(ops):
@@ -383,6 +398,36 @@ def test_attn_nan_in_seen_rows(ops, D):
             assert bool(nan[:2].all()) and bool(torch.isnan(lse[0, :2]).all())
         else:
             assert bool(nan[:2, G:2 * G].all()) and int(nan.sum()) == 2 * G and bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("G,D", [(2, 64), (8, 128), (9, 64), (4, 256)])
+@pytest.mark.parametrize("name", ["v_scale", "k_scale"])
+def test_attn_of_the_largest_scales(ops, G, D, name):
+    """One group of one seen row under scales up to NaN: no other feature (of K: no other key head) gets another bit; of
+    V its own are right while 2^8 times the sum of the row's |v| is below 2^128, and not finite from 2^128 on."""
+    c = cache4([300], Hq=2 * G, Hkv=2, D=D, bs=64, seed=23)
+    page, group = int(c["table"][0, 3]), slice(32, 64)
+    c[name.replace("scale", "pages")].view(torch.uint8)[page, 0, 5, 16:32] = 0x77  # (6 in every feature of the group)
+    d = on_gpu(c)
+    want, wl = attend(ops, d)
+    apart = torch.ones(want.shape, dtype=torch.bool, device=DEV)
+    apart[0, :G, group if name == "v_scale" else slice(None)] = False
+    for byte in (200, 230, 240, 244, 246, 248, 250, 251, 252, 253, 254, 255):
+        c[name].view(torch.uint8)[page, 0, 5, 1] = byte
+        d[name] = c[name].to(DEV)
+        out, lse = attend(ops, d)
+        assert torch.equal(out[apart], want[apart]), byte
+        if name == "k_scale":
+            assert torch.equal(lse[0, G:], wl[0, G:]), byte
+            continue
+        assert torch.equal(lse, wl), byte
+        if byte <= 244:  # (2^8 · 6 · 2^117 and little more)
+            assert bool(torch.isfinite(out.float()).all()), byte
+            r = OP.decode_attn(c["q"], OP.e2m1_values(c["k_pages"], c["k_scale"]), OP.e2m1_values(c["v_pages"], c["v_scale"]), c["table"],
+                               c["lens"], scale=0.12)
+            assert_within("out", out, r["out"], bounds4(c["q"].dtype, D, r)[0])
+        elif byte > 252:
+            assert not bool(torch.isfinite(out[0, :G, group].float()).any()), byte
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
