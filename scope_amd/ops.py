@@ -1262,17 +1262,19 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)
     if len(shape) != 3 or shape != v.shape or v.dtype != dtype or shape[1] != c.Hkv or shape[2] != c.D or ks[2] != 1 or vs[2] != 1:
         raise RuntimeError(f"{who}: k and v must be [N, {c.Hkv}, {c.D}] of one type with a contiguous last dimension")
-    fp4 = k_pages.dtype == _FP4
-    for t in (k_pages, v_pages) + ((k_scale, v_scale) if fp4 else ()):
-        if 0 in t.stride() and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-            raise RuntimeError(f"{who}: the pages are an expanded tensor: their rows share memory")
+    scales = _paged_scales(who, c, k_scale, v_scale) if k_pages.dtype == _FP4 else None
+    if not (c.k_sp and c.k_sh and c.k_sr and c.v_sp and c.v_sh and c.v_sr) or (
+            scales and not (scales.k_sp and scales.k_sh and scales.v_sp and scales.v_sh)):
+        for t in (k_pages, v_pages, k_scale, v_scale) if scales else (k_pages, v_pages):
+            if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                raise RuntimeError(f"{who}: the pages are an expanded tensor: their rows share memory")
     lens = _ints(who, "lens", lens, c.B, dev)
     cu = _ints(who, "cu", cu, c.B + 1, dev)
     N, one = shape[0], c.Hkv == 1
     args = (N, k.data_ptr(), ks[0] if N > 1 else 0, 0 if one else ks[1], v.data_ptr(), vs[0] if N > 1 else 0, 0 if one else vs[1],
             _ptr(cu), table.data_ptr(), lens.data_ptr(), _ptr(k_scale), _ptr(v_scale), k_pages.data_ptr(), v_pages.data_ptr())
-    if fp4:
-        _launch(dev, "scope_paged_append_fp4", C.byref(c), C.byref(_paged_scales(who, c, k_scale, v_scale)), *args)
+    if scales:
+        _launch(dev, "scope_paged_append_fp4", C.byref(c), C.byref(scales), *args)
     else:
         _launch(dev, "scope_paged_append", C.byref(c), *args)
 

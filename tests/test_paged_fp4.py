@@ -125,6 +125,27 @@ def test_scales_that_do_not_fit_are_refused(on_cpu):  # noqa: F811
                          v_scale=c["v_scale"])
 
 
+@pytest.mark.parametrize("name", ["k_pages", "v_pages", "k_scale", "v_scale"])
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_rows_are_not_written_into_expanded_tensors(on_cpu, name, dim):  # noqa: F811
+    """Any of them, along any dimension; one of a single element is no expansion."""
+    ops = on_cpu
+    kv = torch.zeros((2, 2, 64), dtype=torch.bfloat16)
+    of = dict(Hq=4, Hkv=2, D=64, bs=16)
+
+    def call(c, kv=kv):
+        ops.paged_append(kv, kv, c["k_pages"], c["v_pages"], c["table"], c["lens"], k_scale=c["k_scale"], v_scale=c["v_scale"])
+
+    for c in (cache4([40, 5], **of),) + ((cache([40, 5], **of),) if name.endswith("pages") else ()):
+        with pytest.raises(RuntimeError, match="expanded|contiguous in a page's head"):
+            call(dict(c, **{name: c[name].narrow(dim, 0, 1).expand(c[name].shape)}))
+    c = cache4([5, 0], Hq=1, Hkv=1, D=64, bs=16)
+    one = {n: c[n][:1] for n in ("k_pages", "v_pages", "k_scale", "v_scale")}
+    one[name] = one[name][0, 0][None, None].expand(1, 1, -1, -1)
+    with pytest.raises(Reached):
+        call(dict(c, **one), kv[:, :1])
+
+
 def test_reads_that_do_not_fit_are_refused(on_cpu):  # noqa: F811
     ops = on_cpu
     c = cache([40, 5], Hq=4, Hkv=2, D=64, bs=16)
