@@ -14,6 +14,16 @@
 
 namespace scope {
 
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// the sum and the largest over all lanes
+__device__ __forceinline__ float sum_of(float v) {
+  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0u, add_f32), 63));
+}
+__device__ __forceinline__ float max_of(float v) {
+  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0xff800000u, max_f32), 63));
+}
+
 // ---- append ------------------------------------------------------------------
 // Row i of the N new ones belongs to the sequence b with cu[b] <= i < cu[b + 1]
 // (row i to sequence i without cu) and goes to position lens[b] + i - cu[b].
@@ -119,6 +129,36 @@ __global__ __launch_bounds__(256) void paged_append_kernel(scope_paged_cache c, 
 }
 
 // ---- attention of one new token -------------------------------------------------
+// the largest 16-bit values below two positive numbers (0 below 0)
+template <int TYPE>
+__device__ __forceinline__ uint32_t below2(float lo, float hi) {
+  const uint32_t a = __builtin_elementwise_sub_sat(__float_as_uint(lo), 1u), b = __builtin_elementwise_sub_sat(__float_as_uint(hi), 1u);
+  if constexpr (TYPE == SCOPE_BF16)
+    return pack_hi16(a, b);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(a), __uint_as_float(b)));
+}
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+
+// N words that are read once: they are not kept in the caches in front of others
+template <int N>
+__device__ __forceinline__ Words<N> load_once(const char* p) {
+  Words<N> x;
+  if constexpr (N == 1) {
+    x.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  } else {
+    typedef uint32_t words_t __attribute__((ext_vector_type(N), aligned(4)));
+    const words_t v = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(p));
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.w[i] = v[i];
+  }
+  return x;
+}
+
 template <int TYPE>
 __device__ __forceinline__ f32x4_t mfma_16(const uint4& a, const uint4& b, const f32x4_t& acc) {
   if constexpr (TYPE == SCOPE_BF16) {
@@ -233,7 +273,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
     qf[j] = make_uint4(0, 0, 0, 0);
     if (c16 < nq) qf[j] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (h0 + c16) * a.q_sh + d);
   }
-  const float to_log2 = a.scale * kLog2e * (a.k_scale ? a.k_scale[hk] : 1.f);
+  const float to_log2 = a.scale * kLog2e * (a.k_scale ? static_cast<const float*>(a.k_scale)[hk] : 1.f);
 
   f32x4_t acc[NH * VE];
 #pragma unroll
@@ -434,7 +474,7 @@ __global__ __launch_bounds__(kAttnThreads, attn_waves(D, FP8)) void paged_attn_k
               acc[h * VE + j][r], acc[h * VE + j + 1][r], acc[h * VE + j + 2][r], acc[h * VE + j + 3][r]);
   }
   __syncthreads();
-  join_shares<TYPE, D>(a, s, p, h0, nq, a.v_scale ? a.v_scale[hk] : 1.f, z);
+  join_shares<TYPE, D>(a, s, p, h0, nq, a.v_scale ? static_cast<const float*>(a.v_scale)[hk] : 1.f, z);
 }
 
 // (maximum, sum relative to it) of a row from its n pieces' (maximum, sum) pairs,
@@ -513,7 +553,7 @@ __global__ __launch_bounds__(256) void paged_finish_kernel(scope_paged_cache c, 
       float o = 0.f;
 #pragma unroll
       for (int i = 0; i < NG; ++i) o += so[i][tid];
-      const float y = ML.y == 0.f ? 0.f : o / ML.y * (a.v_scale ? a.v_scale[hk] : 1.f);
+      const float y = ML.y == 0.f ? 0.f : o / ML.y * (a.v_scale ? static_cast<const float*>(a.v_scale)[hk] : 1.f);
       a.out[(static_cast<int64_t>(b) * a.Hq + h) * D + tid] = c.type == SCOPE_FP16 ? f32_to_half(y) : f32_to_bf16(y);
       if (tid == 0)
         a.lse[static_cast<int64_t>(b) * a.Hq + h] = ML.y == 0.f ? -INFINITY : (ML.x + __builtin_amdgcn_logf(ML.y)) * kLn2;
@@ -816,8 +856,10 @@ int check_attn(const scope_paged_cache& c, const PagedAttnArgs& a, void* work, A
   return SCOPE_OK;
 }
 
-int launch_paged_finish(const scope_paged_cache& c, const PagedAttnArgs& a, const AttnSplit& s, hipStream_t st) {
-  if (!s.po && !a.mass) return SCOPE_OK;  // every sequence is one piece
+int launch_paged_finish(const scope_paged_cache& c, const PagedAttnArgs& args, const float* v_scale, const AttnSplit& s, hipStream_t st) {
+  if (!s.po && !args.mass) return SCOPE_OK;  // every sequence is one piece
+  PagedAttnArgs a = args;
+  a.v_scale = v_scale;
   const int G = a.Hq / c.Hkv, blocks = a.kv_idx ? a.maxkv : c.MP;
   const dim3 fg((s.po ? G : 0) + (a.mass ? ceil_div(blocks, 256) : 0), c.Hkv, c.B);
   if (c.D == 64)
@@ -898,7 +940,7 @@ int scope_paged_decode_attn(const scope_paged_cache* c, int Hq, int maxkv, float
     c->fp8 ? launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, true>{})
            : launch(integral_constant<int, SCOPE_FP16>{}, integral_constant<bool, false>{});
   if (int rc = check_launch("paged_attn_kernel")) return rc;
-  return launch_paged_finish(*c, a, s, st);
+  return launch_paged_finish(*c, a, v_scale, s, st);
 }
 
 int scope_paged_evict(int B, int Hkv, int MP, int bs, int window, int n_global, const int32_t* table, const float* mass,

@@ -786,24 +786,8 @@ int scope_paged_decode_attn_fp4(const scope_paged_cache* c, const scope_paged_sc
   const scope_paged_cache bytes = in_bytes(*c);
   if (int rc = check_cache(&bytes, k_pages, v_pages, fn)) return rc;
   if (int rc = check_scales(c, z, k_scale, v_scale, fn)) return rc;
-  PagedAttnArgs a{Hq,
-                  maxkv,
-                  scale,
-                  q_sb,
-                  q_sh,
-                  q,
-                  k_pages,
-                  v_pages,
-                  reinterpret_cast<const float*>(k_scale),
-                  reinterpret_cast<const float*>(v_scale),
-                  table,
-                  lens,
-                  first,
-                  kv_num,
-                  kv_idx,
-                  mass,
-                  out,
-                  lse};
+  const PagedAttnArgs a{Hq,      maxkv, scale, q_sb,  q_sh,   q,      k_pages, v_pages, k_scale,
+                        v_scale, table, lens,  first, kv_num, kv_idx, mass,    out,     lse};
   AttnSplit s;
   if (int rc = check_attn(bytes, a, work, &s, fn)) return rc;
   const int G = Hq / c->Hkv, ng = (G + 15) / 16;
@@ -826,8 +810,7 @@ int scope_paged_decode_attn_fp4(const scope_paged_cache* c, const scope_paged_sc
   const auto of_type = [&](auto type) { c->bs == 16 ? of_width(type, true_type{}) : of_width(type, false_type{}); };
   c->type == SCOPE_BF16 ? of_type(std::integral_constant<int, SCOPE_BF16>{}) : of_type(std::integral_constant<int, SCOPE_FP16>{});
   if (int rc = check_launch("paged_attn4_kernel")) return rc;
-  a.v_scale = nullptr;
-  return launch_paged_finish(bytes, a, s, st);
+  return launch_paged_finish(bytes, a, nullptr, s, st);
 }
 
 }  // extern "C"

@@ -13,7 +13,6 @@ namespace scope {
 __device__ __forceinline__ float half_to_f32(uint16_t h) { return static_cast<float>(__builtin_bit_cast(_Float16, h)); }
 __device__ __forceinline__ uint16_t f32_to_half(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
 
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 // op over a wavefront in six steps on neighbouring lanes' registers (row shifts by
@@ -52,14 +51,8 @@ __device__ __forceinline__ float over_rows(float v, Op op) {
   const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return __uint_as_float(op(r[0], r[1]));
 }
-// the sums over lanes 0 .. l of a count, and over all lanes
+// the sums over lanes 0 .. l of a count
 __device__ __forceinline__ int prefix_of(int v) { return static_cast<int>(lane_prefix(static_cast<uint32_t>(v), 0u, add_u32)); }
-__device__ __forceinline__ float sum_of(float v) {
-  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0u, add_f32), 63));
-}
-__device__ __forceinline__ float max_of(float v) {
-  return __uint_as_float(__builtin_amdgcn_readlane(lane_prefix(__float_as_uint(v), 0xff800000u, max_f32), 63));
-}
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -81,8 +74,8 @@ struct PagedAttnArgs {
   const uint16_t* q;
   const void* k_pages;
   const void* v_pages;
-  const float* k_scale;
-  const float* v_scale;
+  const void* k_scale;  // of e4m3 pages [Hkv] fp32, of 4-bit ones their bytes
+  const void* v_scale;
   const int32_t* table;
   const int32_t* lens;
   const int32_t* first;
@@ -93,8 +86,9 @@ struct PagedAttnArgs {
   float* lse;
 };
 
-// Workgroups of kAttnWaves wavefronts; piece i of the batch (paged_plan.h) is
-// blockIdx.x, (key head, group of 16 query heads) blockIdx.y.
+// Workgroups of kAttnWaves wavefronts, one for each piece of the batch (paged_plan.h) and
+// column (key head, group of 16 query heads): blockIdx.x and blockIdx.y over 16-bit and
+// 8-bit pages; over 4-bit ones the columns of a piece come one after the other.
 constexpr int kAttnThreads = 64 * kAttnWaves;
 
 struct AttnSplit {
@@ -173,16 +167,6 @@ __device__ __forceinline__ uint32_t round2(float lo, float hi) {
   }
 }
 
-// the largest 16-bit values below two positive numbers (0 below 0)
-template <int TYPE>
-__device__ __forceinline__ uint32_t below2(float lo, float hi) {
-  const uint32_t a = __builtin_elementwise_sub_sat(__float_as_uint(lo), 1u), b = __builtin_elementwise_sub_sat(__float_as_uint(hi), 1u);
-  if constexpr (TYPE == SCOPE_BF16)
-    return pack_hi16(a, b);
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(a), __uint_as_float(b)));
-}
-
 // the halves of a word of two 16-bit values
 template <int TYPE>
 __device__ __forceinline__ float low_half(uint32_t w) {
@@ -191,26 +175,6 @@ __device__ __forceinline__ float low_half(uint32_t w) {
 template <int TYPE>
 __device__ __forceinline__ float high_half(uint32_t w) {
   return TYPE == SCOPE_BF16 ? __uint_as_float(w & 0xffff0000u) : half_to_f32(static_cast<uint16_t>(w >> 16));
-}
-
-template <int N>
-struct Words {
-  uint32_t w[N];
-};
-
-// N words that are read once: they are not kept in the caches in front of others
-template <int N>
-__device__ __forceinline__ Words<N> load_once(const char* p) {
-  Words<N> x;
-  if constexpr (N == 1) {
-    x.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
-  } else {
-    typedef uint32_t words_t __attribute__((ext_vector_type(N), aligned(4)));
-    const words_t v = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(p));
-#pragma unroll
-    for (int i = 0; i < N; ++i) x.w[i] = v[i];
-  }
-  return x;
 }
 
 // The end of a piece: the wavefronts' maxima and sums (relative to those) in sm, sl
@@ -263,7 +227,7 @@ inline bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 
 int check_cache(const scope_paged_cache* c, const void* k_pages, const void* v_pages, const char* fn);
 // The checks of an attention call beside those of its pages, and its pieces in *s.
 int check_attn(const scope_paged_cache& c, const PagedAttnArgs& a, void* work, AttnSplit* s, const char* fn);
-// What follows the pieces' kernel.
-int launch_paged_finish(const scope_paged_cache& c, const PagedAttnArgs& a, const AttnSplit& s, hipStream_t st);
+// What follows the pieces' kernel; v_scale: the factors [Hkv] of joined outputs, or null.
+int launch_paged_finish(const scope_paged_cache& c, const PagedAttnArgs& a, const float* v_scale, const AttnSplit& s, hipStream_t st);
 
 }  // namespace scope
