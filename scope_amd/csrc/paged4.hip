@@ -73,7 +73,7 @@ __device__ __forceinline__ void each_chunk(const MoveArgs& m, int n, int2 places
 
 // Rows written: a quad of lanes has a group of 32 features, so that its largest value
 // takes two steps in registers, and every lane moves 16 bytes in and 4 out.  Bound by
-// memory: 65539 rows of 8 heads of 128 (340 MB) 66 us, 5.1 TB/s, as a large copy (four
+// memory: 65539 rows of 8 heads of 128 (340 MB) 66.5 us, 5.1 TB/s, as a large copy (four
 // rows a wavefront instead of two, or none passing the caches, 5 to 20 us more).
 struct Append4Args {
   int64_t k_sn, k_sh, v_sn, v_sh;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void paged_append4_kernel(scope_paged_cache c,
 }
 
 // Rows read: 16 bytes out a lane, past the caches (131072 rows of 4 bits 149 -> 140 us, 4.9
-// TB/s; 12k of e4m3 38.5 -> 26.6; one row a wavefront 142, K and V by workgroups of their
+// TB/s; 24k of e4m3 38.5 -> 26.6; one row a wavefront 142, K and V by workgroups of their
 // own 158).
 struct ReadArgs {
   const int32_t* lens;
@@ -271,10 +271,10 @@ struct Tile4 {  // a lane's share of 32 keys and their scales
 //                 A probability is the sum of three bf16 values, the upper halves of what
 //                 is left of it: all of its 24 bits, so that the product is fp32's.
 // Bound by memory while a wavefront has tiles enough: 24 sequences of 9k to 65k with 64
-// query heads (928 MB) 6.2 TB/s with the launch behind it.  Below that the start counts
-// (four dependent loads from the lengths to the first row, some 5 us) and the second launch
-// (6 us): 131k positions with weights (143 MB) 33.4 us, of which the kernel 29.5; at D = 64
-// the vector units are busy 64% of the time (48 windows of 4096, 69 MB: 26 us).
+// query heads (798 MB) 155 us, 5.1 TB/s with the launch behind it.  Below that the start
+// counts (four dependent loads from the lengths to the first row, some 5 us) and the second
+// launch (4.5 us): 131k positions with weights (143 MB) 33.1 us, of which the kernel 29.5; at
+// D = 64 the vector units are busy 66% of the time (48 windows of 4096, 62 MB: 26 us).
 // The next tile's loads are under way while one is worked on: a tile has a quarter of the
 // bytes of 16-bit rows and as many instructions (131k positions 46.6 -> 32.8 us).  Two
 // tiles ahead 31.4 us for 30.3 at D = 64, spilling elsewhere.  WIDE at D = 256 has no
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(kAttnThreads, attn4_waves(D, WIDE)) void paged_attn
     n_list = min(max(a.kv_num[static_cast<int64_t>(p.b) * c.Hkv + hk], 0), a.maxkv);
     piece_range(0, static_cast<int>(s.tiles_cap), p.n, p.i, &p.t0, &p.t1);
   } else {
-    const auto wanted = [&](int64_t total) { return min(s.pieces, pieces_wanted4(total, cols, c.B, 256 * attn4_waves(D, WIDE))); };
+    const auto wanted = [&](int64_t total) { return min(s.pieces, pieces_wanted4(total, cols, c.B, kUnits * attn4_waves(D, WIDE))); };
     if (!find_piece(c, a, slot, piece_turn(D), wanted, p)) return;
   }
   p.b = same(p.b);

@@ -40,15 +40,19 @@ constexpr int kMostPieces = 1536;
 SCOPE_HD int pieces_wanted(int B, int D) { return B == 1 || D == 256 ? 1024 : kMostPieces; }
 SCOPE_HD int piece_turn(int D) { return D == 256 ? kAttnWaves : 1; }
 
+// compute units of the whole card (on a part of it fewer workgroups start together, no more)
+constexpr int kUnits = 256;
+
 // Pieces aimed at over 4-bit pages, for a batch of `total` tiles in each of `cols`
 // columns (key head and group of 16 query heads), where the device holds `resident`
-// workgroups at once.  A tile takes a quarter of the time that it takes in 16 bits, so a
-// workgroup's start counts: they start together (a sequence adds one piece at most to
-// those aimed at), and are more than 512 only where they have some ten tiles each (16
-// sequences at D = 256 47.1 us with 512 whatever the batch, this way 43.1; 20000 positions
-// 21.9 with 1024, 16.2; 64 sequences to 4k 23.9 with 1536, 19.0; 8 to 60k at D = 64 62.3
-// with 1024, 56.2).  Pieces of more than 120 tiles are cut, that their ends are even (24
-// sequences of 9k to 65k 165 -> 162).
+// workgroups at once.  A tile takes half of the time that it takes in 16 bits at D = 64, a
+// third at 128 and 256 (16 sequences of 8k to 32k, one head a key head: 28 us for 56, 35 for
+// 102, 70 for 209), so a workgroup's start counts: they start together (a sequence adds one
+// piece at most to those aimed at), and are more than 512 only where they have some ten
+// tiles each (16 sequences at D = 256 47.1 us with 512 whatever the batch, this way 43.1;
+// 20000 positions 21.9 with 1024, 16.2; 64 sequences to 4k 23.9 with 1536, 19.0; 8 to 60k at
+// D = 64 62.3 with 1024, 56.2).  Pieces of more than 120 tiles are cut, that their ends are
+// even (24 sequences of 9k to 65k 165 -> 162).  512, ten and 120 were chosen on these batches.
 SCOPE_HD int pieces_wanted4(int64_t total, int cols, int B, int resident) {
   const int all = resident / cols, less = B > 1 ? all - B : all, one = less > all / 2 ? less : all / 2;
   const int64_t few = 512 / cols, by_tiles = total / 10, some = few > by_tiles ? few : by_tiles;
