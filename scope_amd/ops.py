@@ -1157,10 +1157,6 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError(f"{ctx.who} is not differentiable: detach its inputs or its results")
 
 
-def _wants_grad(t: torch.Tensor | None) -> bool:
-    return t is not None and t.requires_grad
-
-
 def _sat32(x: torch.Tensor) -> torch.Tensor:
     """Integers as contiguous int32; those past 32 bits as the nearest one, on the
     same side of every length and index."""
@@ -1262,7 +1258,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     c = _paged_cache(who, k_pages, v_pages, table, dtype, k_scale, v_scale)
     if len(shape) != 3 or shape != v.shape or v.dtype != dtype or shape[1] != c.Hkv or shape[2] != c.D or ks[2] != 1 or vs[2] != 1:
         raise RuntimeError(f"{who}: k and v must be [N, {c.Hkv}, {c.D}] of one type with a contiguous last dimension")
-    scales = _paged_scales(who, c, k_scale, v_scale) if k_pages.dtype == _FP4 else None
+    scales = _paged_scales(who, c, k_scale, v_scale) if k_scale is not None and k_pages.dtype == _FP4 else None
     if not (c.k_sp and c.k_sh and c.k_sr and c.v_sp and c.v_sh and c.v_sr) or (
             scales and not (scales.k_sp and scales.k_sh and scales.v_sp and scales.v_sh)):
         for t in (k_pages, v_pages, k_scale, v_scale) if scales else (k_pages, v_pages):
@@ -1295,10 +1291,12 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     pages are read in their own type (the default then), others in bfloat16 by
     default.  4-bit values are exact in bfloat16 but for those of 2^128 and more
     (under scales that no append writes), which are infinite there, as in float16
-    what it does not hold; e4m3 ones are the fp32 product with their scale, rounded.  Nothing of it waits for the GPU.  It has no backward: a
-    gradient that reaches its results raises."""
+    what it does not hold; e4m3 ones are the fp32 product with their scale, rounded.
+    Nothing of it waits for the GPU.  It has no backward: a gradient that reaches
+    its results raises."""
     who = "paged_read"
-    if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad or _wants_grad(k_scale) or _wants_grad(v_scale)):
+    if torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad or (k_scale is not None and k_scale.requires_grad)
+                                    or (v_scale is not None and v_scale.requires_grad)):
         return _NoGradient.apply(who, functools.partial(paged_read, k_pages, v_pages, table, lens, rows=rows, cu=cu, first=first,
                                                         k_scale=k_scale, v_scale=v_scale, dtype=dtype), k_pages, v_pages, k_scale, v_scale)
     dev = _device(who, k_pages, v_pages, table, lens, cu, first if isinstance(first, torch.Tensor) else None, k_scale, v_scale)
@@ -1351,8 +1349,8 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     can be captured and replayed while the lengths and the table change.  It has
     no backward: a gradient that reaches its results raises."""
     who = "paged_decode_attn"
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad or _wants_grad(k_scale)
-                                    or _wants_grad(v_scale)):
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+                                    or (k_scale is not None and k_scale.requires_grad) or (v_scale is not None and v_scale.requires_grad)):
         return _NoGradient.apply(who, functools.partial(paged_decode_attn, q, k_pages, v_pages, table, lens, scale=scale, first=first,
                                                         kv_num=kv_num, kv_idx=kv_idx, mass=mass, k_scale=k_scale, v_scale=v_scale),
                                  q, k_pages, v_pages, k_scale, v_scale)
@@ -1367,18 +1365,19 @@ def paged_decode_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     if kv_num is not None or kv_idx is not None:
         if kv_num is None or kv_idx is None:
             raise RuntimeError(f"{who}: kv_num and kv_idx come together")
-        if kv_idx.dim() != 3 or not 1 <= kv_idx.shape[2] <= _INT_MAX or kv_idx.shape[:2] != (B, Hkv) or kv_num.shape != (B, Hkv):
+        listed = kv_idx.shape
+        if len(listed) != 3 or not 1 <= listed[2] <= _INT_MAX or listed[:2] != (B, Hkv) or kv_num.shape != (B, Hkv):
             raise RuntimeError(f"{who}: kv_num must be [{B}, {Hkv}] and kv_idx [{B}, {Hkv}, maxkv]")
         if kv_num.is_floating_point() or kv_idx.is_floating_point():
             raise RuntimeError(f"{who}: kv_num and kv_idx must be integers (got {kv_num.dtype} and {kv_idx.dtype})")
-        maxkv = kv_idx.shape[2]
+        maxkv = listed[2]
         kv_num, kv_idx = _sat32(kv_num), _sat32(kv_idx)
     if mass is not None and (mass.dtype != torch.float32 or mass.shape != (B, Hkv, MP) or not mass.is_contiguous()):
         raise RuntimeError(f"{who}: mass must be a contiguous float32 [{B}, {Hkv}, {MP}]")
     lens = _ints(who, "lens", lens, B, dev)
     first = _ints(who, "first", first, B, dev)
     out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=dev)
-    lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
     need = _paged_work_bytes(query, B, Hkv, D, c.bs, MP, Hq, maxkv, mass is not None)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     args = (Hq, maxkv, float(scale), q.data_ptr(), qs[0] if B > 1 else 0, qs[1] if Hq > 1 else 0, k_pages.data_ptr(),
@@ -1457,8 +1456,8 @@ def logit_penalties(logits: torch.Tensor, tokens: torch.Tensor, lens, *, first=N
     who = "logit_penalties"
     numbers = (repetition, presence, frequency, temperature)
     floats = all([type(x) is float for x in numbers])
-    if torch.is_grad_enabled() and out is None and (logits.requires_grad or _wants_grad(bias) or (
-            not floats and any(_wants_grad(x) for x in numbers if isinstance(x, torch.Tensor)))):
+    if torch.is_grad_enabled() and out is None and (logits.requires_grad or (bias is not None and bias.requires_grad) or (
+            not floats and any(isinstance(x, torch.Tensor) and x.requires_grad for x in numbers))):
         return _NoGradient.apply(who, functools.partial(logit_penalties, logits, tokens, lens, first=first, n_prompt=n_prompt,
                                                         repetition=repetition, presence=presence, frequency=frequency,
                                                         temperature=temperature, bias=bias, mask=mask), logits, bias, *numbers)
