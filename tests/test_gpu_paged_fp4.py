@@ -11,7 +11,7 @@ import torch
 
 from oracle import paged as OP
 from tests.paged_fp4_inputs import E8M0, FP4, bounds4, cache4, check4, pages
-from tests.paged_inputs import TYPES, assert_within, cache, tables
+from tests.paged_inputs import TYPES, assert_within, cache, check_attn, tables
 from tests.test_paged_fp4 import groups
 
 pytestmark = pytest.mark.gpu
@@ -428,6 +428,16 @@ def test_attn_of_the_largest_scales(ops, G, D, name):
             assert_within("out", out, r["out"], bounds4(c["q"].dtype, D, r)[0])
         elif byte > 252:
             assert not bool(torch.isfinite(out[0, :G, group].float()).any()), byte
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attn_of_large_values_in_16_bits(ops, D):
+    """bf16 pages whose values of V are up to 2^108: 2^8 times their sum over 700 rows is below 2^128."""
+    c = cache([700, 33], Hq=4, Hkv=2, D=D, bs=32, seed=24)
+    c["v_pages"] = c["v_pages"] * 2.0 ** 106
+    seen = c["v_pages"].double().abs().amax() * 700 * 2 ** 8
+    assert seen < 2.0 ** 128
+    check_attn(ops, c, DEV, scale=0.12)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
